@@ -543,11 +543,100 @@ size_t sta_decode_workspace_bytes(const sta_decode_args* a);
 int sta_decode_forward(const sta_decode_args* a, void* workspace, size_t workspace_bytes,
                        void* stream);
 
+/* ---------------------------------------------------------------------------------------
+ * Paged key-value cache: rows of new tokens written into pages, attention of one new token per
+ * sequence over its pages, and eviction by accumulated attention weight.
+ *
+ * A cache is a pool of pages (n_pages, n_kv_heads, page_size, d) for K and for V, holding RAW
+ * (unrotated) rows like the caches of the decode entry points.  Slot j of sequence b lies in
+ * page table[b, j / page_size] at row j % page_size; a slot's number is its position.  Entries
+ * of `table` beyond a sequence's last page are not read.  A page number outside [0, n_pages)
+ * never faults: what would be read there makes the sequence's result NaN, what would be written
+ * there is dropped, and the device error word is set (sta_device_error).  Lengths are clamped to
+ * [0, table_width * page_size].  K and V rows start on 16-byte boundaries.
+ * ------------------------------------------------------------------------------------- */
+typedef struct sta_paged_cache {
+  void* k; int64_t k_stride_p; int64_t k_stride_h; int64_t k_stride_n;
+  void* v; int64_t v_stride_p; int64_t v_stride_h; int64_t v_stride_n;
+  float* weights;          /* (n_pages, n_kv_heads, page_size) accumulated attention weights, or NULL */
+  int64_t weights_stride_p; int64_t weights_stride_h;   /* page_size rows contiguous */
+  const int32_t* table;    /* (batch, table_width) */
+  int64_t table_stride;
+  const int32_t* lens;     /* (batch,) tokens each sequence holds */
+  int32_t dtype;
+  int32_t d;               /* 64 or 128 */
+  int64_t n_pages;
+  int64_t n_kv_heads;
+  int64_t page_size;       /* 1 .. 65536 */
+  int64_t batch;
+  int64_t table_width;     /* table_width * page_size below 2^31 - 64 */
+} sta_paged_cache;
+
+/* Write rows i < counts[b] of k_new / v_new (batch, n_kv_heads, n, d) to the slots lens[b] + i
+ * (counts NULL: all n), zero their weights (when the cache has them) and store the new lengths
+ * lens[b] + counts[b] in lens_out, which may be the cache's own lens.  Rows past the table's
+ * last slot are dropped (device error word). */
+typedef struct sta_paged_append_args {
+  const void* k; int64_t k_stride_b; int64_t k_stride_h; int64_t k_stride_n;
+  const void* v; int64_t v_stride_b; int64_t v_stride_h; int64_t v_stride_n;
+  int64_t n;
+  const int32_t* counts;
+  int32_t* lens_out;
+} sta_paged_append_args;
+
+int sta_paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, void* stream);
+
+/* Dense attention of the token at position lens[b] - 1 (its own row included in the cache) over
+ * all slots of its sequence; one softmax in fp32, a sequence of length 0 gives zeros.  Keys are
+ * rotated where they are read: position i * pos_scale with inv_freq and cos / sin times
+ * rope_scale, or, with chunk_size > 0, Dual Chunk Attention positions (as sta_dca_forward;
+ * chunk_size - local_window a multiple of 64, pos_scale 1).  Angles are formed in 64 bits.
+ * With weights_out (laid out like the cache's weights, possibly the same array) slot j of kv
+ * head h gets weights[j] + the sum over h's q heads of the attention weight of j; other slots
+ * are left as they were, and pages must not be shared between sequences then. */
+typedef struct sta_paged_decode_args {
+  const void* q; int64_t q_stride_b; int64_t q_stride_h;   /* (batch, n_heads, d) */
+  void* out;               /* (batch, n_heads, d) contiguous, dtype */
+  int64_t n_heads;
+  const float* inv_freq;   /* (d/2,) */
+  double pos_scale;
+  float rope_scale;
+  float sm_scale;
+  int32_t chunk_size;      /* 0 = plain positions */
+  int32_t local_window;
+  float* weights_out;      /* or NULL */
+} sta_paged_decode_args;
+
+size_t sta_paged_decode_workspace_bytes(const sta_paged_cache* c, const sta_paged_decode_args* a);
+int sta_paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void* workspace,
+                     size_t workspace_bytes, void* stream);
+
+/* Keep min(lens[b], budget) slots of every sequence and kv head: the first n_global, the last
+ * n_local, and of the others those with the largest weight (ties: lowest slot; NaN counts as
+ * the smallest).  Kept rows of K, V and weights are copied in order into the pages of table_out
+ * (none of which may hold rows of the input), so a kept key's rank is its slot and position
+ * there; kept receives the original slots (-1 beyond), lens_out the new lengths.
+ * n_global + n_local <= budget. */
+typedef struct sta_paged_evict_args {
+  int64_t budget;
+  int64_t n_global;
+  int64_t n_local;
+  const int32_t* table_out; int64_t table_out_stride; int64_t table_out_width;
+  int32_t* kept;           /* (batch, n_kv_heads, budget) */
+  int32_t* lens_out;       /* (batch,), not the cache's lens */
+} sta_paged_evict_args;
+
+size_t sta_paged_evict_workspace_bytes(const sta_paged_cache* c, const sta_paged_evict_args* a);
+int sta_paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
 /* Error word of the bounded device waits on the current device (0 = none; 101-104 name the
  * wait of the selection kernel that expired).  Kernels report an expired wait only through
  * this word -- the launching call has already returned STA_OK -- so a C caller that needs to
  * know polls it after the stream's work: it synchronises `stream`, stores the word in
- * *code_out, clears it, and returns STA_ERR_TIMEOUT when it was set. */
+ * *code_out, clears it, and returns STA_ERR_TIMEOUT when it was set.  Codes 201-203 come from
+ * the paged cache (append, decode, evict): a page number outside the pool, or rows past the
+ * table's last slot; the call then returns STA_ERR_ARG. */
 int sta_device_error(void* stream, int32_t* code_out);
 
 #ifdef __cplusplus

@@ -624,6 +624,28 @@ int sta_decode_forward(const sta_decode_args* a, void* workspace, size_t workspa
   return decode_forward(a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
+int sta_paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, void* stream) {
+  return paged_append(c, a, static_cast<cudaStream_t>(stream));
+}
+
+size_t sta_paged_decode_workspace_bytes(const sta_paged_cache* c, const sta_paged_decode_args* a) {
+  return paged_decode_workspace_bytes(c, a);
+}
+
+int sta_paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void* workspace,
+                     size_t workspace_bytes, void* stream) {
+  return paged_decode(c, a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+size_t sta_paged_evict_workspace_bytes(const sta_paged_cache* c, const sta_paged_evict_args* a) {
+  return paged_evict_workspace_bytes(c, a);
+}
+
+int sta_paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+  return paged_evict(c, a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
 int sta_device_error(void* stream, int32_t* code_out) {
   int* p = device_error_word();
   if (!p) return fail(STA_ERR_CUDA, "sta_device_error: symbol lookup failed");
@@ -638,6 +660,8 @@ int sta_device_error(void* stream, int32_t* code_out) {
     cudaMemcpyAsync(p, &zero, sizeof(int), cudaMemcpyHostToDevice, st);
     cudaStreamSynchronize(st);
   }
+  if (host >= 201)
+    return fail(STA_ERR_ARG, "a paged cache named a page outside its pool or had no slot for a row");
   return host != 0 ? fail(STA_ERR_TIMEOUT, "a bounded device wait expired") : STA_OK;
 }
 

@@ -1,0 +1,80 @@
+// The paged key-value cache on the device: slot -> page lookup and the argument checks that the
+// append, decode and evict kernels share.
+#pragma once
+
+#include "common.cuh"
+#include "sta_internal.h"
+
+namespace sta {
+
+enum : int { kErrPageAppend = 201, kErrPageDecode = 202, kErrPageEvict = 203 };
+
+struct PagedView {
+  char* k;
+  char* v;
+  int64_t ksp, ksh, ksn, vsp, vsh, vsn;  // bytes
+  float* w;
+  int64_t wsp, wsh;                      // elements
+  const int32_t* table;
+  int64_t ts;
+  const int32_t* lens;
+  int64_t n_pages;
+  uint32_t page, cap;                    // page size, slots that a table row can name
+  int B, Hkv;
+};
+
+inline PagedView paged_view(const sta_paged_cache* c) {
+  const int64_t es = c->dtype == STA_DTYPE_F32 ? 4 : 2;
+  PagedView v;
+  v.k = static_cast<char*>(c->k);
+  v.v = static_cast<char*>(c->v);
+  v.ksp = c->k_stride_p * es; v.ksh = c->k_stride_h * es; v.ksn = c->k_stride_n * es;
+  v.vsp = c->v_stride_p * es; v.vsh = c->v_stride_h * es; v.vsn = c->v_stride_n * es;
+  v.w = c->weights; v.wsp = c->weights_stride_p; v.wsh = c->weights_stride_h;
+  v.table = c->table; v.ts = c->table_stride;
+  v.lens = c->lens;
+  v.n_pages = c->n_pages;
+  v.page = (uint32_t)c->page_size;
+  v.cap = (uint32_t)(c->table_width * c->page_size);
+  v.B = (int)c->batch;
+  v.Hkv = (int)c->n_kv_heads;
+  return v;
+}
+
+__device__ __forceinline__ int paged_len(const PagedView& c, int b) {
+  const int n = c.lens[b];  // (an append may store the new length in place: not a read-only load)
+  return n < 0 ? 0 : ((uint32_t)n > c.cap ? (int)c.cap : n);
+}
+
+// page number of slot j (j < cap) of sequence b, -1 where it lies outside the pool
+__device__ __forceinline__ int64_t paged_page(const PagedView& c, const int32_t* table, int64_t ts,
+                                              int b, uint32_t t) {
+  const int64_t pg = __ldg(table + b * ts + t);
+  return pg >= 0 && pg < c.n_pages ? pg : -1;
+}
+
+inline int paged_check(const sta_paged_cache* c) {
+  if (!c || !c->k || !c->v || !c->table || !c->lens)
+    return fail(STA_ERR_ARG, "sta_paged: null pointer");
+  if (c->d != 64 && c->d != 128) return fail(STA_ERR_UNSUPPORTED, "sta_paged: d must be 64 or 128");
+  if (c->dtype != STA_DTYPE_F32 && c->dtype != STA_DTYPE_BF16)
+    return fail(STA_ERR_UNSUPPORTED, "sta_paged: dtype must be f32 or bf16");
+  if (c->n_pages <= 0 || c->n_kv_heads <= 0 || c->batch < 0 || c->table_width <= 0)
+    return fail(STA_ERR_ARG, "sta_paged: bad sizes");
+  if (c->page_size < 1 || c->page_size > 65536)
+    return fail(STA_ERR_UNSUPPORTED, "sta_paged: page_size must lie in 1 .. 65536");
+  if (c->table_width >= ((int64_t)1 << 31) || c->table_width * c->page_size > ((int64_t)1 << 31) - 65)
+    return fail(STA_ERR_UNSUPPORTED, "sta_paged: table_width * page_size must stay below 2^31 - 64");
+  if (c->n_kv_heads > 65535 || c->batch > ((int64_t)1 << 24))
+    return fail(STA_ERR_UNSUPPORTED, "sta_paged: too many kv heads / sequences");
+  const int64_t es = c->dtype == STA_DTYPE_F32 ? 4 : 2;
+  const int64_t strides[6] = {c->k_stride_p, c->k_stride_h, c->k_stride_n,
+                              c->v_stride_p, c->v_stride_h, c->v_stride_n};
+  for (int64_t s : strides)
+    if (s * es % 16) return fail(STA_ERR_ARG, "sta_paged: K / V strides must be multiples of 16 bytes");
+  if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15u)
+    return fail(STA_ERR_ARG, "sta_paged: K / V must start on a 16-byte boundary");
+  return STA_OK;
+}
+
+}  // namespace sta

@@ -1,0 +1,150 @@
+// Rows of new tokens into the pages of their sequences.
+//
+// A pure copy: every row is read once and written once (2 * d * element size bytes each for K
+// and V), so HBM bounds it for prompts and launch latency for single tokens.  One thread moves
+// kIter 16-byte chunks whose loads are all in flight before the first store; chunks of a row lie
+// in neighbouring threads, kv heads of a token in neighbouring rows (the order in which a
+// projection leaves them).  Sources that are not 16-byte aligned take element loads.
+#include "paged.cuh"
+
+namespace sta {
+
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kIter = 4;
+
+struct AppP {
+  PagedView c;
+  const char* k;
+  const char* v;
+  int64_t ksb, ksh, ksn, vsb, vsh, vsn;  // bytes
+  uint32_t n;
+  const int32_t* counts;
+  int32_t* lens_out;
+  int store_lens;  // the first block of a sequence stores its new length
+  int es;
+  int* err;
+};
+
+__device__ __forceinline__ int new_len(const AppP& p, int b, int len, int& cnt) {
+  cnt = (int)p.n;
+  if (p.counts) cnt = min(max(__ldg(p.counts + b), 0), (int)p.n);
+  return (uint32_t)len + (uint32_t)cnt > p.c.cap ? (int)p.c.cap : len + cnt;
+}
+
+template <bool VEC>
+__device__ __forceinline__ uint4 load_chunk(const char* s, int es) {
+  if (VEC) return *reinterpret_cast<const uint4*>(s);
+  uint4 u;
+  if (es == 4) {
+    const uint32_t* e = reinterpret_cast<const uint32_t*>(s);
+    u = make_uint4(e[0], e[1], e[2], e[3]);
+  } else {
+    const uint16_t* e = reinterpret_cast<const uint16_t*>(s);
+    u = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
+                   e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+  }
+  return u;
+}
+
+// CH: 16-byte chunks of a row (8, 16 or 32); a unit is the K and V row of one (token, kv head).
+template <int CH, bool VEC>
+__global__ void __launch_bounds__(kThreads) paged_append_kernel(const AppP p) {
+  constexpr int UNITS = kThreads / (2 * CH);  // units that one pass of the block moves
+  const int tid = threadIdx.x;
+  const int ch = tid % CH, is_v = (tid / CH) & 1, sub = tid / (2 * CH);
+  for (int b = blockIdx.y; b < p.c.B; b += gridDim.y) {
+    const int len = paged_len(p.c, b);
+    int cnt;
+    const int total = new_len(p, b, len, cnt);
+    const int64_t units = (int64_t)cnt * p.c.Hkv;
+    const int64_t u0 = (int64_t)blockIdx.x * (UNITS * kIter) + sub;
+    uint4 x[kIter];
+    char* dst[kIter];
+#pragma unroll
+    for (int i = 0; i < kIter; ++i) {
+      const int64_t u = u0 + i * UNITS;
+      dst[i] = nullptr;
+      if (u >= units) continue;
+      const uint32_t r = (uint32_t)(u / p.c.Hkv), h = (uint32_t)(u - (int64_t)r * p.c.Hkv);
+      const uint32_t j = (uint32_t)len + r;
+      const uint32_t t = j / p.c.page;
+      const int64_t pg = j < p.c.cap ? paged_page(p.c, p.c.table, p.c.ts, b, t) : -1;
+      if (pg < 0) {
+        if (ch == 0) atomicCAS(p.err, 0, kErrPageAppend);
+        continue;
+      }
+      const uint32_t slot = j - t * p.c.page;
+      const char* s = is_v ? p.v + b * p.vsb + h * p.vsh + r * p.vsn
+                           : p.k + b * p.ksb + h * p.ksh + r * p.ksn;
+      dst[i] = (is_v ? p.c.v + pg * p.c.vsp + h * p.c.vsh + slot * p.c.vsn
+                     : p.c.k + pg * p.c.ksp + h * p.c.ksh + slot * p.c.ksn) + ch * 16;
+      x[i] = load_chunk<VEC>(s + ch * 16, p.es);
+      if (p.c.w && ch == 0 && is_v) p.c.w[pg * p.c.wsp + h * p.c.wsh + slot] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < kIter; ++i)
+      if (dst[i]) *reinterpret_cast<uint4*>(dst[i]) = x[i];
+    if (p.store_lens && blockIdx.x == 0) {
+      __syncthreads();  // lens_out may be lens: every thread of the (then only) block has read it
+      if (tid == 0) p.lens_out[b] = total;
+    }
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) paged_lens_kernel(const AppP p) {
+  const int b = blockIdx.x * kThreads + threadIdx.x;
+  if (b >= p.c.B) return;
+  int cnt;
+  p.lens_out[b] = new_len(p, b, paged_len(p.c, b), cnt);
+}
+
+template <int CH>
+void launch(const AppP& p, bool vec, dim3 grid, cudaStream_t st) {
+  if (vec) paged_append_kernel<CH, true><<<grid, kThreads, 0, st>>>(p);
+  else paged_append_kernel<CH, false><<<grid, kThreads, 0, st>>>(p);
+}
+
+}  // namespace
+
+int paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, cudaStream_t st) {
+  const int rc = paged_check(c);
+  if (rc != STA_OK) return rc;
+  if (!a || !a->lens_out) return fail(STA_ERR_ARG, "sta_paged_append: null pointer");
+  if (a->n < 0 || a->n > ((int64_t)1 << 31) - 65) return fail(STA_ERR_ARG, "sta_paged_append: bad n");
+  if (a->n > 0 && (!a->k || !a->v)) return fail(STA_ERR_ARG, "sta_paged_append: null pointer");
+  if (a->lens_out != c->lens && a->lens_out < c->lens + c->batch && c->lens < a->lens_out + c->batch)
+    return fail(STA_ERR_ARG, "sta_paged_append: lens_out overlaps lens without being it");
+  if (c->batch == 0) return STA_OK;
+  AppP p;
+  p.c = paged_view(c);
+  p.es = c->dtype == STA_DTYPE_F32 ? 4 : 2;
+  p.k = static_cast<const char*>(a->k);
+  p.v = static_cast<const char*>(a->v);
+  p.ksb = a->k_stride_b * p.es; p.ksh = a->k_stride_h * p.es; p.ksn = a->k_stride_n * p.es;
+  p.vsb = a->v_stride_b * p.es; p.vsh = a->v_stride_h * p.es; p.vsn = a->v_stride_n * p.es;
+  p.n = (uint32_t)a->n;
+  p.counts = a->counts;
+  p.lens_out = a->lens_out;
+  p.err = device_error_word();
+  if (!p.err) return fail(STA_ERR_CUDA, "sta_paged_append: no device");
+  const bool vec = ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | p.ksb |
+                     p.ksh | p.ksn | p.vsb | p.vsh | p.vsn) & 15) == 0;
+  const int ch = c->d * p.es / 16;
+  const int64_t per_block = (int64_t)kThreads / (2 * ch) * kIter;
+  const int64_t gx = (a->n * c->n_kv_heads + per_block - 1) / per_block;
+  if (gx > ((int64_t)1 << 31) - 1) return fail(STA_ERR_UNSUPPORTED, "sta_paged_append: too many rows");
+  const dim3 grid((unsigned)(gx > 0 ? gx : 1), (unsigned)(c->batch < 65535 ? c->batch : 65535));
+  // a length that is overwritten in place is read by one block only, or stored by a second launch
+  p.store_lens = a->lens_out != c->lens || grid.x == 1;
+  if (ch == 8) launch<8>(p, vec, grid, st);
+  else if (ch == 16) launch<16>(p, vec, grid, st);
+  else launch<32>(p, vec, grid, st);
+  if (!p.store_lens)
+    paged_lens_kernel<<<(unsigned)((c->batch + kThreads - 1) / kThreads), kThreads, 0, st>>>(p);
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? STA_OK : fail(STA_ERR_CUDA, cudaGetErrorString(e));
+}
+
+}  // namespace sta

@@ -1,0 +1,676 @@
+// Dense attention of one new token per sequence over a paged cache of raw keys.
+//
+//   s_j = scale * (R(p_i) q) . (R(p_j) k_j)     p = softmax(s)     out = sum_j p_j v_j
+//
+// Split over the length: the 64-key tiles of all (sequence, kv head, q-head group) segments form
+// one list, cut into equal shares for a fixed number of CTAs, so that ragged batches and single
+// long sequences load the whole GPU alike without the host knowing a length.  A CTA walks its
+// share with an online softmax per segment; a segment that lies inside one share is finished
+// there, others leave (max, sum, unnormalised output) partials that a second launch joins.
+//
+// Rotation: within a tile p_j = p_0 + t * pos_scale with t = 0 .. 63, and only differences of
+// positions matter, so keys are rotated by the tile-local t * pos_scale (one 64 x d/2 table for
+// the whole call) and the query once per tile by p_i - p_0 (64-bit angles).  Dual Chunk
+// Attention positions fit the same scheme: a tile lies in one chunk, whose relation to the
+// query's chunk sets p_i.
+//
+// Each key and value row is read from HBM once: the read of the cache bounds the call.
+#include <float.h>
+
+#include <type_traits>
+
+#include "paged.cuh"
+
+namespace sta {
+
+namespace {
+
+constexpr int kTile = 64;      // keys per tile
+constexpr int kThreads = 128;  // 4 warps, 16 keys of a tile each
+constexpr int kWarps = kThreads / 32;
+
+struct PDecP {
+  PagedView c;
+  const void* q;
+  int64_t qsb, qsh;  // elements
+  void* out;
+  int H, G, NG, GT;  // q heads, per kv head, groups of GT of them
+  const float* inv_freq;
+  double pos_scale;
+  float qscale;      // sm_scale * rope_scale^2 * log2(e): scores are in units of log2
+  int L, s;          // Dual Chunk Attention: chunk length and chunk size, L = 0 for plain positions
+  float* part;       // (2 * W, GT, D + 2): unnormalised output, max, sum
+  float* ml;         // (B, H, 2): final max and 1 / sum
+  float* scores;     // (B, Hkv * NG, capacity tiles, GT, 64) or null
+  int64_t cap_tiles;
+  float* w_out;
+  int* err;
+};
+
+__device__ __forceinline__ int n_tiles(int len) { return (len + kTile - 1) / kTile; }
+
+// A CTA's place in the list of tiles.
+struct Place {
+  int b, hg, n, tiles, len;
+};
+
+__device__ __forceinline__ void seek_sequence(const PagedView& c, Place& a) {
+  a.tiles = 0;
+  while (a.b < c.B) {
+    a.len = paged_len(c, a.b);
+    a.tiles = n_tiles(a.len);
+    if (a.tiles > 0) return;
+    ++a.b;
+  }
+}
+
+__device__ __forceinline__ void step(const PDecP& p, Place& a) {
+  if (++a.n < a.tiles) return;
+  a.n = 0;
+  if (++a.hg < p.c.Hkv * p.NG) return;
+  a.hg = 0;
+  ++a.b;
+  seek_sequence(p.c, a);
+}
+
+// Number of tiles of all segments (block-wide, NT threads), and with `find` >= 0 the place of
+// tile `find`; `before` receives the tiles of the sequences before sequence `until`.
+template <int NT>
+__device__ int64_t scan_lengths(const PDecP& p, int until, int64_t* before) {
+  __shared__ int64_t s_all[NT / 32], s_bef[NT / 32];
+  const int tid = threadIdx.x;
+  int64_t all = 0, bef = 0;
+  for (int b = tid; b < p.c.B; b += NT) {
+    const int t = n_tiles(paged_len(p.c, b));
+    all += t;
+    if (b < until) bef += t;
+  }
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffffu, all, o);
+    bef += __shfl_xor_sync(0xffffffffu, bef, o);
+  }
+  if ((tid & 31) == 0) {
+    s_all[tid >> 5] = all;
+    s_bef[tid >> 5] = bef;
+  }
+  __syncthreads();
+  all = bef = 0;
+#pragma unroll
+  for (int i = 0; i < NT / 32; ++i) {
+    all += s_all[i];
+    bef += s_bef[i];
+  }
+  __syncthreads();
+  const int64_t hg = (int64_t)p.c.Hkv * p.NG;
+  if (before) *before = bef * hg;
+  return all * hg;
+}
+
+template <int NT>
+__device__ Place find_tile(const PDecP& p, int64_t t) {
+  __shared__ int s_b, s_hit;
+  __shared__ int64_t s_rest, s_sum[NT / 32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t hg = (int64_t)p.c.Hkv * p.NG;
+  int64_t base = 0;
+  Place a{};
+  if (tid == 0) s_hit = 0;
+  __syncthreads();
+  for (int b0 = 0; b0 < p.c.B; b0 += NT) {
+    const int b = b0 + tid;
+    const int64_t mine = b < p.c.B ? (int64_t)n_tiles(paged_len(p.c, b)) * hg : 0;
+    int64_t inc = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+      if (lane >= o) inc += y;
+    }
+    if (lane == 31) s_sum[warp] = inc;
+    __syncthreads();
+    int64_t off = base, tot = 0;
+#pragma unroll
+    for (int i = 0; i < NT / 32; ++i) {
+      if (i < warp) off += s_sum[i];
+      tot += s_sum[i];
+    }
+    const int64_t lo = off + inc - mine;
+    if (mine > 0 && t >= lo && t < lo + mine) {
+      s_b = b;
+      s_rest = t - lo;
+      s_hit = 1;
+    }
+    __syncthreads();
+    if (s_hit) break;
+    base += tot;
+  }
+  a.b = s_b;
+  a.len = paged_len(p.c, a.b);
+  a.tiles = n_tiles(a.len);
+  a.hg = (int)(s_rest / a.tiles);
+  a.n = (int)(s_rest - (int64_t)a.hg * a.tiles);
+  return a;
+}
+
+// cos / sin of pos * inv_freq: the angle in turns is formed and reduced in 64 bits
+__device__ __forceinline__ void turn(double pos, float inv_freq, float& c, float& s) {
+  const double x = pos * ((double)inv_freq * 0.15915494309189533577);  // 1 / (2 pi)
+  sincospif((float)(2.0 * (x - rint(x))), &s, &c);
+}
+
+// p_i - p_0 of a tile (position of the query minus that of the tile's first key)
+__device__ __forceinline__ double query_offset(const PDecP& p, const Place& a) {
+  const int i = a.len - 1, j0 = a.n * kTile;
+  if (p.L == 0) return (double)i * p.pos_scale - (double)j0 * p.pos_scale;
+  const int away = i / p.L - j0 / p.L, in = i % p.L;
+  const int qp = away == 0 ? in : (away == 1 ? min(p.L + in, p.s) : min(2 * p.L - 1, p.s));
+  return (double)(qp - j0 % p.L);
+}
+
+template <typename TV>
+__device__ __forceinline__ float to_f(TV x);
+template <>
+__device__ __forceinline__ float to_f<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
+
+__device__ __forceinline__ void store_out(float* o, float x) { *o = x; }
+__device__ __forceinline__ void store_out(__nv_bfloat16* o, float x) { *o = __float2bfloat16_rn(x); }
+
+// Sums of NV values (a power of two up to 32) over the warp: lane l returns the sum of value
+// l / (32 / NV).  Each round halves the values a lane carries, so NV = 32 takes 31 shuffles.
+template <int NV>
+__device__ __forceinline__ float warp_reduce(float (&v)[NV]) {
+  const int lane = threadIdx.x & 31;
+  int n = NV;
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    if (n > 1) {
+      n >>= 1;
+      const bool hi = lane & o;
+#pragma unroll
+      for (int i = 0; i < NV / 2; ++i) {
+        if (i >= n) break;
+        const float send = hi ? v[i] : v[i + n];
+        const float mine = hi ? v[i + n] : v[i];
+        v[i] = mine + __shfl_xor_sync(0xffffffffu, send, o);
+      }
+    } else {
+      v[0] += __shfl_xor_sync(0xffffffffu, v[0], o);
+    }
+  }
+  return v[0];
+}
+
+template <int D, typename TV, int GT>
+struct Smem {
+  static constexpr int STAGES = sizeof(TV) == 2 ? 3 : 2;
+  static constexpr int CH = D * (int)sizeof(TV) / 16;  // 16-byte chunks of a row
+  uint4 k[STAGES][kTile * CH];
+  uint4 v[STAGES][kTile * CH];
+  float2 rot[kTile][D / 2];          // cos / sin of t * pos_scale * inv_freq
+  float q[2][GT][D];                 // rotated, scaled queries of this tile and the next
+  float p[kWarps][16][GT];           // a warp's probabilities of 16 keys
+  float acc[kWarps][GT][D];
+  float m[kWarps][GT], l[kWarps][GT];
+  int64_t koff[2][kTile], voff[2][kTile];
+};
+
+template <int D, typename TV, int GT>
+__global__ void __launch_bounds__(kThreads) paged_decode_kernel(const PDecP p) {
+  using S = Smem<D, TV, GT>;
+  constexpr int HALF = D / 2, CH = S::CH, ST = S::STAGES;
+  constexpr int FP = HALF / 32;               // frequencies of a lane
+  constexpr int KB = GT == 8 ? 4 : (GT == 4 ? 8 : 16), NV = KB * GT;  // keys of one reduction
+  constexpr int LPV = 32 / NV;                // lanes that hold the same value
+  constexpr int QH = GT * HALF / kThreads > 0 ? GT * HALF / kThreads : 1;  // q pairs of a thread
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  S& sm = *reinterpret_cast<S*>(smem_raw);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t total = scan_lengths<kThreads>(p, 0, nullptr);
+  const int64_t t0 = total * blockIdx.x / gridDim.x, t1 = total * (blockIdx.x + 1) / gridDim.x;
+  if (t0 >= t1) return;
+  const int count = (int)(t1 - t0);
+  Place cur = find_tile<kThreads>(p, t0);
+  Place qa = cur, oa = cur;  // where queries and row offsets stand
+  int q_it = 0, l_it = 0, o_it = 0;
+
+  // ---- row offsets of a tile (threads 0 .. 63), -1: no row, -2: a page outside the pool
+  auto offsets = [&]() {
+    if (o_it < count) {
+      if (tid < kTile) {
+        const int j = oa.n * kTile + tid;
+        int64_t ko = -1, vo = -1;
+        if (j < oa.len) {
+          const uint32_t t = (uint32_t)j / p.c.page;
+          const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, oa.b, t);
+          if (pg < 0) {
+            ko = -2;
+            atomicCAS(p.err, 0, kErrPageDecode);
+          } else {
+            const int64_t slot = (uint32_t)j - t * p.c.page, h = oa.hg / p.NG;
+            ko = pg * p.c.ksp + h * p.c.ksh + slot * p.c.ksn;
+            vo = pg * p.c.vsp + h * p.c.vsh + slot * p.c.vsn;
+          }
+        }
+        sm.koff[o_it & 1][tid] = ko;
+        sm.voff[o_it & 1][tid] = vo;
+      }
+      step(p, oa);
+    }
+    ++o_it;
+  };
+  // ---- copies of a tile's rows (rows without data are zero; of a bad page, K is NaN)
+  auto loads = [&]() {
+    if (l_it < count) {
+      const int st = l_it % ST;
+#pragma unroll 4
+      for (int i = tid; i < kTile * CH; i += kThreads) {
+        const int row = i / CH, ch = i % CH;
+        const int64_t ko = sm.koff[l_it & 1][row], vo = sm.voff[l_it & 1][row];
+        cp_async16(&sm.v[st][i], p.c.v + (vo >= 0 ? vo + ch * 16 : 0), vo >= 0 ? 16 : 0);
+        if (ko == -2) {
+          sm.k[st][i] = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+        } else {
+          cp_async16(&sm.k[st][i], p.c.k + (ko >= 0 ? ko + ch * 16 : 0), ko >= 0 ? 16 : 0);
+        }
+      }
+    }
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
+    ++l_it;
+  };
+  // ---- queries of a tile: rotated by p_i - p_0
+  float q1[QH], q2[QH];
+  const int qf = tid % HALF, qg = tid / HALF;  // frequency, first head (step kThreads / HALF)
+  auto queries = [&]() {
+    if (q_it < count) {
+      if (q_it == 0 || qa.n == 0) {
+        const int h0 = (qa.hg / p.NG) * p.G + (qa.hg % p.NG) * GT;
+#pragma unroll
+        for (int i = 0; i < QH; ++i) {
+          const int g = qg + i * (kThreads / HALF);
+          const bool in = g < GT && (qa.hg % p.NG) * GT + g < p.G;
+          const TV* src = static_cast<const TV*>(p.q) + qa.b * p.qsb + (h0 + g) * p.qsh;
+          q1[i] = in ? to_f(src[qf]) * p.qscale : 0.f;
+          q2[i] = in ? to_f(src[qf + HALF]) * p.qscale : 0.f;
+        }
+      }
+      float c, s;
+      turn(query_offset(p, qa), __ldg(p.inv_freq + qf), c, s);
+#pragma unroll
+      for (int i = 0; i < QH; ++i) {
+        const int g = qg + i * (kThreads / HALF);
+        if (g < GT) {
+          sm.q[q_it & 1][g][qf] = q1[i] * c - q2[i] * s;
+          sm.q[q_it & 1][g][qf + HALF] = q2[i] * c + q1[i] * s;
+        }
+      }
+      step(p, qa);
+    }
+    ++q_it;
+  };
+
+  for (int i = 0; i < ST - 1; ++i) {
+    offsets();
+    __syncthreads();
+    loads();
+  }
+  offsets();
+  queries();
+  for (int i = tid; i < kTile * HALF; i += kThreads) {
+    const int t = i / HALF, f = i % HALF;
+    float c, s;
+    turn((double)t * p.pos_scale, __ldg(p.inv_freq + f), c, s);
+    sm.rot[t][f] = make_float2(c, s);
+  }
+
+  float acc[GT][2 * FP];
+  float mx = -INFINITY, sum = 0.f;  // of head (lane / LPV) % GT, replicated over its lanes
+#pragma unroll
+  for (int g = 0; g < GT; ++g)
+#pragma unroll
+    for (int e = 0; e < 2 * FP; ++e) acc[g][e] = 0.f;
+
+  for (int it = 0; it < count; ++it) {
+    asm volatile("cp.async.wait_group %0;\n" ::"n"(ST - 2) : "memory");
+    __syncthreads();
+    loads();
+    const int st = it % ST;
+    const TV* ks = reinterpret_cast<const TV*>(sm.k[st]);
+    const TV* vs = reinterpret_cast<const TV*>(sm.v[st]);
+    float qr[GT][2 * FP];
+#pragma unroll
+    for (int g = 0; g < GT; ++g)
+#pragma unroll
+      for (int e = 0; e < FP; ++e) {
+        qr[g][e] = sm.q[it & 1][g][lane * FP + e];
+        qr[g][FP + e] = sm.q[it & 1][g][HALF + lane * FP + e];
+      }
+    const int valid = cur.len - cur.n * kTile;  // keys of this tile
+    float* sc = p.scores
+        ? p.scores + ((((int64_t)cur.b * p.c.Hkv * p.NG + cur.hg) * p.cap_tiles + cur.n) * GT) * kTile
+        : nullptr;
+#pragma unroll
+    for (int kb = 0; kb < 16 / KB; ++kb) {
+      const int key0 = warp * 16 + kb * KB;
+      float v[NV];
+#pragma unroll
+      for (int kk = 0; kk < KB; ++kk) {
+        const int t = key0 + kk;
+        float r1[FP], r2[FP];
+#pragma unroll
+        for (int e = 0; e < FP; ++e) {
+          const float x1 = to_f(ks[t * D + lane * FP + e]);
+          const float x2 = to_f(ks[t * D + HALF + lane * FP + e]);
+          const float2 cs = sm.rot[t][lane * FP + e];
+          r1[e] = x1 * cs.x - x2 * cs.y;
+          r2[e] = x2 * cs.x + x1 * cs.y;
+        }
+#pragma unroll
+        for (int g = 0; g < GT; ++g) {
+          float d = 0.f;
+#pragma unroll
+          for (int e = 0; e < FP; ++e) d = fmaf(qr[g][FP + e], r2[e], fmaf(qr[g][e], r1[e], d));
+          v[kk * GT + g] = d;
+        }
+      }
+      float s = warp_reduce<NV>(v);
+      const int idx = lane / LPV, kk = idx / GT, g = idx % GT;
+      if (key0 + kk >= valid) s = -INFINITY;
+      if (sc && (LPV == 1 || lane % LPV == 0)) sc[g * kTile + key0 + kk] = s;
+      float mb = s;
+#pragma unroll
+      for (int o = GT * LPV; o < 32; o <<= 1) mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
+      const float mn = fmaxf(mx, mb), ms = mn == -INFINITY ? 0.f : mn;
+      const float a = exp2f(mx - ms), e = exp2f(s - ms);
+      float se = e;
+#pragma unroll
+      for (int o = GT * LPV; o < 32; o <<= 1) se += __shfl_xor_sync(0xffffffffu, se, o);
+      sum = sum * a + se;
+      mx = mn;
+      if (LPV == 1 || lane % LPV == 0) sm.p[warp][kk][g] = e;
+#pragma unroll
+      for (int gg = 0; gg < GT; ++gg) {
+        const float ag = __shfl_sync(0xffffffffu, a, gg * LPV);
+#pragma unroll
+        for (int x = 0; x < 2 * FP; ++x) acc[gg][x] *= ag;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int k2 = 0; k2 < KB; ++k2) {
+        const int t = key0 + k2;
+        float vv[2 * FP];
+#pragma unroll
+        for (int x = 0; x < FP; ++x) {
+          vv[x] = to_f(vs[t * D + lane * FP + x]);
+          vv[FP + x] = to_f(vs[t * D + HALF + lane * FP + x]);
+        }
+#pragma unroll
+        for (int gg = 0; gg < GT; ++gg) {
+          const float pr = sm.p[warp][k2][gg];
+#pragma unroll
+          for (int x = 0; x < 2 * FP; ++x) acc[gg][x] = fmaf(pr, vv[x], acc[gg][x]);
+        }
+      }
+      __syncwarp();
+    }
+    const bool seg_end = cur.n == cur.tiles - 1;
+    if (seg_end || it == count - 1) {
+      // the warps' partial results of this segment, joined and stored
+      const int idx = lane / LPV;
+      if (idx < GT && lane % LPV == 0) {
+        sm.m[warp][idx] = mx;
+        sm.l[warp][idx] = sum;
+      }
+#pragma unroll
+      for (int g = 0; g < GT; ++g)
+#pragma unroll
+        for (int x = 0; x < FP; ++x) {
+          sm.acc[warp][g][lane * FP + x] = acc[g][x];
+          sm.acc[warp][g][HALF + lane * FP + x] = acc[g][FP + x];
+        }
+      __syncthreads();
+      const bool started = cur.n <= it;  // the segment's first tile lies in this share
+      const bool whole = seg_end && started;
+      const int slot = 2 * blockIdx.x + (started ? 1 : 0);
+      const int h0 = (cur.hg / p.NG) * p.G + (cur.hg % p.NG) * GT;
+      for (int i = tid; i < GT * D; i += kThreads) {
+        const int g = i / D, d = i % D;
+        if ((cur.hg % p.NG) * GT + g >= p.G) continue;
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.m[w][g]);
+        const float ms = M == -INFINITY ? 0.f : M;
+        float L = 0.f, o = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float f = exp2f(sm.m[w][g] - ms);
+          L += sm.l[w][g] * f;
+          o += sm.acc[w][g][d] * f;
+        }
+        if (whole) {
+          store_out(static_cast<TV*>(p.out) + ((int64_t)cur.b * p.H + h0 + g) * D + d, o / L);
+          if (d == 0) {
+            float* ml = p.ml + ((int64_t)cur.b * p.H + h0 + g) * 2;
+            ml[0] = ms;
+            ml[1] = 1.f / L;
+          }
+        } else {
+          float* part = p.part + ((int64_t)slot * GT + g) * (D + 2);
+          part[d] = o;
+          if (d == 0) {
+            part[D] = M;
+            part[D + 1] = L;
+          }
+        }
+      }
+#pragma unroll
+      for (int g = 0; g < GT; ++g)
+#pragma unroll
+        for (int x = 0; x < 2 * FP; ++x) acc[g][x] = 0.f;
+      mx = -INFINITY;
+      sum = 0.f;
+    }
+    offsets();
+    queries();
+    step(p, cur);
+  }
+}
+
+// One CTA per segment: joins the partials of the shares that cut it.  Empty sequences give zeros.
+template <int D, typename TV>
+__global__ void __launch_bounds__(D) paged_join_kernel(const PDecP p, int W) {
+  const int hgs = p.c.Hkv * p.NG;
+  const int b = blockIdx.x / hgs, hg = blockIdx.x % hgs, d = threadIdx.x;
+  const int h0 = (hg / p.NG) * p.G + (hg % p.NG) * p.GT, ng = min(p.GT, p.G - (hg % p.NG) * p.GT);
+  int64_t before;
+  const int64_t total = scan_lengths<D>(p, b, &before);
+  const int64_t tiles = n_tiles(paged_len(p.c, b));
+  TV* out = static_cast<TV*>(p.out) + ((int64_t)b * p.H + h0) * D;
+  if (tiles == 0) {
+    for (int g = 0; g < ng; ++g) store_out(out + g * D + d, 0.f);
+    return;
+  }
+  // the shares of this segment's first and last tile (share w holds [total w / W, total (w+1) / W))
+  const int64_t s0 = before + hg * tiles, s1 = s0 + tiles;
+  int64_t w0 = s0 * W / total, w1 = (s1 - 1) * W / total;
+  while (total * (w0 + 1) / W <= s0) ++w0;
+  while (total * (w1 + 1) / W <= s1 - 1) ++w1;
+  if (w0 == w1) return;  // finished by its share
+  for (int g = 0; g < ng; ++g) {
+    float M = -INFINITY, L = 0.f, o = 0.f;
+    for (int64_t w = w0; w <= w1; ++w) {
+      const int64_t slot = 2 * w + (total * w / W <= s0 ? 1 : 0);
+      if (total * w / W == total * (w + 1) / W) continue;  // an empty share
+      const float* part = p.part + (slot * p.GT + g) * (D + 2);
+      const float m = part[D], l = part[D + 1], x = part[d];
+      const float mn = fmaxf(M, m), ms = mn == -INFINITY ? 0.f : mn;
+      const float a = exp2f(M - ms), e = exp2f(m - ms);
+      L = L * a + l * e;
+      o = o * a + x * e;
+      M = mn;
+    }
+    store_out(out + g * D + d, o / L);
+    if (d == 0) {
+      float* ml = p.ml + ((int64_t)b * p.H + h0 + g) * 2;
+      ml[0] = M == -INFINITY ? 0.f : M;
+      ml[1] = 1.f / L;
+    }
+  }
+}
+
+// weights_out[j] = weights[j] + sum_g exp2(s_gj - M_g) / L_g
+__global__ void __launch_bounds__(256) paged_weights_kernel(const PDecP p) {
+  const int b = blockIdx.z, h = blockIdx.y;
+  const int len = paged_len(p.c, b);
+  const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (j >= len) return;
+  const uint32_t t = (uint32_t)j / p.c.page;
+  const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
+  if (pg < 0) return;
+  float w = 0.f;
+  for (int g = 0; g < p.G; ++g) {
+    const int hg = h * p.NG + g / p.GT;
+    const float s = p.scores[((((int64_t)b * p.c.Hkv * p.NG + hg) * p.cap_tiles + j / kTile) * p.GT +
+                              g % p.GT) * kTile + j % kTile];
+    const float* ml = p.ml + ((int64_t)b * p.H + h * p.G + g) * 2;
+    w += exp2f(s - ml[0]) * ml[1];
+  }
+  const int64_t at = pg * p.c.wsp + h * p.c.wsh + ((uint32_t)j - t * p.c.page);
+  p.w_out[at] = p.c.w[at] + w;
+}
+
+struct PLayout {
+  size_t part, ml, scores, total;
+  int GT, NG, W;
+  int64_t cap_tiles;
+};
+
+inline size_t al(size_t x) { return (x + 255) & ~size_t(255); }
+
+int sm_count() {
+  static int n[64] = {0};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+  if (!n[dev]) {
+    int v = 0;
+    if (cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess) return 148;
+    n[dev] = v;
+  }
+  return n[dev];
+}
+
+PLayout layout(const sta_paged_cache* c, const sta_paged_decode_args* a) {
+  PLayout L{};
+  const int64_t G = a->n_heads / c->n_kv_heads;
+  L.GT = G > 4 ? 8 : (G > 2 ? 4 : (int)G);
+  L.NG = (int)((G + L.GT - 1) / L.GT);
+  L.cap_tiles = (c->table_width * c->page_size + kTile - 1) / kTile;
+  const int64_t most = c->batch * c->n_kv_heads * L.NG * L.cap_tiles;
+  const int64_t w = 2 * (int64_t)sm_count();
+  L.W = (int)(most < w ? most : w);
+  size_t o = 0;
+  auto take = [&](size_t bytes) {
+    const size_t r = o;
+    o += al(bytes);
+    return r;
+  };
+  L.part = take((size_t)2 * L.W * L.GT * (c->d + 2) * 4);
+  L.ml = take((size_t)c->batch * a->n_heads * 8);
+  L.scores = a->weights_out ? take((size_t)most * L.GT * kTile * 4) : 0;
+  L.total = o + 256;
+  return L;
+}
+
+int check(const sta_paged_cache* c, const sta_paged_decode_args* a) {
+  const int rc = paged_check(c);
+  if (rc != STA_OK) return rc;
+  if (!a || (c->batch > 0 && (!a->q || !a->out)) || !a->inv_freq)
+    return fail(STA_ERR_ARG, "sta_paged_decode: null pointer");
+  if (a->n_heads <= 0 || a->n_heads % c->n_kv_heads)
+    return fail(STA_ERR_ARG, "sta_paged_decode: n_heads must be a multiple of n_kv_heads");
+  if (a->chunk_size < 0 || (a->chunk_size > 0 && (a->local_window <= 0 || a->chunk_size <= a->local_window)))
+    return fail(STA_ERR_ARG, "sta_paged_decode: bad chunk_size / local_window");
+  if (a->chunk_size > 0 && (a->chunk_size - a->local_window) % kTile)
+    return fail(STA_ERR_UNSUPPORTED, "sta_paged_decode: chunk_size - local_window must be a multiple of 64");
+  if (a->chunk_size > 0 && a->pos_scale != 1.0)
+    return fail(STA_ERR_ARG, "sta_paged_decode: Dual Chunk Attention positions take pos_scale 1");
+  if (a->weights_out && !c->weights)
+    return fail(STA_ERR_ARG, "sta_paged_decode: weights_out needs a cache with weights");
+  if (a->weights_out && c->batch > 65535)
+    return fail(STA_ERR_UNSUPPORTED, "sta_paged_decode: weights take at most 65535 sequences");
+  if (c->batch * a->n_heads > ((int64_t)1 << 30))
+    return fail(STA_ERR_UNSUPPORTED, "sta_paged_decode: too many heads");
+  return STA_OK;
+}
+
+template <int D, typename TV, int GT>
+int launch(const PDecP& p, int W, cudaStream_t st) {
+  constexpr int bytes = (int)sizeof(Smem<D, TV, GT>);
+  const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<D, TV, GT>,
+                                             cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e != cudaSuccess) return fail(STA_ERR_CUDA, cudaGetErrorString(e));
+  paged_decode_kernel<D, TV, GT><<<W, kThreads, bytes, st>>>(p);
+  paged_join_kernel<D, TV><<<(unsigned)(p.c.B * p.c.Hkv * p.NG), D, 0, st>>>(p, W);
+  return STA_OK;
+}
+
+template <int D, typename TV>
+int launch_g(const PDecP& p, int W, cudaStream_t st) {
+  if (p.GT == 1) return launch<D, TV, 1>(p, W, st);
+  if (p.GT == 2) return launch<D, TV, 2>(p, W, st);
+  if (p.GT == 4) return launch<D, TV, 4>(p, W, st);
+  return launch<D, TV, 8>(p, W, st);
+}
+
+}  // namespace
+
+size_t paged_decode_workspace_bytes(const sta_paged_cache* c, const sta_paged_decode_args* a) {
+  if (check(c, a) != STA_OK) return 0;
+  return layout(c, a).total;
+}
+
+int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void* ws, size_t ws_len,
+                 cudaStream_t st) {
+  int rc = check(c, a);
+  if (rc != STA_OK) return rc;
+  if (c->batch == 0) return STA_OK;
+  const PLayout L = layout(c, a);
+  if (!ws || ws_len < L.total) return fail(STA_ERR_WORKSPACE, "sta_paged_decode: workspace too small");
+  uint8_t* w = static_cast<uint8_t*>(ws);
+  w += (256 - reinterpret_cast<uintptr_t>(w) % 256) % 256;
+  PDecP p;
+  p.c = paged_view(c);
+  p.q = a->q; p.qsb = a->q_stride_b; p.qsh = a->q_stride_h;
+  p.out = a->out;
+  p.H = (int)a->n_heads;
+  p.G = (int)(a->n_heads / c->n_kv_heads);
+  p.NG = L.NG;
+  p.GT = L.GT;
+  p.inv_freq = a->inv_freq;
+  p.pos_scale = a->pos_scale;
+  p.qscale = (float)((double)a->sm_scale * a->rope_scale * a->rope_scale * 1.4426950408889634);
+  p.L = a->chunk_size > 0 ? a->chunk_size - a->local_window : 0;
+  p.s = a->chunk_size;
+  p.part = reinterpret_cast<float*>(w + L.part);
+  p.ml = reinterpret_cast<float*>(w + L.ml);
+  p.scores = a->weights_out ? reinterpret_cast<float*>(w + L.scores) : nullptr;
+  p.cap_tiles = L.cap_tiles;
+  p.w_out = a->weights_out;
+  p.err = device_error_word();
+  if (!p.err) return fail(STA_ERR_CUDA, "sta_paged_decode: no device");
+  const bool f32 = c->dtype == STA_DTYPE_F32;
+  if (c->d == 128)
+    rc = f32 ? launch_g<128, float>(p, L.W, st) : launch_g<128, __nv_bfloat16>(p, L.W, st);
+  else
+    rc = f32 ? launch_g<64, float>(p, L.W, st) : launch_g<64, __nv_bfloat16>(p, L.W, st);
+  if (rc != STA_OK) return rc;
+  if (a->weights_out) {
+    const dim3 grid((unsigned)((p.c.cap + 255) / 256), (unsigned)p.c.Hkv, (unsigned)p.c.B);
+    paged_weights_kernel<<<grid, 256, 0, st>>>(p);
+  }
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? STA_OK : fail(STA_ERR_CUDA, cudaGetErrorString(e));
+}
+
+}  // namespace sta

@@ -37,6 +37,13 @@ int launch_gather_attend(const sta_attend_args* a, cudaStream_t stream);
 int launch_pqstream(const sta_pqstream_args* a, cudaStream_t stream);
 size_t decode_workspace_bytes(const sta_decode_args* a);
 int decode_forward(const sta_decode_args* a, void* ws, size_t ws_len, cudaStream_t stream);
+int paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, cudaStream_t stream);
+size_t paged_decode_workspace_bytes(const sta_paged_cache* c, const sta_paged_decode_args* a);
+int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void* ws, size_t ws_len,
+                 cudaStream_t stream);
+size_t paged_evict_workspace_bytes(const sta_paged_cache* c, const sta_paged_evict_args* a);
+int paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* ws, size_t ws_len,
+                cudaStream_t stream);
 
 // cuTensorMapEncodeTiled obtained through the runtime's driver entry point
 bool make_tmap_bf16_3d(CUtensorMap* map, const void* base, uint64_t d, uint64_t n,

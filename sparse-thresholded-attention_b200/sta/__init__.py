@@ -12,10 +12,12 @@ Host-side mirror of the reference repository's prefill call surfaces, backed by 
     sta.shared_selection_chunked        <- shared_selection_triton_chunked (chunk_exact)
     sta.hooks                           the HuggingFace attention hooks of every family
     sta.core                            forward / forward_host / decode and the stage calls
+    sta.paged                           the paged key-value cache: append, decode, evict
     sta.partition                       multi-GPU units (kv-head ranges, query slabs)
 """
 from . import core  # noqa: F401
 from ._lib import lib  # noqa: F401
 from .core import Geometry  # noqa: F401
+from . import paged  # noqa: F401
 
-__all__ = ["core", "lib", "Geometry"]
+__all__ = ["core", "lib", "Geometry", "paged"]

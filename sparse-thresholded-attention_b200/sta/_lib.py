@@ -139,6 +139,34 @@ class DcaArgs(ctypes.Structure):
                 ("local_window", c_i32), ("q_pos_base", c_i64)]
 
 
+class PagedCacheArgs(ctypes.Structure):
+    _fields_ = [("k", c_vp), ("k_stride_p", c_i64), ("k_stride_h", c_i64), ("k_stride_n", c_i64),
+                ("v", c_vp), ("v_stride_p", c_i64), ("v_stride_h", c_i64), ("v_stride_n", c_i64),
+                ("weights", c_vp), ("weights_stride_p", c_i64), ("weights_stride_h", c_i64),
+                ("table", c_vp), ("table_stride", c_i64), ("lens", c_vp), ("dtype", c_i32),
+                ("d", c_i32), ("n_pages", c_i64), ("n_kv_heads", c_i64), ("page_size", c_i64),
+                ("batch", c_i64), ("table_width", c_i64)]
+
+
+class PagedAppendArgs(ctypes.Structure):
+    _fields_ = [("k", c_vp), ("k_stride_b", c_i64), ("k_stride_h", c_i64), ("k_stride_n", c_i64),
+                ("v", c_vp), ("v_stride_b", c_i64), ("v_stride_h", c_i64), ("v_stride_n", c_i64),
+                ("n", c_i64), ("counts", c_vp), ("lens_out", c_vp)]
+
+
+class PagedDecodeArgs(ctypes.Structure):
+    _fields_ = [("q", c_vp), ("q_stride_b", c_i64), ("q_stride_h", c_i64), ("out", c_vp),
+                ("n_heads", c_i64), ("inv_freq", c_vp), ("pos_scale", ctypes.c_double),
+                ("rope_scale", c_f32), ("sm_scale", c_f32), ("chunk_size", c_i32),
+                ("local_window", c_i32), ("weights_out", c_vp)]
+
+
+class PagedEvictArgs(ctypes.Structure):
+    _fields_ = [("budget", c_i64), ("n_global", c_i64), ("n_local", c_i64), ("table_out", c_vp),
+                ("table_out_stride", c_i64), ("table_out_width", c_i64), ("kept", c_vp),
+                ("lens_out", c_vp)]
+
+
 # every symbol include/sta.h declares (checked by the CPU test suite)
 EXPORTED = ["sta_last_error", "sta_version", "sta_tri_head_stride", "sta_rope_split",
             "sta_select", "sta_build_sets", "sta_build_sets_pq", "sta_gather_attend",
@@ -148,7 +176,9 @@ EXPORTED = ["sta_last_error", "sta_version", "sta_tri_head_stride", "sta_rope_sp
             "sta_shared_forward_static", "sta_build_sets_chunk", "sta_chunk_workspace_bytes",
             "sta_chunk_forward", "sta_rope_split_dca", "sta_rope_table", "sta_tri_head_stride_q",
             "sta_decode_workspace_bytes", "sta_decode_forward", "sta_dca_workspace_bytes",
-            "sta_dca_forward", "sta_select_screen_bytes"]
+            "sta_dca_forward", "sta_select_screen_bytes", "sta_paged_append",
+            "sta_paged_decode_workspace_bytes", "sta_paged_decode",
+            "sta_paged_evict_workspace_bytes", "sta_paged_evict"]
 
 _lib = None
 
@@ -198,6 +228,16 @@ def lib():
     L.sta_dca_workspace_bytes.argtypes = [ctypes.POINTER(DcaArgs)]
     L.sta_dca_forward.restype = ctypes.c_int
     L.sta_dca_forward.argtypes = [ctypes.POINTER(DcaArgs), c_vp, ctypes.c_size_t, c_vp]
+    cache = ctypes.POINTER(PagedCacheArgs)
+    L.sta_paged_append.restype = ctypes.c_int
+    L.sta_paged_append.argtypes = [cache, ctypes.POINTER(PagedAppendArgs), c_vp]
+    for name, st in (("sta_paged_decode", PagedDecodeArgs), ("sta_paged_evict", PagedEvictArgs)):
+        f = getattr(L, name)
+        f.restype = ctypes.c_int
+        f.argtypes = [cache, ctypes.POINTER(st), c_vp, ctypes.c_size_t, c_vp]
+        f = getattr(L, name + "_workspace_bytes")
+        f.restype = ctypes.c_size_t
+        f.argtypes = [cache, ctypes.POINTER(st)]
     L.sta_select_screen_bytes.restype = ctypes.c_size_t
     L.sta_select_screen_bytes.argtypes = [ctypes.POINTER(SelectArgs)]
     L.sta_shared_forward_static.restype = ctypes.c_int

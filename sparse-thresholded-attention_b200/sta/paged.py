@@ -1,0 +1,185 @@
+"""The paged key-value cache: ``append`` rows of new tokens, ``decode`` one new token per
+sequence, ``evict`` the keys that attention has used least.
+
+``core.decode`` runs the thresholded rules over one contiguous cache; here a batch of sequences
+of any lengths shares a pool of fixed-size pages.  As everywhere in this package the cache holds
+RAW keys: ``decode`` rotates them where it reads them, so one cache serves every geometry
+(positions interpolated, YaRN, Dual Chunk Attention), and evicted caches are read at dense ranks
+(slot = position), like the sets of the PQ-Union rule.
+
+Every call launches on torch's current stream of the cache's device and reads the lengths on the
+device: nothing synchronises, and calls can be captured into CUDA graphs.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib as L
+from .core import Geometry, _rows, _stream, dtype_code
+
+
+def _on(t, dev, dtype, shape, name):
+    """t is a tensor of this device, type and shape (None entries: any) with a dense last dim."""
+    if not torch.is_tensor(t) or t.device != dev:
+        raise ValueError(f"{name} must be a tensor on {dev}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.dim() != len(shape) or any(n is not None and s != n for s, n in zip(t.shape, shape)):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+
+
+class PagedCache:
+    """A batch of sequences over a pool of pages.
+
+    k, v (n_pages, Hkv, page_size, D): the pool, float32 or bfloat16, D 64 or 128, any strides
+    that are multiples of 16 bytes (last dimension contiguous).  table (batch, width) int32: slot
+    j of sequence b lies in page ``table[b, j // page_size]`` at row ``j % page_size``; entries
+    past a sequence's last page are not read.  lens (batch,) int32: tokens each sequence holds.
+    weights (n_pages, Hkv, page_size) float32, optional: the attention weight that each key has
+    received so far (``decode(weights_out=...)``), which ``evict`` ranks by.
+
+    The tensors are used in place and may be written by the program between calls (new table
+    entries, new lengths); the object itself only keeps them and their addresses.  A page number
+    outside the pool never faults: its sequence's result is NaN, its rows are dropped, and
+    ``core.device_error()`` is 201 (append), 202 (decode) or 203 (evict)."""
+
+    __slots__ = ("k", "v", "table", "lens", "weights", "device", "_args", "_ref")
+
+    def __init__(self, k, v, table, lens, weights=None):
+        if not (torch.is_tensor(k) and k.is_cuda):
+            raise ValueError("the cache must hold CUDA tensors (there is no CPU path)")
+        if k.dim() != 4:
+            raise ValueError("k, v must be (n_pages, Hkv, page_size, D)")
+        dev = k.device
+        code = dtype_code(k.dtype)
+        _on(k, dev, k.dtype, k.shape, "k")
+        _on(v, dev, k.dtype, k.shape, "v")
+        _on(table, dev, torch.int32, (None, None), "table")
+        _on(lens, dev, torch.int32, (table.shape[0],), "lens")
+        n_pages, hk, page, d = k.shape
+        if weights is not None:
+            _on(weights, dev, torch.float32, (n_pages, hk, page), "weights")
+        self.k, self.v, self.table, self.lens, self.weights, self.device = k, v, table, lens, weights, dev
+        a = L.PagedCacheArgs()
+        a.k, a.k_stride_p, a.k_stride_h, a.k_stride_n = k.data_ptr(), k.stride(0), k.stride(1), k.stride(2)
+        a.v, a.v_stride_p, a.v_stride_h, a.v_stride_n = v.data_ptr(), v.stride(0), v.stride(1), v.stride(2)
+        if weights is not None:
+            a.weights, a.weights_stride_p, a.weights_stride_h = weights.data_ptr(), weights.stride(0), weights.stride(1)
+        a.table, a.table_stride, a.lens = table.data_ptr(), table.stride(0), lens.data_ptr()
+        a.dtype, a.d = code, d
+        a.n_pages, a.n_kv_heads, a.page_size = n_pages, hk, page
+        a.batch, a.table_width = table.shape
+        self._args, self._ref = a, ctypes.byref(a)
+
+    @property
+    def batch(self):
+        return self.table.shape[0]
+
+    def with_pages(self, table, lens):
+        """The same pool under other page tables / lengths."""
+        return PagedCache(self.k, self.v, table, lens, weights=self.weights)
+
+
+def append(cache: PagedCache, k, v, *, counts=None, lens_out=None):
+    """Write the first ``counts[b]`` of the rows k, v (batch, Hkv, n, D) to slots ``lens[b]`` on of
+    sequence b (counts None: all n; a decode step has n = 1), set their weights to zero, and
+    return the new lengths in ``lens_out`` (batch,) int32 (default: the cache's own ``lens``).
+    The caller has put pages for the new slots into the table; rows past its last slot are
+    dropped and reported by ``core.device_error()``."""
+    a = cache._args
+    dev = cache.device
+    shape = (a.batch, a.n_kv_heads, None, a.d)
+    k, v = _rows(k), _rows(v)
+    _on(k, dev, cache.k.dtype, shape, "k")
+    _on(v, dev, cache.k.dtype, k.shape, "v")
+    if counts is not None:
+        _on(counts, dev, torch.int32, (a.batch,), "counts")
+    if lens_out is None:
+        lens_out = cache.lens
+    else:
+        _on(lens_out, dev, torch.int32, (a.batch,), "lens_out")
+    b = L.PagedAppendArgs(k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
+                          v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), k.shape[2],
+                          None if counts is None else counts.data_ptr(), lens_out.data_ptr())
+    with torch.cuda.device(dev):
+        L.check(L.lib().sta_paged_append(cache._ref, ctypes.byref(b), _stream()), "sta_paged_append")
+    return lens_out
+
+
+def decode(q, cache: PagedCache, geometry: Geometry, *, sm_scale=None, weights_out=None):
+    """Attention of one new token per sequence, q (batch, H, D) at position ``lens[b] - 1`` (its
+    own key and value appended before), over all slots of its sequence.  ``geometry`` gives the
+    positions: ``pos_scale`` and ``rope_scale``, or ``dca`` = (chunk_size, local_window) with a
+    chunk length that is a multiple of 64.  Returns out (batch, H, D); a sequence of length 0
+    gives zeros.
+
+    With ``weights_out`` (a tensor with the shape and strides of the cache's ``weights``, or the
+    weights themselves) every slot receives its weight plus the attention weight that this token
+    gave it, summed over the q heads of its kv head; pages must not be shared between sequences
+    then."""
+    a = cache._args
+    dev = cache.device
+    _on(q, dev, cache.k.dtype, (a.batch, None, a.d), "q")
+    inv = geometry.inv_freq
+    if inv.dtype != torch.float32 or inv.device != dev or not inv.is_contiguous():
+        inv = inv.to(device=dev, dtype=torch.float32).contiguous()
+    if inv.numel() != a.d // 2:
+        raise ValueError("inv_freq must have head_dim/2 entries")
+    H = q.shape[1]
+    out = torch.empty((a.batch, H, a.d), dtype=q.dtype, device=dev)
+    b = L.PagedDecodeArgs(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), H, inv.data_ptr(),
+                          geometry.pos_scale, geometry.rope_scale,
+                          1.0 / math.sqrt(a.d) if sm_scale is None else sm_scale)
+    if geometry.dca is not None:
+        b.chunk_size, b.local_window = int(geometry.dca[0]), int(geometry.dca[1])
+        if b.chunk_size <= 0:
+            raise ValueError("dca needs a positive chunk_size")
+    if weights_out is not None:
+        if cache.weights is None:
+            raise ValueError("weights_out needs a cache with weights")
+        _on(weights_out, dev, torch.float32, cache.weights.shape, "weights_out")
+        if weights_out.stride() != cache.weights.stride():
+            raise ValueError("weights_out must have the strides of the cache's weights")
+        b.weights_out = weights_out.data_ptr()
+    lib, ref = L.lib(), ctypes.byref(b)
+    with torch.cuda.device(dev):
+        n = lib.sta_paged_decode_workspace_bytes(cache._ref, ref)
+        if n == 0:
+            L.check(1, "sta_paged_decode")
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        L.check(lib.sta_paged_decode(cache._ref, ref, ws.data_ptr(), n, _stream()), "sta_paged_decode")
+    return out
+
+
+def evict(cache: PagedCache, budget: int, table_out, *, n_global=32, n_local=32):
+    """Cut every sequence to at most ``budget`` keys per kv head: the first ``n_global``, the last
+    ``n_local``, and of the others those with the largest ``weights`` (ties: lowest slot).  The
+    kept rows of k, v and weights are copied, in order, into the pages of ``table_out`` (batch,
+    >= ceil(min(budget, slots) / page_size)) int32, which must not hold rows of the cache; the old
+    pages stay as they are (they may be shared) until the caller frees them.
+
+    Returns (the cache over the new pages, kept (batch, Hkv, budget) int32: the original slots in
+    order, -1 beyond a sequence's new length)."""
+    a = cache._args
+    dev = cache.device
+    budget = int(budget)
+    _on(table_out, dev, torch.int32, (a.batch, None), "table_out")
+    if budget <= 0:
+        raise ValueError("budget must be positive")
+    kept = torch.empty((a.batch, a.n_kv_heads, budget), dtype=torch.int32, device=dev)
+    lens = torch.empty((a.batch,), dtype=torch.int32, device=dev)
+    b = L.PagedEvictArgs(budget, int(n_global), int(n_local), table_out.data_ptr(),
+                         table_out.stride(0), table_out.shape[1], kept.data_ptr(), lens.data_ptr())
+    lib, ref = L.lib(), ctypes.byref(b)
+    with torch.cuda.device(dev):
+        n = lib.sta_paged_evict_workspace_bytes(cache._ref, ref)
+        if n == 0:
+            L.check(1, "sta_paged_evict")
+        ws = torch.empty(n, dtype=torch.uint8, device=dev)
+        L.check(lib.sta_paged_evict(cache._ref, ref, ws.data_ptr(), n, _stream()), "sta_paged_evict")
+    return cache.with_pages(table_out, lens), kept
