@@ -19,163 +19,11 @@
 
 #include <type_traits>
 
-#include "paged.cuh"
+#include "paged_decode.cuh"
 
 namespace sta {
 
 namespace {
-
-constexpr int kTile = 64;      // keys per tile
-constexpr int kThreads = 128;  // 4 warps, 16 keys of a tile each
-constexpr int kWarps = kThreads / 32;
-
-struct PDecP {
-  PagedView c;
-  const void* q;
-  int64_t qsb, qsh;  // elements
-  void* out;
-  int H, G, NG, GT;  // q heads, per kv head, groups of GT of them
-  const float* inv_freq;
-  double pos_scale;
-  float qscale;      // sm_scale * rope_scale^2 * log2(e): scores are in units of log2
-  int L, s;          // Dual Chunk Attention: chunk length and chunk size, L = 0 for plain positions
-  float* part;       // (2 * W, GT, D + 2): unnormalised output, max, sum
-  float* ml;         // (B, H, 2): final max and 1 / sum
-  float* scores;     // (B, Hkv * NG, capacity tiles, GT, 64) or null
-  int64_t cap_tiles;
-  float* w_out;
-  int* err;
-};
-
-__device__ __forceinline__ int n_tiles(int len) { return (len + kTile - 1) / kTile; }
-
-// A CTA's place in the list of tiles.
-struct Place {
-  int b, hg, n, tiles, len;
-};
-
-__device__ __forceinline__ void seek_sequence(const PagedView& c, Place& a) {
-  a.tiles = 0;
-  while (a.b < c.B) {
-    a.len = paged_len(c, a.b);
-    a.tiles = n_tiles(a.len);
-    if (a.tiles > 0) return;
-    ++a.b;
-  }
-}
-
-__device__ __forceinline__ void step(const PDecP& p, Place& a) {
-  if (++a.n < a.tiles) return;
-  a.n = 0;
-  if (++a.hg < p.c.Hkv * p.NG) return;
-  a.hg = 0;
-  ++a.b;
-  seek_sequence(p.c, a);
-}
-
-// Number of tiles of all segments (block-wide, NT threads), and with `find` >= 0 the place of
-// tile `find`; `before` receives the tiles of the sequences before sequence `until`.
-template <int NT>
-__device__ int64_t scan_lengths(const PDecP& p, int until, int64_t* before) {
-  __shared__ int64_t s_all[NT / 32], s_bef[NT / 32];
-  const int tid = threadIdx.x;
-  int64_t all = 0, bef = 0;
-  for (int b = tid; b < p.c.B; b += NT) {
-    const int t = n_tiles(paged_len(p.c, b));
-    all += t;
-    if (b < until) bef += t;
-  }
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffffu, all, o);
-    bef += __shfl_xor_sync(0xffffffffu, bef, o);
-  }
-  if ((tid & 31) == 0) {
-    s_all[tid >> 5] = all;
-    s_bef[tid >> 5] = bef;
-  }
-  __syncthreads();
-  all = bef = 0;
-#pragma unroll
-  for (int i = 0; i < NT / 32; ++i) {
-    all += s_all[i];
-    bef += s_bef[i];
-  }
-  __syncthreads();
-  const int64_t hg = (int64_t)p.c.Hkv * p.NG;
-  if (before) *before = bef * hg;
-  return all * hg;
-}
-
-template <int NT>
-__device__ Place find_tile(const PDecP& p, int64_t t) {
-  __shared__ int s_b, s_hit;
-  __shared__ int64_t s_rest, s_sum[NT / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int64_t hg = (int64_t)p.c.Hkv * p.NG;
-  int64_t base = 0;
-  Place a{};
-  if (tid == 0) s_hit = 0;
-  __syncthreads();
-  for (int b0 = 0; b0 < p.c.B; b0 += NT) {
-    const int b = b0 + tid;
-    const int64_t mine = b < p.c.B ? (int64_t)n_tiles(paged_len(p.c, b)) * hg : 0;
-    int64_t inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += y;
-    }
-    if (lane == 31) s_sum[warp] = inc;
-    __syncthreads();
-    int64_t off = base, tot = 0;
-#pragma unroll
-    for (int i = 0; i < NT / 32; ++i) {
-      if (i < warp) off += s_sum[i];
-      tot += s_sum[i];
-    }
-    const int64_t lo = off + inc - mine;
-    if (mine > 0 && t >= lo && t < lo + mine) {
-      s_b = b;
-      s_rest = t - lo;
-      s_hit = 1;
-    }
-    __syncthreads();
-    if (s_hit) break;
-    base += tot;
-  }
-  a.b = s_b;
-  a.len = paged_len(p.c, a.b);
-  a.tiles = n_tiles(a.len);
-  a.hg = (int)(s_rest / a.tiles);
-  a.n = (int)(s_rest - (int64_t)a.hg * a.tiles);
-  return a;
-}
-
-// cos / sin of pos * inv_freq: the angle in turns is formed and reduced in 64 bits
-__device__ __forceinline__ void turn(double pos, float inv_freq, float& c, float& s) {
-  const double x = pos * ((double)inv_freq * 0.15915494309189533577);  // 1 / (2 pi)
-  sincospif((float)(2.0 * (x - rint(x))), &s, &c);
-}
-
-// p_i - p_0 of a tile (position of the query minus that of the tile's first key)
-__device__ __forceinline__ double query_offset(const PDecP& p, const Place& a) {
-  const int i = a.len - 1, j0 = a.n * kTile;
-  if (p.L == 0) return (double)i * p.pos_scale - (double)j0 * p.pos_scale;
-  const int away = i / p.L - j0 / p.L, in = i % p.L;
-  const int qp = away == 0 ? in : (away == 1 ? min(p.L + in, p.s) : min(2 * p.L - 1, p.s));
-  return (double)(qp - j0 % p.L);
-}
-
-template <typename TV>
-__device__ __forceinline__ float to_f(TV x);
-template <>
-__device__ __forceinline__ float to_f<float>(float x) { return x; }
-template <>
-__device__ __forceinline__ float to_f<__nv_bfloat16>(__nv_bfloat16 x) { return __bfloat162float(x); }
-
-__device__ __forceinline__ void store_out(float* o, float x) { *o = x; }
-__device__ __forceinline__ void store_out(__nv_bfloat16* o, float x) { *o = __float2bfloat16_rn(x); }
 
 // Sums of NV values (a power of two up to 32) over the warp: lane l returns the sum of value
 // l / (32 / NV).  Each round halves the values a lane carries, so NV = 32 takes 31 shuffles.
@@ -202,36 +50,39 @@ __device__ __forceinline__ float warp_reduce(float (&v)[NV]) {
   return v[0];
 }
 
-template <int D, typename TV, int GT>
+// The f32 kernel: CUDA cores, so that scores keep full fp32 products (8 warps, 8 keys of a tile
+// each; a lane holds D / 32 dims and reduces its partial dots with the other lanes').
+constexpr int kF32Threads = 256;
+constexpr int kF32Warps = kF32Threads / 32;
+constexpr int kF32Keys = kTile / kF32Warps;  // keys of a tile per warp
+
+template <int D, int GT>
 struct Smem {
-  static constexpr int STAGES = sizeof(TV) == 2 ? 3 : 2;
-  static constexpr int CH = D * (int)sizeof(TV) / 16;  // 16-byte chunks of a row
-  uint4 k[STAGES][kTile * CH];
-  uint4 v[STAGES][kTile * CH];
-  float2 rot[kTile][D / 2];          // cos / sin of t * pos_scale * inv_freq
+  static constexpr int STAGES = 3;
+  static constexpr int CH = D / 4;   // 16-byte chunks of a row
+  uint4 kv[STAGES][2][kTile * CH];   // K rows, V rows (also the flush's scratch)
   float q[2][GT][D];                 // rotated, scaled queries of this tile and the next
-  float p[kWarps][16][GT];           // a warp's probabilities of 16 keys
-  float acc[kWarps][GT][D];
-  float m[kWarps][GT], l[kWarps][GT];
+  float p[kF32Warps][kF32Keys][GT];  // a warp's probabilities
+  float m[kF32Warps][GT], l[kF32Warps][GT];
   int64_t koff[2][kTile], voff[2][kTile];
 };
 
-template <int D, typename TV, int GT>
-__global__ void __launch_bounds__(kThreads) paged_decode_kernel(const PDecP p) {
-  using S = Smem<D, TV, GT>;
+template <int D, int GT>
+__global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDecP p) {
+  using S = Smem<D, GT>;
   constexpr int HALF = D / 2, CH = S::CH, ST = S::STAGES;
   constexpr int FP = HALF / 32;               // frequencies of a lane
-  constexpr int KB = GT == 8 ? 4 : (GT == 4 ? 8 : 16), NV = KB * GT;  // keys of one reduction
+  constexpr int KB = GT == 8 ? 4 : 8, NV = KB * GT;  // keys of one reduction
   constexpr int LPV = 32 / NV;                // lanes that hold the same value
-  constexpr int QH = GT * HALF / kThreads > 0 ? GT * HALF / kThreads : 1;  // q pairs of a thread
+  constexpr int QH = GT * HALF / kF32Threads > 0 ? GT * HALF / kF32Threads : 1;  // q pairs of a thread
   extern __shared__ __align__(128) unsigned char smem_raw[];
   S& sm = *reinterpret_cast<S*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t total = scan_lengths<kThreads>(p, 0, nullptr);
+  const int64_t total = scan_lengths<kF32Threads>(p, 0, nullptr);
   const int64_t t0 = total * blockIdx.x / gridDim.x, t1 = total * (blockIdx.x + 1) / gridDim.x;
   if (t0 >= t1) return;
   const int count = (int)(t1 - t0);
-  Place cur = find_tile<kThreads>(p, t0);
+  Place cur = find_tile<kF32Threads>(p, t0);
   Place qa = cur, oa = cur;  // where queries and row offsets stand
   int q_it = 0, l_it = 0, o_it = 0;
 
@@ -265,14 +116,14 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const PDecP p) {
     if (l_it < count) {
       const int st = l_it % ST;
 #pragma unroll 4
-      for (int i = tid; i < kTile * CH; i += kThreads) {
+      for (int i = tid; i < kTile * CH; i += kF32Threads) {
         const int row = i / CH, ch = i % CH;
         const int64_t ko = sm.koff[l_it & 1][row], vo = sm.voff[l_it & 1][row];
-        cp_async16(&sm.v[st][i], p.c.v + (vo >= 0 ? vo + ch * 16 : 0), vo >= 0 ? 16 : 0);
+        cp_async16(&sm.kv[st][1][i], p.c.v + (vo >= 0 ? vo + ch * 16 : 0), vo >= 0 ? 16 : 0);
         if (ko == -2) {
-          sm.k[st][i] = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+          sm.kv[st][0][i] = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
         } else {
-          cp_async16(&sm.k[st][i], p.c.k + (ko >= 0 ? ko + ch * 16 : 0), ko >= 0 ? 16 : 0);
+          cp_async16(&sm.kv[st][0][i], p.c.k + (ko >= 0 ? ko + ch * 16 : 0), ko >= 0 ? 16 : 0);
         }
       }
     }
@@ -281,25 +132,25 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const PDecP p) {
   };
   // ---- queries of a tile: rotated by p_i - p_0
   float q1[QH], q2[QH];
-  const int qf = tid % HALF, qg = tid / HALF;  // frequency, first head (step kThreads / HALF)
+  const int qf = tid % HALF, qg = tid / HALF;  // frequency, first head (step kF32Threads / HALF)
   auto queries = [&]() {
     if (q_it < count) {
       if (q_it == 0 || qa.n == 0) {
         const int h0 = (qa.hg / p.NG) * p.G + (qa.hg % p.NG) * GT;
 #pragma unroll
         for (int i = 0; i < QH; ++i) {
-          const int g = qg + i * (kThreads / HALF);
+          const int g = qg + i * (kF32Threads / HALF);
           const bool in = g < GT && (qa.hg % p.NG) * GT + g < p.G;
-          const TV* src = static_cast<const TV*>(p.q) + qa.b * p.qsb + (h0 + g) * p.qsh;
-          q1[i] = in ? to_f(src[qf]) * p.qscale : 0.f;
-          q2[i] = in ? to_f(src[qf + HALF]) * p.qscale : 0.f;
+          const float* src = static_cast<const float*>(p.q) + qa.b * p.qsb + (h0 + g) * p.qsh;
+          q1[i] = in ? (src[qf]) * p.qscale : 0.f;
+          q2[i] = in ? (src[qf + HALF]) * p.qscale : 0.f;
         }
       }
       float c, s;
       turn(query_offset(p, qa), __ldg(p.inv_freq + qf), c, s);
 #pragma unroll
       for (int i = 0; i < QH; ++i) {
-        const int g = qg + i * (kThreads / HALF);
+        const int g = qg + i * (kF32Threads / HALF);
         if (g < GT) {
           sm.q[q_it & 1][g][qf] = q1[i] * c - q2[i] * s;
           sm.q[q_it & 1][g][qf + HALF] = q2[i] * c + q1[i] * s;
@@ -317,12 +168,13 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const PDecP p) {
   }
   offsets();
   queries();
-  for (int i = tid; i < kTile * HALF; i += kThreads) {
-    const int t = i / HALF, f = i % HALF;
-    float c, s;
-    turn((double)t * p.pos_scale, __ldg(p.inv_freq + f), c, s);
-    sm.rot[t][f] = make_float2(c, s);
-  }
+  float2 rot[kF32Keys][FP];  // cos / sin of the warp's key offsets at the lane's frequencies
+#pragma unroll
+  for (int t = 0; t < kF32Keys; ++t)
+#pragma unroll
+    for (int e = 0; e < FP; ++e)
+      turn((double)(warp * kF32Keys + t) * p.pos_scale, __ldg(p.inv_freq + lane * FP + e), rot[t][e].x,
+           rot[t][e].y);
 
   float acc[GT][2 * FP];
   float mx = -INFINITY, sum = 0.f;  // of head (lane / LPV) % GT, replicated over its lanes
@@ -336,8 +188,8 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const PDecP p) {
     __syncthreads();
     loads();
     const int st = it % ST;
-    const TV* ks = reinterpret_cast<const TV*>(sm.k[st]);
-    const TV* vs = reinterpret_cast<const TV*>(sm.v[st]);
+    const float* ks = reinterpret_cast<const float*>(sm.kv[st][0]);
+    const float* vs = reinterpret_cast<const float*>(sm.kv[st][1]);
     float qr[GT][2 * FP];
 #pragma unroll
     for (int g = 0; g < GT; ++g)
@@ -351,8 +203,8 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const PDecP p) {
         ? p.scores + ((((int64_t)cur.b * p.c.Hkv * p.NG + cur.hg) * p.cap_tiles + cur.n) * GT) * kTile
         : nullptr;
 #pragma unroll
-    for (int kb = 0; kb < 16 / KB; ++kb) {
-      const int key0 = warp * 16 + kb * KB;
+    for (int kb = 0; kb < kF32Keys / KB; ++kb) {
+      const int key0 = warp * kF32Keys + kb * KB;
       float v[NV];
 #pragma unroll
       for (int kk = 0; kk < KB; ++kk) {
@@ -360,9 +212,9 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const PDecP p) {
         float r1[FP], r2[FP];
 #pragma unroll
         for (int e = 0; e < FP; ++e) {
-          const float x1 = to_f(ks[t * D + lane * FP + e]);
-          const float x2 = to_f(ks[t * D + HALF + lane * FP + e]);
-          const float2 cs = sm.rot[t][lane * FP + e];
+          const float x1 = (ks[t * D + lane * FP + e]);
+          const float x2 = (ks[t * D + HALF + lane * FP + e]);
+          const float2 cs = rot[kb * KB + kk][e];
           r1[e] = x1 * cs.x - x2 * cs.y;
           r2[e] = x2 * cs.x + x1 * cs.y;
         }
@@ -402,8 +254,8 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const PDecP p) {
         float vv[2 * FP];
 #pragma unroll
         for (int x = 0; x < FP; ++x) {
-          vv[x] = to_f(vs[t * D + lane * FP + x]);
-          vv[FP + x] = to_f(vs[t * D + HALF + lane * FP + x]);
+          vv[x] = (vs[t * D + lane * FP + x]);
+          vv[FP + x] = (vs[t * D + HALF + lane * FP + x]);
         }
 #pragma unroll
         for (int gg = 0; gg < GT; ++gg) {
@@ -417,6 +269,8 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const PDecP p) {
     const bool seg_end = cur.n == cur.tiles - 1;
     if (seg_end || it == count - 1) {
       // the warps' partial results of this segment, joined and stored
+      float* part_acc = reinterpret_cast<float*>(sm.kv[st][0]);  // [warp][head][d]
+      __syncthreads();
       const int idx = lane / LPV;
       if (idx < GT && lane % LPV == 0) {
         sm.m[warp][idx] = mx;
@@ -426,30 +280,30 @@ __global__ void __launch_bounds__(kThreads) paged_decode_kernel(const PDecP p) {
       for (int g = 0; g < GT; ++g)
 #pragma unroll
         for (int x = 0; x < FP; ++x) {
-          sm.acc[warp][g][lane * FP + x] = acc[g][x];
-          sm.acc[warp][g][HALF + lane * FP + x] = acc[g][FP + x];
+          part_acc[(warp * GT + g) * D + lane * FP + x] = acc[g][x];
+          part_acc[(warp * GT + g) * D + HALF + lane * FP + x] = acc[g][FP + x];
         }
       __syncthreads();
       const bool started = cur.n <= it;  // the segment's first tile lies in this share
       const bool whole = seg_end && started;
       const int slot = 2 * blockIdx.x + (started ? 1 : 0);
       const int h0 = (cur.hg / p.NG) * p.G + (cur.hg % p.NG) * GT;
-      for (int i = tid; i < GT * D; i += kThreads) {
+      for (int i = tid; i < GT * D; i += kF32Threads) {
         const int g = i / D, d = i % D;
         if ((cur.hg % p.NG) * GT + g >= p.G) continue;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) M = fmaxf(M, sm.m[w][g]);
+        for (int w = 0; w < kF32Warps; ++w) M = fmaxf(M, sm.m[w][g]);
         const float ms = M == -INFINITY ? 0.f : M;
         float L = 0.f, o = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
+        for (int w = 0; w < kF32Warps; ++w) {
           const float f = exp2f(sm.m[w][g] - ms);
           L += sm.l[w][g] * f;
-          o += sm.acc[w][g][d] * f;
+          o += part_acc[(w * GT + g) * D + d] * f;
         }
         if (whole) {
-          store_out(static_cast<TV*>(p.out) + ((int64_t)cur.b * p.H + h0 + g) * D + d, o / L);
+          store_out(static_cast<float*>(p.out) + ((int64_t)cur.b * p.H + h0 + g) * D + d, o / L);
           if (d == 0) {
             float* ml = p.ml + ((int64_t)cur.b * p.H + h0 + g) * 2;
             ml[0] = ms;
@@ -563,11 +417,16 @@ int sm_count() {
 PLayout layout(const sta_paged_cache* c, const sta_paged_decode_args* a) {
   PLayout L{};
   const int64_t G = a->n_heads / c->n_kv_heads;
-  L.GT = G > 4 ? 8 : (G > 2 ? 4 : (int)G);
+  const bool f32 = c->dtype == STA_DTYPE_F32;
+  // q heads that one pass over a kv head's keys serves: f32 by registers (padded to 1, 2, 4 or 8),
+  // bf16 by the 8 columns of a tensor-core product, one or two of them
+  if (f32) L.GT = G > 4 ? 8 : (G > 2 ? 4 : (int)G);
+  else L.GT = G > 8 ? 16 : 8;
   L.NG = (int)((G + L.GT - 1) / L.GT);
   L.cap_tiles = (c->table_width * c->page_size + kTile - 1) / kTile;
   const int64_t most = c->batch * c->n_kv_heads * L.NG * L.cap_tiles;
-  const int64_t w = 2 * (int64_t)sm_count();
+  const int per_sm = f32 ? (c->d == 128 ? 1 : 2) : paged_decode_bf16_ctas(c->d, L.GT);
+  const int64_t w = per_sm * (int64_t)sm_count();
   L.W = (int)(most < w ? most : w);
   size_t o = 0;
   auto take = [&](size_t bytes) {
@@ -604,23 +463,29 @@ int check(const sta_paged_cache* c, const sta_paged_decode_args* a) {
   return STA_OK;
 }
 
-template <int D, typename TV, int GT>
-int launch(const PDecP& p, int W, cudaStream_t st) {
-  constexpr int bytes = (int)sizeof(Smem<D, TV, GT>);
-  const cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<D, TV, GT>,
+template <int D, int GT>
+int launch_f32(const PDecP& p, int W, cudaStream_t st) {
+  constexpr int bytes = (int)sizeof(Smem<D, GT>);
+  const cudaError_t e = cudaFuncSetAttribute(paged_decode_f32_kernel<D, GT>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(STA_ERR_CUDA, cudaGetErrorString(e));
-  paged_decode_kernel<D, TV, GT><<<W, kThreads, bytes, st>>>(p);
-  paged_join_kernel<D, TV><<<(unsigned)(p.c.B * p.c.Hkv * p.NG), D, 0, st>>>(p, W);
+  paged_decode_f32_kernel<D, GT><<<W, kF32Threads, bytes, st>>>(p);
   return STA_OK;
 }
 
-template <int D, typename TV>
-int launch_g(const PDecP& p, int W, cudaStream_t st) {
-  if (p.GT == 1) return launch<D, TV, 1>(p, W, st);
-  if (p.GT == 2) return launch<D, TV, 2>(p, W, st);
-  if (p.GT == 4) return launch<D, TV, 4>(p, W, st);
-  return launch<D, TV, 8>(p, W, st);
+template <int D>
+int launch_f32(const PDecP& p, int W, cudaStream_t st) {
+  if (p.GT == 1) return launch_f32<D, 1>(p, W, st);
+  if (p.GT == 2) return launch_f32<D, 2>(p, W, st);
+  if (p.GT == 4) return launch_f32<D, 4>(p, W, st);
+  return launch_f32<D, 8>(p, W, st);
+}
+
+template <typename TV>
+void launch_join(const PDecP& p, int d, int W, cudaStream_t st) {
+  const unsigned grid = (unsigned)(p.c.B * p.c.Hkv * p.NG);
+  if (d == 128) paged_join_kernel<128, TV><<<grid, 128, 0, st>>>(p, W);
+  else paged_join_kernel<64, TV><<<grid, 64, 0, st>>>(p, W);
 }
 
 }  // namespace
@@ -660,11 +525,11 @@ int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void*
   p.err = device_error_word();
   if (!p.err) return fail(STA_ERR_CUDA, "sta_paged_decode: no device");
   const bool f32 = c->dtype == STA_DTYPE_F32;
-  if (c->d == 128)
-    rc = f32 ? launch_g<128, float>(p, L.W, st) : launch_g<128, __nv_bfloat16>(p, L.W, st);
-  else
-    rc = f32 ? launch_g<64, float>(p, L.W, st) : launch_g<64, __nv_bfloat16>(p, L.W, st);
+  if (f32) rc = c->d == 128 ? launch_f32<128>(p, L.W, st) : launch_f32<64>(p, L.W, st);
+  else rc = launch_paged_decode_bf16(p, c->d, L.W, st);
   if (rc != STA_OK) return rc;
+  if (f32) launch_join<float>(p, c->d, L.W, st);
+  else launch_join<__nv_bfloat16>(p, c->d, L.W, st);
   if (a->weights_out) {
     const dim3 grid((unsigned)((p.c.cap + 255) / 256), (unsigned)p.c.Hkv, (unsigned)p.c.B);
     paged_weights_kernel<<<grid, 256, 0, st>>>(p);
