@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
         }
       }
       float c, s;
-      turn(query_offset(p, qa), __ldg(p.inv_freq + qf), c, s);
+      turn(query_offset(p, qa.len, qa.n), __ldg(p.inv_freq + qf), c, s);
 #pragma unroll
       for (int i = 0; i < QH; ++i) {
         const int g = qg + i * (kF32Threads / HALF);
@@ -304,18 +304,10 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
         }
         if (whole) {
           store_out(static_cast<float*>(p.out) + ((int64_t)cur.b * p.H + h0 + g) * D + d, o / L);
-          if (d == 0) {
-            float* ml = p.ml + ((int64_t)cur.b * p.H + h0 + g) * 2;
-            ml[0] = ms;
-            ml[1] = 1.f / L;
-          }
+          if (d == 0) p.ml[(int64_t)cur.b * p.H + h0 + g] = make_float2(ms, 1.f / L);
         } else {
-          float* part = p.part + ((int64_t)slot * GT + g) * (D + 2);
-          part[d] = o;
-          if (d == 0) {
-            part[D] = M;
-            part[D + 1] = L;
-          }
+          p.part[((int64_t)slot * GT + g) * D + d] = o;
+          if (d == 0) p.part_ml[(int64_t)slot * GT + g] = make_float2(M, L);
         }
       }
 #pragma unroll
@@ -331,71 +323,155 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
   }
 }
 
-// One CTA per segment: joins the partials of the shares that cut it.  Empty sequences give zeros.
-template <int D, typename TV>
-__global__ void __launch_bounds__(D) paged_join_kernel(const PDecP p, int W) {
-  const int hgs = p.c.Hkv * p.NG;
-  const int b = blockIdx.x / hgs, hg = blockIdx.x % hgs, d = threadIdx.x;
-  const int h0 = (hg / p.NG) * p.G + (hg % p.NG) * p.GT, ng = min(p.GT, p.G - (hg % p.NG) * p.GT);
+constexpr int kFinish = 256;   // threads of the finishing kernel
+constexpr int kKeysPer = 4;    // keys of a thread in the weights update
+
+// The shares [w0, w1] that cut a segment; one share (w0 == w1) has finished it.
+struct Cut {
+  int64_t total, s0, w0, w1;
+};
+
+__device__ __forceinline__ Cut cut_of(const PDecP& p, int b, int hg, int64_t tiles, int W) {
+  Cut c;
   int64_t before;
-  const int64_t total = scan_lengths<D>(p, b, &before);
-  const int64_t tiles = n_tiles(paged_len(p.c, b));
-  TV* out = static_cast<TV*>(p.out) + ((int64_t)b * p.H + h0) * D;
-  if (tiles == 0) {
-    for (int g = 0; g < ng; ++g) store_out(out + g * D + d, 0.f);
-    return;
-  }
-  // the shares of this segment's first and last tile (share w holds [total w / W, total (w+1) / W))
-  const int64_t s0 = before + hg * tiles, s1 = s0 + tiles;
-  int64_t w0 = s0 * W / total, w1 = (s1 - 1) * W / total;
-  while (total * (w0 + 1) / W <= s0) ++w0;
-  while (total * (w1 + 1) / W <= s1 - 1) ++w1;
-  if (w0 == w1) return;  // finished by its share
-  for (int g = 0; g < ng; ++g) {
-    float M = -INFINITY, L = 0.f, o = 0.f;
-    for (int64_t w = w0; w <= w1; ++w) {
-      const int64_t slot = 2 * w + (total * w / W <= s0 ? 1 : 0);
-      if (total * w / W == total * (w + 1) / W) continue;  // an empty share
-      const float* part = p.part + (slot * p.GT + g) * (D + 2);
-      const float m = part[D], l = part[D + 1], x = part[d];
-      const float mn = fmaxf(M, m), ms = mn == -INFINITY ? 0.f : mn;
-      const float a = exp2f(M - ms), e = exp2f(m - ms);
-      L = L * a + l * e;
-      o = o * a + x * e;
-      M = mn;
-    }
-    store_out(out + g * D + d, o / L);
-    if (d == 0) {
-      float* ml = p.ml + ((int64_t)b * p.H + h0 + g) * 2;
-      ml[0] = M == -INFINITY ? 0.f : M;
-      ml[1] = 1.f / L;
-    }
-  }
+  c.total = scan_lengths<kFinish>(p, b, &before);
+  c.s0 = before + hg * tiles;
+  c.w0 = c.w1 = 0;
+  if (tiles == 0) return c;
+  // share w holds the tiles [total * w / W, total * (w + 1) / W)
+  const int64_t last = c.s0 + tiles - 1;
+  c.w0 = c.s0 * W / c.total;
+  c.w1 = last * W / c.total;
+  while (c.total * (c.w0 + 1) / W <= c.s0) ++c.w0;
+  while (c.total * (c.w1 + 1) / W <= last) ++c.w1;
+  return c;
 }
 
-// weights_out[j] = weights[j] + sum_g exp2(s_gj - M_g) / L_g
-__global__ void __launch_bounds__(256) paged_weights_kernel(const PDecP p) {
-  const int b = blockIdx.z, h = blockIdx.y;
-  const int len = paged_len(p.c, b);
-  const int64_t j = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (j >= len) return;
-  const uint32_t t = (uint32_t)j / p.c.page;
-  const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
-  if (pg < 0) return;
-  float w = 0.f;
-  for (int g = 0; g < p.G; ++g) {
-    const int hg = h * p.NG + g / p.GT;
-    const float s = p.scores[((((int64_t)b * p.c.Hkv * p.NG + hg) * p.cap_tiles + j / kTile) * p.GT +
-                              g % p.GT) * kTile + j % kTile];
-    const float* ml = p.ml + ((int64_t)b * p.H + h * p.G + g) * 2;
-    w += exp2f(s - ml[0]) * ml[1];
+// the partial that share w left of the segment (-1: the share is empty)
+__device__ __forceinline__ int64_t slot_of(const Cut& c, int64_t w, int W) {
+  const int64_t t0 = c.total * w / W;
+  if (t0 == c.total * (w + 1) / W) return -1;
+  return 2 * w + (t0 <= c.s0 ? 1 : 0);
+}
+
+// max and sum of one head over the partials of a segment, by one warp
+__device__ __forceinline__ void join_ml(const PDecP& p, const Cut& c, int g, int W, float& M, float& L) {
+  const int lane = threadIdx.x & 31;
+  M = -INFINITY;
+  L = 0.f;
+  for (int64_t w = c.w0 + lane; w <= c.w1; w += 32) {
+    const int64_t slot = slot_of(c, w, W);
+    if (slot < 0) continue;
+    const float2 ml = p.part_ml[slot * p.GT + g];
+    const float mn = fmaxf(M, ml.x), ms = mn == -INFINITY ? 0.f : mn;
+    L = L * exp2f(M - ms) + ml.y * exp2f(ml.x - ms);
+    M = mn;
   }
-  const int64_t at = pg * p.c.wsp + h * p.c.wsh + ((uint32_t)j - t * p.c.page);
-  p.w_out[at] = p.c.w[at] + w;
+#pragma unroll
+  for (int o = 16; o >= 1; o >>= 1) {
+    const float m = __shfl_xor_sync(0xffffffffu, M, o), l = __shfl_xor_sync(0xffffffffu, L, o);
+    const float mn = fmaxf(M, m), ms = mn == -INFINITY ? 0.f : mn;
+    L = L * exp2f(M - ms) + l * exp2f(m - ms);
+    M = mn;
+  }
+  if (M == -INFINITY) M = 0.f;
+}
+
+// One block per (sequence, q head) joins the partials of the shares that cut its segment: a warp
+// takes every eighth partial, so that their loads are in flight together.  Empty sequences give
+// zeros.  With weights, blocks behind those update 1024 keys of a (sequence, kv head) each:
+// weights_out[j] = weights[j] + sum_g exp2(s_gj - M_g) / L_g, where they form M and L themselves.
+template <int D, typename TV>
+__global__ void __launch_bounds__(kFinish) paged_finish_kernel(const PDecP p, int W) {
+  constexpr int NW = kFinish / 32, V = D / 32;
+  __shared__ float s_o[NW][D];
+  __shared__ float2 s_ml[128];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t joins = (int64_t)p.c.B * p.H;
+  if (blockIdx.x < joins) {
+    const int b = blockIdx.x / p.H, h = blockIdx.x % p.H;
+    const int g0 = h % p.G, hg = h / p.G * p.NG + g0 / p.GT, g = g0 % p.GT;
+    const int64_t tiles = n_tiles(paged_len(p.c, b));
+    TV* out = static_cast<TV*>(p.out) + (int64_t)blockIdx.x * D;
+    if (tiles == 0) {
+      if (tid < D) store_out(out + tid, 0.f);
+      return;
+    }
+    const Cut c = cut_of(p, b, hg, tiles, W);
+    if (c.w0 == c.w1) return;
+    float M, L;
+    join_ml(p, c, g, W, M, L);
+    float o[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] = 0.f;
+#pragma unroll 4
+    for (int64_t w = c.w0 + warp; w <= c.w1; w += NW) {
+      const int64_t slot = slot_of(c, w, W);
+      if (slot < 0) continue;
+      const float f = exp2f(p.part_ml[slot * p.GT + g].x - M);
+      const float* part = p.part + (slot * p.GT + g) * D + lane * V;
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = fmaf(part[i], f, o[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) s_o[warp][lane * V + i] = o[i];
+    __syncthreads();
+    if (tid < D) {
+      float x = 0.f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) x += s_o[i][tid];
+      store_out(out + tid, x / L);
+    }
+    return;
+  }
+  const int64_t chunks = (p.c.cap + kFinish * kKeysPer - 1) / (kFinish * kKeysPer);
+  const int64_t at = blockIdx.x - joins, seg = at / chunks;
+  const int b = (int)(seg / p.c.Hkv), h = (int)(seg % p.c.Hkv);
+  const int len = paged_len(p.c, b);
+  const int64_t j0 = (at % chunks) * (kFinish * kKeysPer) + tid;
+  if (at % chunks * (kFinish * kKeysPer) >= len) return;
+  float sum[kKeysPer];
+#pragma unroll
+  for (int i = 0; i < kKeysPer; ++i) sum[i] = 0.f;
+  for (int grp = 0; grp < p.NG; ++grp) {
+    const int hg = h * p.NG + grp, heads = min(p.GT, p.G - grp * p.GT);
+    const Cut c = cut_of(p, b, hg, n_tiles(len), W);
+    for (int g = warp; g < heads; g += NW) {
+      float2 ml;
+      if (c.w0 == c.w1) {
+        ml = p.ml[(int64_t)b * p.H + h * p.G + grp * p.GT + g];
+      } else {
+        join_ml(p, c, g, W, ml.x, ml.y);
+        ml.y = 1.f / ml.y;
+      }
+      if (lane == 0) s_ml[g] = ml;
+    }
+    __syncthreads();
+    const float* sc = p.scores + ((int64_t)b * p.c.Hkv * p.NG + hg) * p.cap_tiles * p.GT * kTile;
+    for (int g = 0; g < heads; ++g) {
+      const float2 ml = s_ml[g];
+#pragma unroll
+      for (int i = 0; i < kKeysPer; ++i) {
+        const int64_t j = j0 + i * kFinish;
+        if (j < len) sum[i] += exp2f(sc[(j / kTile * p.GT + g) * kTile + j % kTile] - ml.x) * ml.y;
+      }
+    }
+    __syncthreads();
+  }
+#pragma unroll
+  for (int i = 0; i < kKeysPer; ++i) {
+    const int64_t j = j0 + i * kFinish;
+    if (j >= len) break;
+    const uint32_t t = (uint32_t)j / p.c.page;
+    const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
+    if (pg < 0) continue;
+    const int64_t w = pg * p.c.wsp + h * p.c.wsh + ((uint32_t)j - t * p.c.page);
+    p.w_out[w] = p.c.w[w] + sum[i];
+  }
 }
 
 struct PLayout {
-  size_t part, ml, scores, total;
+  size_t part, part_ml, ml, scores, total;
   int GT, NG, W;
   int64_t cap_tiles;
 };
@@ -434,7 +510,8 @@ PLayout layout(const sta_paged_cache* c, const sta_paged_decode_args* a) {
     o += al(bytes);
     return r;
   };
-  L.part = take((size_t)2 * L.W * L.GT * (c->d + 2) * 4);
+  L.part = take((size_t)2 * L.W * L.GT * c->d * 4);
+  L.part_ml = take((size_t)2 * L.W * L.GT * 8);
   L.ml = take((size_t)c->batch * a->n_heads * 8);
   L.scores = a->weights_out ? take((size_t)most * L.GT * kTile * 4) : 0;
   L.total = o + 256;
@@ -456,8 +533,8 @@ int check(const sta_paged_cache* c, const sta_paged_decode_args* a) {
     return fail(STA_ERR_ARG, "sta_paged_decode: Dual Chunk Attention positions take pos_scale 1");
   if (a->weights_out && !c->weights)
     return fail(STA_ERR_ARG, "sta_paged_decode: weights_out needs a cache with weights");
-  if (a->weights_out && c->batch > 65535)
-    return fail(STA_ERR_UNSUPPORTED, "sta_paged_decode: weights take at most 65535 sequences");
+  if (a->weights_out && c->batch * c->n_kv_heads * (c->table_width * c->page_size / 1024 + 1) > ((int64_t)1 << 30))
+    return fail(STA_ERR_UNSUPPORTED, "sta_paged_decode: too many slots for one update of the weights");
   if (c->batch * a->n_heads > ((int64_t)1 << 30))
     return fail(STA_ERR_UNSUPPORTED, "sta_paged_decode: too many heads");
   return STA_OK;
@@ -482,10 +559,12 @@ int launch_f32(const PDecP& p, int W, cudaStream_t st) {
 }
 
 template <typename TV>
-void launch_join(const PDecP& p, int d, int W, cudaStream_t st) {
-  const unsigned grid = (unsigned)(p.c.B * p.c.Hkv * p.NG);
-  if (d == 128) paged_join_kernel<128, TV><<<grid, 128, 0, st>>>(p, W);
-  else paged_join_kernel<64, TV><<<grid, 64, 0, st>>>(p, W);
+void launch_finish(const PDecP& p, int d, int W, cudaStream_t st) {
+  int64_t grid = (int64_t)p.c.B * p.H;
+  if (p.scores)
+    grid += (int64_t)p.c.B * p.c.Hkv * ((p.c.cap + kFinish * kKeysPer - 1) / (kFinish * kKeysPer));
+  if (d == 128) paged_finish_kernel<128, TV><<<(unsigned)grid, kFinish, 0, st>>>(p, W);
+  else paged_finish_kernel<64, TV><<<(unsigned)grid, kFinish, 0, st>>>(p, W);
 }
 
 }  // namespace
@@ -518,7 +597,8 @@ int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void*
   p.L = a->chunk_size > 0 ? a->chunk_size - a->local_window : 0;
   p.s = a->chunk_size;
   p.part = reinterpret_cast<float*>(w + L.part);
-  p.ml = reinterpret_cast<float*>(w + L.ml);
+  p.part_ml = reinterpret_cast<float2*>(w + L.part_ml);
+  p.ml = reinterpret_cast<float2*>(w + L.ml);
   p.scores = a->weights_out ? reinterpret_cast<float*>(w + L.scores) : nullptr;
   p.cap_tiles = L.cap_tiles;
   p.w_out = a->weights_out;
@@ -528,12 +608,8 @@ int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void*
   if (f32) rc = c->d == 128 ? launch_f32<128>(p, L.W, st) : launch_f32<64>(p, L.W, st);
   else rc = launch_paged_decode_bf16(p, c->d, L.W, st);
   if (rc != STA_OK) return rc;
-  if (f32) launch_join<float>(p, c->d, L.W, st);
-  else launch_join<__nv_bfloat16>(p, c->d, L.W, st);
-  if (a->weights_out) {
-    const dim3 grid((unsigned)((p.c.cap + 255) / 256), (unsigned)p.c.Hkv, (unsigned)p.c.B);
-    paged_weights_kernel<<<grid, 256, 0, st>>>(p);
-  }
+  if (f32) launch_finish<float>(p, c->d, L.W, st);
+  else launch_finish<__nv_bfloat16>(p, c->d, L.W, st);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? STA_OK : fail(STA_ERR_CUDA, cudaGetErrorString(e));
 }

@@ -20,8 +20,9 @@ struct PDecP {
   double pos_scale;
   float qscale;      // sm_scale * rope_scale^2 * log2(e): scores are in units of log2
   int L, s;          // Dual Chunk Attention: chunk length and chunk size, L = 0 for plain positions
-  float* part;       // (2 * W, GT, D + 2): unnormalised output, max, sum
-  float* ml;         // (B, H, 2): final max and 1 / sum
+  float* part;       // (2 * W, GT, D): unnormalised outputs of cut segments
+  float2* part_ml;   // (2 * W, GT): their max and sum
+  float2* ml;        // (B, H): max and 1 / sum of segments that one share holds
   float* scores;     // (B, Hkv * NG, capacity tiles, GT, 64) or null
   int64_t cap_tiles;
   float* w_out;
@@ -140,8 +141,8 @@ __device__ __forceinline__ void turn(double pos, float inv_freq, float& c, float
 }
 
 // p_i - p_0 of a tile (position of the query minus that of the tile's first key)
-__device__ __forceinline__ double query_offset(const PDecP& p, const Place& a) {
-  const int i = a.len - 1, j0 = a.n * kTile;
+__device__ __forceinline__ double query_offset(const PDecP& p, int len, int n) {
+  const int i = len - 1, j0 = n * kTile;
   if (p.L == 0) return (double)i * p.pos_scale - (double)j0 * p.pos_scale;
   const int away = i / p.L - j0 / p.L, in = i % p.L;
   const int qp = away == 0 ? in : (away == 1 ? min(p.L + in, p.s) : min(2 * p.L - 1, p.s));
