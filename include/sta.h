@@ -596,7 +596,7 @@ int sta_paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, v
  * are left as they were, and pages must not be shared between sequences then. */
 typedef struct sta_paged_decode_args {
   const void* q; int64_t q_stride_b; int64_t q_stride_h;   /* (batch, n_heads, d) */
-  void* out;               /* (batch, n_heads, d) contiguous, dtype */
+  void* out;               /* (batch, n_heads, d) contiguous, dtype, 16-byte aligned */
   int64_t n_heads;
   const float* inv_freq;   /* (d/2,) */
   double pos_scale;

@@ -78,11 +78,11 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
   extern __shared__ __align__(128) unsigned char smem_raw[];
   S& sm = *reinterpret_cast<S*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t total = scan_lengths<kF32Threads>(p, 0, nullptr);
-  const int64_t t0 = total * blockIdx.x / gridDim.x, t1 = total * (blockIdx.x + 1) / gridDim.x;
-  if (t0 >= t1) return;
+  const int64_t total = scan_lengths(p, 0, nullptr), shares = n_shares(p, total);
+  if (blockIdx.x >= shares) return;
+  const int64_t t0 = total * blockIdx.x / shares, t1 = total * (blockIdx.x + 1) / shares;
   const int count = (int)(t1 - t0);
-  Place cur = find_tile<kF32Threads>(p, t0);
+  Place cur = find_unit(p, t0);
   Place qa = cur, oa = cur;  // where queries and row offsets stand
   int q_it = 0, l_it = 0, o_it = 0;
 
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
             ko = -2;
             atomicCAS(p.err, 0, kErrPageDecode);
           } else {
-            const int64_t slot = (uint32_t)j - t * p.c.page, h = oa.hg / p.NG;
+            const int64_t slot = (uint32_t)j - t * p.c.page, h = oa.h;
             ko = pg * p.c.ksp + h * p.c.ksh + slot * p.c.ksn;
             vo = pg * p.c.vsp + h * p.c.vsh + slot * p.c.vsn;
           }
@@ -136,11 +136,11 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
   auto queries = [&]() {
     if (q_it < count) {
       if (q_it == 0 || qa.n == 0) {
-        const int h0 = (qa.hg / p.NG) * p.G + (qa.hg % p.NG) * GT;
+        const int h0 = qa.h * p.G + qa.grp * GT;
 #pragma unroll
         for (int i = 0; i < QH; ++i) {
           const int g = qg + i * (kF32Threads / HALF);
-          const bool in = g < GT && (qa.hg % p.NG) * GT + g < p.G;
+          const bool in = g < GT && qa.grp * GT + g < p.G;
           const float* src = static_cast<const float*>(p.q) + qa.b * p.qsb + (h0 + g) * p.qsh;
           q1[i] = in ? (src[qf]) * p.qscale : 0.f;
           q2[i] = in ? (src[qf + HALF]) * p.qscale : 0.f;
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
       }
     const int valid = cur.len - cur.n * kTile;  // keys of this tile
     float* sc = p.scores
-        ? p.scores + ((((int64_t)cur.b * p.c.Hkv * p.NG + cur.hg) * p.cap_tiles + cur.n) * GT) * kTile
+        ? p.scores + ((((int64_t)cur.b * p.c.Hkv * p.NG + cur.h * p.NG + cur.grp) * p.cap_tiles + cur.n) * GT) * kTile
         : nullptr;
 #pragma unroll
     for (int kb = 0; kb < kF32Keys / KB; ++kb) {
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
       }
       __syncwarp();
     }
-    const bool seg_end = cur.n == cur.tiles - 1;
+    const bool seg_end = cur.n == cur.units - 1;
     if (seg_end || it == count - 1) {
       // the warps' partial results of this segment, joined and stored
       float* part_acc = reinterpret_cast<float*>(sm.kv[st][0]);  // [warp][head][d]
@@ -287,10 +287,10 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
       const bool started = cur.n <= it;  // the segment's first tile lies in this share
       const bool whole = seg_end && started;
       const int slot = 2 * blockIdx.x + (started ? 1 : 0);
-      const int h0 = (cur.hg / p.NG) * p.G + (cur.hg % p.NG) * GT;
+      const int h0 = cur.h * p.G + cur.grp * GT;
       for (int i = tid; i < GT * D; i += kF32Threads) {
         const int g = i / D, d = i % D;
-        if ((cur.hg % p.NG) * GT + g >= p.G) continue;
+        if (cur.grp * GT + g >= p.G) continue;
         float M = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kF32Warps; ++w) M = fmaxf(M, sm.m[w][g]);
@@ -326,43 +326,37 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
 constexpr int kFinish = 256;   // threads of the finishing kernel
 constexpr int kKeysPer = 4;    // keys of a thread in the weights update
 
-// The shares [w0, w1] that cut a segment; one share (w0 == w1) has finished it.
+// The shares [w0, w1] of W that cut a segment; one share (w0 == w1) has finished it.
 struct Cut {
-  int64_t total, s0, w0, w1;
+  int64_t total, W, s0, w0, w1;
 };
 
-__device__ __forceinline__ Cut cut_of(const PDecP& p, int b, int hg, int64_t tiles, int W) {
+__device__ __forceinline__ Cut cut_of(const PDecP& p, int b, int hg, int64_t units) {
   Cut c;
   int64_t before;
-  c.total = scan_lengths<kFinish>(p, b, &before);
-  c.s0 = before + hg * tiles;
-  c.w0 = c.w1 = 0;
-  if (tiles == 0) return c;
-  // share w holds the tiles [total * w / W, total * (w + 1) / W)
-  const int64_t last = c.s0 + tiles - 1;
-  c.w0 = c.s0 * W / c.total;
-  c.w1 = last * W / c.total;
-  while (c.total * (c.w0 + 1) / W <= c.s0) ++c.w0;
-  while (c.total * (c.w1 + 1) / W <= last) ++c.w1;
+  c.total = scan_lengths(p, b, &before);
+  c.W = n_shares(p, c.total);
+  c.s0 = before + hg * units;
+  const int64_t last = c.s0 + units - 1;
+  c.w0 = c.s0 * c.W / c.total;
+  c.w1 = last * c.W / c.total;
+  while (c.total * (c.w0 + 1) / c.W <= c.s0) ++c.w0;
+  while (c.total * (c.w1 + 1) / c.W <= last) ++c.w1;
   return c;
 }
 
-// the partial that share w left of the segment (-1: the share is empty)
-__device__ __forceinline__ int64_t slot_of(const Cut& c, int64_t w, int W) {
-  const int64_t t0 = c.total * w / W;
-  if (t0 == c.total * (w + 1) / W) return -1;
-  return 2 * w + (t0 <= c.s0 ? 1 : 0);
+// the partial that share w left of the segment (no share is empty: W is at most the units)
+__device__ __forceinline__ int64_t slot_of(const Cut& c, int64_t w) {
+  return 2 * w + (c.total * w / c.W <= c.s0 ? 1 : 0);
 }
 
 // max and sum of one head over the partials of a segment, by one warp
-__device__ __forceinline__ void join_ml(const PDecP& p, const Cut& c, int g, int W, float& M, float& L) {
+__device__ __forceinline__ void join_ml(const PDecP& p, const Cut& c, int g, float& M, float& L) {
   const int lane = threadIdx.x & 31;
   M = -INFINITY;
   L = 0.f;
   for (int64_t w = c.w0 + lane; w <= c.w1; w += 32) {
-    const int64_t slot = slot_of(c, w, W);
-    if (slot < 0) continue;
-    const float2 ml = p.part_ml[slot * p.GT + g];
+    const float2 ml = p.part_ml[slot_of(c, w) * p.GT + g];
     const float mn = fmaxf(M, ml.x), ms = mn == -INFINITY ? 0.f : mn;
     L = L * exp2f(M - ms) + ml.y * exp2f(ml.x - ms);
     M = mn;
@@ -382,7 +376,7 @@ __device__ __forceinline__ void join_ml(const PDecP& p, const Cut& c, int g, int
 // zeros.  With weights, blocks behind those update 1024 keys of a (sequence, kv head) each:
 // weights_out[j] = weights[j] + sum_g exp2(s_gj - M_g) / L_g, where they form M and L themselves.
 template <int D, typename TV>
-__global__ void __launch_bounds__(kFinish) paged_finish_kernel(const PDecP p, int W) {
+__global__ void __launch_bounds__(kFinish) paged_finish_kernel(const PDecP p) {
   constexpr int NW = kFinish / 32, V = D / 32;
   __shared__ float s_o[NW][D];
   __shared__ float2 s_ml[128];
@@ -391,23 +385,22 @@ __global__ void __launch_bounds__(kFinish) paged_finish_kernel(const PDecP p, in
   if (blockIdx.x < joins) {
     const int b = blockIdx.x / p.H, h = blockIdx.x % p.H;
     const int g0 = h % p.G, hg = h / p.G * p.NG + g0 / p.GT, g = g0 % p.GT;
-    const int64_t tiles = n_tiles(paged_len(p.c, b));
+    const int units = n_units(p, paged_len(p.c, b));
     TV* out = static_cast<TV*>(p.out) + (int64_t)blockIdx.x * D;
-    if (tiles == 0) {
+    if (units == 0) {
       if (tid < D) store_out(out + tid, 0.f);
       return;
     }
-    const Cut c = cut_of(p, b, hg, tiles, W);
+    const Cut c = cut_of(p, b, hg, units);
     if (c.w0 == c.w1) return;
     float M, L;
-    join_ml(p, c, g, W, M, L);
+    join_ml(p, c, g, M, L);
     float o[V];
 #pragma unroll
     for (int i = 0; i < V; ++i) o[i] = 0.f;
 #pragma unroll 4
     for (int64_t w = c.w0 + warp; w <= c.w1; w += NW) {
-      const int64_t slot = slot_of(c, w, W);
-      if (slot < 0) continue;
+      const int64_t slot = slot_of(c, w);
       const float f = exp2f(p.part_ml[slot * p.GT + g].x - M);
       const float* part = p.part + (slot * p.GT + g) * D + lane * V;
 #pragma unroll
@@ -435,13 +428,13 @@ __global__ void __launch_bounds__(kFinish) paged_finish_kernel(const PDecP p, in
   for (int i = 0; i < kKeysPer; ++i) sum[i] = 0.f;
   for (int grp = 0; grp < p.NG; ++grp) {
     const int hg = h * p.NG + grp, heads = min(p.GT, p.G - grp * p.GT);
-    const Cut c = cut_of(p, b, hg, n_tiles(len), W);
+    const Cut c = cut_of(p, b, hg, n_units(p, len));
     for (int g = warp; g < heads; g += NW) {
       float2 ml;
       if (c.w0 == c.w1) {
         ml = p.ml[(int64_t)b * p.H + h * p.G + grp * p.GT + g];
       } else {
-        join_ml(p, c, g, W, ml.x, ml.y);
+        join_ml(p, c, g, ml.x, ml.y);
         ml.y = 1.f / ml.y;
       }
       if (lane == 0) s_ml[g] = ml;
@@ -472,7 +465,7 @@ __global__ void __launch_bounds__(kFinish) paged_finish_kernel(const PDecP p, in
 
 struct PLayout {
   size_t part, part_ml, ml, scores, total;
-  int GT, NG, W;
+  int GT, NG, W, unit;
   int64_t cap_tiles;
 };
 
@@ -500,9 +493,10 @@ PLayout layout(const sta_paged_cache* c, const sta_paged_decode_args* a) {
   else L.GT = G > 8 ? 16 : 8;
   L.NG = (int)((G + L.GT - 1) / L.GT);
   L.cap_tiles = (c->table_width * c->page_size + kTile - 1) / kTile;
-  const int64_t most = c->batch * c->n_kv_heads * L.NG * L.cap_tiles;
-  const int per_sm = f32 ? (c->d == 128 ? 1 : 2) : paged_decode_bf16_ctas(c->d, L.GT);
-  const int64_t w = per_sm * (int64_t)sm_count();
+  L.unit = f32 ? kUnitF32 : kUnitBf16;
+  const int64_t units = (c->table_width * c->page_size + (1 << L.unit) - 1) >> L.unit;
+  const int64_t most = c->batch * c->n_kv_heads * L.NG * units;
+  const int64_t w = (f32 ? (c->d == 128 ? 1 : 2) : paged_decode_bf16_shares(c->d, L.GT)) * (int64_t)sm_count();
   L.W = (int)(most < w ? most : w);
   size_t o = 0;
   auto take = [&](size_t bytes) {
@@ -513,7 +507,7 @@ PLayout layout(const sta_paged_cache* c, const sta_paged_decode_args* a) {
   L.part = take((size_t)2 * L.W * L.GT * c->d * 4);
   L.part_ml = take((size_t)2 * L.W * L.GT * 8);
   L.ml = take((size_t)c->batch * a->n_heads * 8);
-  L.scores = a->weights_out ? take((size_t)most * L.GT * kTile * 4) : 0;
+  L.scores = a->weights_out ? take((size_t)(c->batch * c->n_kv_heads * L.NG) * L.cap_tiles * L.GT * kTile * 4) : 0;
   L.total = o + 256;
   return L;
 }
@@ -523,6 +517,8 @@ int check(const sta_paged_cache* c, const sta_paged_decode_args* a) {
   if (rc != STA_OK) return rc;
   if (!a || (c->batch > 0 && (!a->q || !a->out)) || !a->inv_freq)
     return fail(STA_ERR_ARG, "sta_paged_decode: null pointer");
+  if (reinterpret_cast<uintptr_t>(a->out) & 15u)
+    return fail(STA_ERR_ARG, "sta_paged_decode: out must start on a 16-byte boundary");
   if (a->n_heads <= 0 || a->n_heads % c->n_kv_heads)
     return fail(STA_ERR_ARG, "sta_paged_decode: n_heads must be a multiple of n_kv_heads");
   if (a->chunk_size < 0 || (a->chunk_size > 0 && (a->local_window <= 0 || a->chunk_size <= a->local_window)))
@@ -541,30 +537,30 @@ int check(const sta_paged_cache* c, const sta_paged_decode_args* a) {
 }
 
 template <int D, int GT>
-int launch_f32(const PDecP& p, int W, cudaStream_t st) {
+int launch_f32(const PDecP& p, cudaStream_t st) {
   constexpr int bytes = (int)sizeof(Smem<D, GT>);
   const cudaError_t e = cudaFuncSetAttribute(paged_decode_f32_kernel<D, GT>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(STA_ERR_CUDA, cudaGetErrorString(e));
-  paged_decode_f32_kernel<D, GT><<<W, kF32Threads, bytes, st>>>(p);
+  paged_decode_f32_kernel<D, GT><<<p.W, kF32Threads, bytes, st>>>(p);
   return STA_OK;
 }
 
 template <int D>
-int launch_f32(const PDecP& p, int W, cudaStream_t st) {
-  if (p.GT == 1) return launch_f32<D, 1>(p, W, st);
-  if (p.GT == 2) return launch_f32<D, 2>(p, W, st);
-  if (p.GT == 4) return launch_f32<D, 4>(p, W, st);
-  return launch_f32<D, 8>(p, W, st);
+int launch_f32(const PDecP& p, cudaStream_t st) {
+  if (p.GT == 1) return launch_f32<D, 1>(p, st);
+  if (p.GT == 2) return launch_f32<D, 2>(p, st);
+  if (p.GT == 4) return launch_f32<D, 4>(p, st);
+  return launch_f32<D, 8>(p, st);
 }
 
 template <typename TV>
-void launch_finish(const PDecP& p, int d, int W, cudaStream_t st) {
+void launch_finish(const PDecP& p, int d, cudaStream_t st) {
   int64_t grid = (int64_t)p.c.B * p.H;
   if (p.scores)
     grid += (int64_t)p.c.B * p.c.Hkv * ((p.c.cap + kFinish * kKeysPer - 1) / (kFinish * kKeysPer));
-  if (d == 128) paged_finish_kernel<128, TV><<<(unsigned)grid, kFinish, 0, st>>>(p, W);
-  else paged_finish_kernel<64, TV><<<(unsigned)grid, kFinish, 0, st>>>(p, W);
+  if (d == 128) paged_finish_kernel<128, TV><<<(unsigned)grid, kFinish, 0, st>>>(p);
+  else paged_finish_kernel<64, TV><<<(unsigned)grid, kFinish, 0, st>>>(p);
 }
 
 }  // namespace
@@ -581,6 +577,7 @@ int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void*
   if (c->batch == 0) return STA_OK;
   const PLayout L = layout(c, a);
   if (!ws || ws_len < L.total) return fail(STA_ERR_WORKSPACE, "sta_paged_decode: workspace too small");
+  const bool f32 = c->dtype == STA_DTYPE_F32;
   uint8_t* w = static_cast<uint8_t*>(ws);
   w += (256 - reinterpret_cast<uintptr_t>(w) % 256) % 256;
   PDecP p;
@@ -591,6 +588,12 @@ int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void*
   p.G = (int)(a->n_heads / c->n_kv_heads);
   p.NG = L.NG;
   p.GT = L.GT;
+  p.unit = L.unit;
+  p.W = L.W;
+  p.min_units = f32 ? 1 : 2;
+  p.sms = sm_count();
+  p.k16 = 16 * p.c.ksn;
+  p.v16 = 16 * p.c.vsn;
   p.inv_freq = a->inv_freq;
   p.pos_scale = a->pos_scale;
   p.qscale = (float)((double)a->sm_scale * a->rope_scale * a->rope_scale * 1.4426950408889634);
@@ -604,12 +607,11 @@ int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void*
   p.w_out = a->weights_out;
   p.err = device_error_word();
   if (!p.err) return fail(STA_ERR_CUDA, "sta_paged_decode: no device");
-  const bool f32 = c->dtype == STA_DTYPE_F32;
-  if (f32) rc = c->d == 128 ? launch_f32<128>(p, L.W, st) : launch_f32<64>(p, L.W, st);
-  else rc = launch_paged_decode_bf16(p, c->d, L.W, st);
+  if (f32) rc = c->d == 128 ? launch_f32<128>(p, st) : launch_f32<64>(p, st);
+  else rc = launch_paged_decode_bf16(p, c->d, st);
   if (rc != STA_OK) return rc;
-  if (f32) launch_finish<float>(p, c->d, L.W, st);
-  else launch_finish<__nv_bfloat16>(p, c->d, L.W, st);
+  if (f32) launch_finish<float>(p, c->d, st);
+  else launch_finish<__nv_bfloat16>(p, c->d, st);
   const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? STA_OK : fail(STA_ERR_CUDA, cudaGetErrorString(e));
 }

@@ -1,14 +1,12 @@
-// What the decode kernels of the paged cache share: the list of tiles and a CTA's place in it, the
-// rotation of a tile's query, and the parameters.
+// What the decode kernels of the paged cache share: the list of units (runs of keys) and a share's
+// place in it, the angles of the rotation, and the parameters.
 #pragma once
 
 #include "paged.cuh"
 
 namespace sta {
 
-constexpr int kTile = 64;      // keys per tile
-constexpr int kDecThreads = 128;  // 4 warps, 16 keys of a tile each
-constexpr int kDecWarps = kDecThreads / 32;
+constexpr int kTile = 64;  // keys whose query is rotated once; block of the scores buffer
 
 struct PDecP {
   PagedView c;
@@ -16,6 +14,10 @@ struct PDecP {
   int64_t qsb, qsh;  // elements
   void* out;
   int H, G, NG, GT;  // q heads, per kv head, groups of GT of them
+  int unit;          // log2 of the keys of a unit of work
+  int W, min_units;  // shares at most, units of a share at least
+  int sms;
+  int64_t k16, v16;  // bytes of 16 rows
   const float* inv_freq;
   double pos_scale;
   float qscale;      // sm_scale * rope_scale^2 * log2(e): scores are in units of log2
@@ -29,108 +31,91 @@ struct PDecP {
   int* err;
 };
 
-__device__ __forceinline__ int n_tiles(int len) { return (len + kTile - 1) / kTile; }
-
-// A CTA's place in the list of tiles.
-struct Place {
-  int b, hg, n, tiles, len;
-};
-
-__device__ __forceinline__ void seek_sequence(const PagedView& c, Place& a) {
-  a.tiles = 0;
-  while (a.b < c.B) {
-    a.len = paged_len(c, a.b);
-    a.tiles = n_tiles(a.len);
-    if (a.tiles > 0) return;
-    ++a.b;
-  }
+__device__ __forceinline__ int n_units(const PDecP& p, int len) {
+  return (int)(((uint32_t)len + (1u << p.unit) - 1u) >> p.unit);
 }
 
-__device__ __forceinline__ void step(const PDecP& p, Place& a) {
-  if (++a.n < a.tiles) return;
-  a.n = 0;
-  if (++a.hg < p.c.Hkv * p.NG) return;
-  a.hg = 0;
-  ++a.b;
-  seek_sequence(p.c, a);
-}
-
-// Number of tiles of all segments (block-wide, NT threads), and with `find` >= 0 the place of
-// tile `find`; `before` receives the tiles of the sequences before sequence `until`.
-template <int NT>
+// Units of all segments (sequence, kv head, q-head group), summed by a warp; `before` receives
+// those of the sequences before `until`.
 __device__ __forceinline__ int64_t scan_lengths(const PDecP& p, int until, int64_t* before) {
-  __shared__ int64_t s_all[NT / 32], s_bef[NT / 32];
-  const int tid = threadIdx.x;
   int64_t all = 0, bef = 0;
-  for (int b = tid; b < p.c.B; b += NT) {
-    const int t = n_tiles(paged_len(p.c, b));
+  for (int b = threadIdx.x & 31; b < p.c.B; b += 32) {
+    const int t = n_units(p, paged_len(p.c, b));
     all += t;
     if (b < until) bef += t;
   }
 #pragma unroll
   for (int o = 16; o >= 1; o >>= 1) {
     all += __shfl_xor_sync(0xffffffffu, all, o);
-    bef += __shfl_xor_sync(0xffffffffu, bef, o);
+    if (before) bef += __shfl_xor_sync(0xffffffffu, bef, o);
   }
-  if ((tid & 31) == 0) {
-    s_all[tid >> 5] = all;
-    s_bef[tid >> 5] = bef;
-  }
-  __syncthreads();
-  all = bef = 0;
-#pragma unroll
-  for (int i = 0; i < NT / 32; ++i) {
-    all += s_all[i];
-    bef += s_bef[i];
-  }
-  __syncthreads();
   const int64_t hg = (int64_t)p.c.Hkv * p.NG;
   if (before) *before = bef * hg;
   return all * hg;
 }
 
-template <int NT>
-__device__ __forceinline__ Place find_tile(const PDecP& p, int64_t t) {
-  __shared__ int s_b, s_hit;
-  __shared__ int64_t s_rest, s_sum[NT / 32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// Shares that the units are cut into: share w holds the units [total w / W, total (w + 1) / W).
+__device__ __forceinline__ int64_t n_shares(const PDecP& p, int64_t total) {
+  const int64_t w = (total + p.min_units - 1) / p.min_units;
+  return w < p.W ? w : p.W;
+}
+
+// A place in the list of units.
+struct Place {
+  int b, h, grp, n, units, len;  // sequence, kv head, q-head group, unit of the segment
+};
+
+__device__ __forceinline__ void seek_sequence(const PDecP& p, Place& a) {
+  a.units = 0;
+  while (a.b < p.c.B) {
+    a.len = paged_len(p.c, a.b);
+    a.units = n_units(p, a.len);
+    if (a.units > 0) return;
+    ++a.b;
+  }
+}
+
+__device__ __forceinline__ void step(const PDecP& p, Place& a) {
+  if (++a.n < a.units) return;
+  a.n = 0;
+  if (++a.grp < p.NG) return;
+  a.grp = 0;
+  if (++a.h < p.c.Hkv) return;
+  a.h = 0;
+  ++a.b;
+  seek_sequence(p, a);
+}
+
+// The place of unit t (t < the number of units), found by a warp.
+__device__ __forceinline__ Place find_unit(const PDecP& p, int64_t t) {
+  const int lane = threadIdx.x & 31;
   const int64_t hg = (int64_t)p.c.Hkv * p.NG;
   int64_t base = 0;
   Place a{};
-  if (tid == 0) s_hit = 0;
-  __syncthreads();
-  for (int b0 = 0; b0 < p.c.B; b0 += NT) {
-    const int b = b0 + tid;
-    const int64_t mine = b < p.c.B ? (int64_t)n_tiles(paged_len(p.c, b)) * hg : 0;
+  for (int b0 = 0; b0 < p.c.B; b0 += 32) {
+    const int b = b0 + lane;
+    const int64_t mine = b < p.c.B ? (int64_t)n_units(p, paged_len(p.c, b)) * hg : 0;
     int64_t inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += y;
     }
-    if (lane == 31) s_sum[warp] = inc;
-    __syncthreads();
-    int64_t off = base, tot = 0;
-#pragma unroll
-    for (int i = 0; i < NT / 32; ++i) {
-      if (i < warp) off += s_sum[i];
-      tot += s_sum[i];
+    const uint32_t hit = __ballot_sync(0xffffffffu, mine > 0 && t >= base + inc - mine && t < base + inc);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int64_t rest = t - __shfl_sync(0xffffffffu, base + inc - mine, src);
+      a.b = b0 + src;
+      a.len = paged_len(p.c, a.b);
+      a.units = n_units(p, a.len);
+      const int g = (int)(rest / a.units);
+      a.n = (int)(rest - (int64_t)g * a.units);
+      a.h = g / p.NG;
+      a.grp = g - a.h * p.NG;
+      return a;
     }
-    const int64_t lo = off + inc - mine;
-    if (mine > 0 && t >= lo && t < lo + mine) {
-      s_b = b;
-      s_rest = t - lo;
-      s_hit = 1;
-    }
-    __syncthreads();
-    if (s_hit) break;
-    base += tot;
+    base += __shfl_sync(0xffffffffu, inc, 31);
   }
-  a.b = s_b;
-  a.len = paged_len(p.c, a.b);
-  a.tiles = n_tiles(a.len);
-  a.hg = (int)(s_rest / a.tiles);
-  a.n = (int)(s_rest - (int64_t)a.hg * a.tiles);
   return a;
 }
 
@@ -141,8 +126,8 @@ __device__ __forceinline__ void turn(double pos, float inv_freq, float& c, float
 }
 
 // p_i - p_0 of a tile (position of the query minus that of the tile's first key)
-__device__ __forceinline__ double query_offset(const PDecP& p, int len, int n) {
-  const int i = len - 1, j0 = n * kTile;
+__device__ __forceinline__ double query_offset(const PDecP& p, int len, int tile) {
+  const int i = len - 1, j0 = tile * kTile;
   if (p.L == 0) return (double)i * p.pos_scale - (double)j0 * p.pos_scale;
   const int away = i / p.L - j0 / p.L, in = i % p.L;
   const int qp = away == 0 ? in : (away == 1 ? min(p.L + in, p.s) : min(2 * p.L - 1, p.s));
@@ -152,8 +137,10 @@ __device__ __forceinline__ double query_offset(const PDecP& p, int len, int n) {
 __device__ __forceinline__ void store_out(float* o, float x) { *o = x; }
 __device__ __forceinline__ void store_out(__nv_bfloat16* o, float x) { *o = __float2bfloat16_rn(x); }
 
-// Decode kernel for bf16 caches (tensor cores): CTAs that fit one SM, and the launch of W CTAs.
-int paged_decode_bf16_ctas(int d, int GT);
-int launch_paged_decode_bf16(const PDecP& p, int d, int W, cudaStream_t st);
+// Decode kernel for bf16 caches (tensor cores): shares per SM that it runs, keys of a unit
+// (log2), and the launch for p.W shares.
+int paged_decode_bf16_shares(int d, int GT);
+constexpr int kUnitBf16 = 4, kUnitF32 = 6;
+int launch_paged_decode_bf16(const PDecP& p, int d, cudaStream_t st);
 
 }  // namespace sta

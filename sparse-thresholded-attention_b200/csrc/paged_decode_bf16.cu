@@ -1,18 +1,20 @@
 // Decode over a paged bf16 cache on the tensor cores (schedule and rotation: paged_decode.cuh).
 //
-// One new token has few q heads per kv head, so the products are (64 keys) x (d) x (8 or 16
+// One new token has few q heads per kv head, so the products are (16 keys) x (d) x (8 or 16
 // heads): warp-level m16n8k16 with the keys as rows wastes nothing up to 8 heads, where a
-// 128-row tcgen05 tile would spend 15 of 16 rows on padding.  A warp owns 16 keys of each tile:
-//   S^T (16 keys x heads) = K (rotated) . Q^T     A = K rows (ldmatrix), B = the tile's queries
-//   O^T (d x heads)      += V^T . P^T             A = V^T (ldmatrix.trans), B = P transposed in
-//                                                 registers (movmatrix)
+// 128-row tcgen05 tile would spend 15 of 16 rows on padding.  Per 16 keys a warp forms
+//   S^T (16 keys x heads) = K (rotated) . Q^T     A = K rows, B = the tile's rotated queries
+//   O^T (d x heads)      += V^T . P^T             A = V^T, B = P transposed in registers (movmatrix)
 // Rotated keys, queries and probabilities are fp32 values carried as hi + lo bf16 pieces (four
 // products for S, two for P.V: V is exact), which leaves errors of 2^-15 (keys, whose hi piece is
 // cut instead of rounded) and 2^-16, far below the output's own rounding; running max, sums and
 // accumulators are fp32.
 //
-// The rows of two to four tiles are in flight per CTA (cp.async, 16-byte chunks swizzled by row); a
-// thread's cos / sin of the tile-local key offsets stay in registers for the whole call.
+// Every warp walks a share of its own and needs no barrier: its rows come by cp.async (16-byte
+// chunks, swizzled by row) into a ring of its own, two units of K and one of V, so that some 7 KB
+// per warp (d = 128) are in flight all the time; 12 warps per SM hide each other's latencies.  The
+// cos / sin of the 64 key offsets of a tile lie in shared memory in the order the lanes read them,
+// the queries of a tile in registers as B fragments.
 #include "mma_frag.cuh"
 #include "paged_decode.cuh"
 
@@ -20,28 +22,25 @@ namespace sta {
 
 namespace {
 
-// A tile as its producer describes it.
-struct TileInfo {
-  uint32_t b;  // sequence, and kFull / kFresh / kStart
-  int hg, n, len;
-};
-constexpr uint32_t kFull = 1u << 31;   // 64 keys, every page inside the pool
-constexpr uint32_t kFresh = 1u << 30;  // the query's angle does not follow from the tile before
-constexpr uint32_t kStart = 1u << 29;  // another segment than the tile before
-constexpr uint32_t kSeq = kStart - 1;
-// tiles after which the running angle is formed anew: it drifts by 2^-24 per tile
+// tiles after which the running angle of the query is formed anew: it drifts by 2^-24 per tile
 constexpr int kRenew = 32;
 
 template <int D, int NT>
+struct Cfg {
+  // warps of a CTA and CTAs of an SM by registers: 168 a thread for <128, 1> and <64, 2>, 255 for
+  // <128, 2>, 128 for <64, 1>
+  static constexpr int NW = D == 128 ? (NT == 1 ? 12 : 8) : (NT == 1 ? 8 : 12);
+  static constexpr int CTAS = D == 64 && NT == 1 ? 2 : 1;
+};
+
+template <int D, int NT>
 struct SmemB {
-  static constexpr int ST = D == 128 && NT == 1 ? 3 : 5;  // two CTAs per SM, one for <128, 2>
-  static constexpr int KS = D / 16;          // k steps of the score product
-  static constexpr int RING = ST + 2;
-  uint4 kv[ST][2][kTile * D / 8];            // K rows, V rows (also the flush's scratch)
-  uint4 q[2][NT][KS][32];                    // B fragments (hi b0, hi b1, lo b0, lo b1)
-  longlong2 off[2][kTile];                   // byte offsets of the K and V rows (of 8 rows each)
-  TileInfo info[RING];
-  float m[kDecWarps][8 * NT], l[kDecWarps][8 * NT];
+  static constexpr int NW = Cfg<D, NT>::NW;
+  uint4 k[NW][2][16 * D / 8];             // K rows of two units
+  uint4 v[NW][16 * D / 8];                // V rows of one
+  float4 rot[4][D / 32][4][32];           // (cos, cos, sin, sin) of two dims: unit, k step, register, lane
+  float2 ang[NW][D / 2];                  // cos / sin of the query's angle at this tile
+  int4 seg[NW][4];                        // segments entered by the loads: sequence, kv head, group, length
 };
 
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
@@ -54,6 +53,16 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+
+// C = A (16x16 bf16, row) * B (16x8 bf16, col)
+__device__ __forceinline__ void mma_bf16_first(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
+                                               uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 "
+      "{%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 
 // two fp32 values in a register pair, and the packed arithmetic on them
@@ -91,207 +100,176 @@ __device__ __forceinline__ void split_cut(f32x2 x, f32x2 minus_one, uint32_t& hi
   lo = pack_bf16(a, b);
 }
 
-// ROWS: rows that share one page lookup (8 where the page size is a multiple of 8, else 1).
-template <int D, int NT, int ROWS>
-__global__ void __launch_bounds__(kDecThreads) paged_decode_bf16_kernel(const PDecP p) {
+// Where the 16 keys of a unit lie: entry of the page table and slot in that page (of this lane's
+// row where the page size is no multiple of 16).
+struct Rows {
+  int32_t entry;
+  uint32_t slot, t;
+  bool fresh;  // another page than the unit before
+};
+
+// P16: the page size is a multiple of 16, so that 16 keys share one page.
+template <int D, int NT, bool P16>
+__global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
+    paged_decode_bf16_kernel(const PDecP p) {
   using S = SmemB<D, NT>;
-  constexpr int HALF = D / 2, CH = D / 8, ST = S::ST, KS = S::KS, MT = D / 16, GT = 8 * NT;
-  constexpr int RPP = kDecThreads / CH;            // rows that one pass of the CTA copies
-  constexpr int HP = HALF / 2;                     // frequency pairs
-  constexpr int QH = GT * HP / kDecThreads;        // heads of a thread in the query rotation
+  constexpr int HALF = D / 2, CH = D / 8, NW = Cfg<D, NT>::NW, NH = D / 32, MT = D / 16, GT = 8 * NT;
+  constexpr int FPL = D / 64;      // frequencies of a lane in the angles
+  constexpr int RPI = 32 / CH;     // rows that one copy of the warp covers
   extern __shared__ __align__(128) unsigned char smem_raw[];
   S& sm = *reinterpret_cast<S*>(smem_raw);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t total = scan_lengths<kDecThreads>(p, 0, nullptr);
-  const int64_t t0 = total * blockIdx.x / gridDim.x, t1 = total * (blockIdx.x + 1) / gridDim.x;
-  if (t0 >= t1) return;
-  const int count = (int)(t1 - t0);
-  Place oa = find_tile<kDecThreads>(p, t0);  // where the producer stands
-  int q_it = 0, l_it = 0, o_it = 0;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int fr = lane >> 2, fc = lane & 3;
 
-  // ---- page lookups of a tile, by one warp at a time (the warps take turns).  The table entry is
-  // read in lookup() and used in publish(), after the products of the tile in between.
-  constexpr int LK = kTile / ROWS / 32 > 0 ? kTile / ROWS / 32 : 1;  // lookups of a lane
-  int32_t entry[LK];
-  auto lookup = [&]() {
-    if (o_it < count && warp == (o_it & 3)) {
-#pragma unroll
-      for (int i = 0; i < LK; ++i) {
-        const int r = (lane + 32 * i) * ROWS, j = oa.n * kTile + r;
-        entry[i] = -1;
-        if (r < kTile && j < oa.len) entry[i] = __ldg(p.c.table + oa.b * p.c.ts + (uint32_t)j / p.c.page);
-      }
+  const int64_t total = scan_lengths(p, 0, nullptr);
+  const int64_t shares = n_shares(p, total), me = (int64_t)warp * gridDim.x + blockIdx.x;
+  int count = 0;
+  Place nx{};                       // the unit whose K rows are loaded next
+  Rows rows{-1, 0, 0, true};
+  if (me < shares) {
+    const int64_t t0 = total * me / shares;
+    count = (int)(total * (me + 1) / shares - t0);
+    nx = find_unit(p, t0);
+  }
+  int segs = 0, k_it = 0;           // segments entered, units whose K rows are loaded
+  int n = nx.n;                     // the unit in hand, of its segment
+
+  // ---- page lookup of unit nx
+  auto lookup = [&](bool first) {
+    if (first || nx.n == 0) {
+      if (lane == 0) sm.seg[warp][segs & 3] = make_int4(nx.b, nx.h, nx.grp, nx.len);
+      ++segs;
     }
-  };
-  auto publish = [&]() {
-    if (o_it < count) {
-      if (warp == (o_it & 3)) {
-        bool good = true;
-#pragma unroll
-        for (int i = 0; i < LK; ++i) {
-          const int r = (lane + 32 * i) * ROWS;
-          const uint32_t j = (uint32_t)(oa.n * kTile + r);
-          if (r < kTile) {
-            longlong2 o = make_longlong2(-1, -1);  // no row
-            if (j < (uint32_t)oa.len) {
-              if (entry[i] < 0 || entry[i] >= p.c.n_pages) {
-                o.x = -2;  // a page outside the pool
-                good = false;
-                atomicCAS(p.err, 0, kErrPageDecode);
-              } else {
-                const int64_t slot = j % p.c.page, h = oa.hg / p.NG;
-                o = make_longlong2(entry[i] * p.c.ksp + h * p.c.ksh + slot * p.c.ksn,
-                                   entry[i] * p.c.vsp + h * p.c.vsh + slot * p.c.vsn);
-              }
-            }
-            sm.off[o_it & 1][r / ROWS] = o;
-          }
-        }
-        good = __all_sync(0xffffffffu, good);
-        if (lane == 0) {
-          TileInfo t;
-          t.b = (uint32_t)oa.b;
-          if (good && oa.len - oa.n * kTile >= kTile) t.b |= kFull;
-          if (oa.n == 0 || o_it == 0) t.b |= kStart;
-          if (oa.n % kRenew == 0 || o_it == 0 || (p.L > 0 && oa.n * kTile % p.L == 0)) t.b |= kFresh;
-          t.hg = oa.hg;
-          t.n = oa.n;
-          t.len = oa.len;
-          sm.info[o_it % S::RING] = t;
+    if (P16) {
+      rows.fresh = true;
+      if (first || nx.n == 0) {
+        const uint32_t j = (uint32_t)nx.n * 16;
+        rows.t = j / p.c.page;
+        rows.slot = j - rows.t * p.c.page;
+      } else {
+        rows.slot += 16;
+        rows.fresh = rows.slot == p.c.page;
+        if (rows.fresh) {
+          rows.slot = 0;
+          ++rows.t;
         }
       }
-      step(p, oa);
+      if (rows.fresh) rows.entry = __ldg(p.c.table + nx.b * p.c.ts + rows.t);
+    } else {
+      const uint32_t j = (uint32_t)nx.n * 16 + (lane & 15);
+      const uint32_t t = j / p.c.page;
+      rows.slot = j - t * p.c.page;
+      rows.entry = j < (uint32_t)nx.len ? __ldg(p.c.table + nx.b * p.c.ts + t) : -1;
     }
-    ++o_it;
   };
-  // ---- copies of a tile's rows (rows without data are zero; of a bad page, K is NaN)
-  const int lch = tid % CH, lrow = tid / CH;
-  const int ldst = lrow * CH + (lch ^ (lrow & 7));  // 16-byte chunk in the stage, first pass
-  const int64_t kthr = (lrow % ROWS) * p.c.ksn + lch * 16, vthr = (lrow % ROWS) * p.c.vsn + lch * 16;
-  auto loads = [&]() {
-    if (l_it < count) {
-      uint4* ks = sm.kv[l_it % ST][0];
-      uint4* vs = sm.kv[l_it % ST][1];
-      const TileInfo t = sm.info[l_it % S::RING];
-      if (t.b & kFull) {
+  // ---- copies.  Rows without data are zero; of a bad page, K is NaN.
+  const int lch = lane % CH, lrow = lane / CH;
+  const uint32_t ring_k = smem_u32(sm.k[warp][0]), ring_v = smem_u32(sm.v[warp]);
+  const uint32_t dst0 = (uint32_t)lrow * (D * 2);
+  const char *kbase = p.c.k, *vbase = p.c.v, *vnext = p.c.v;  // P16: this lane's first row
+  int64_t koff = 0, voff = 0, vonext = 0;  // otherwise: of row (lane & 15); -1: no row, -2: bad page
+  int left = 0, vleft = 0;                 // keys of the unit from its first on; 0: a bad page
+  auto copy = [&](uint32_t ring, const char* base, const char* pool, int64_t off, int64_t stride, int rest) {
 #pragma unroll
-        for (int i = 0; i < kTile / RPP; ++i) {
-          const longlong2 o = sm.off[l_it & 1][(lrow + i * RPP) / ROWS];
-          cp_async16(ks + ldst + i * RPP * CH, p.c.k + (o.x + kthr), 16);
-          cp_async16(vs + ldst + i * RPP * CH, p.c.v + (o.y + vthr), 16);
+    for (int i = 0; i < 16 / RPI; ++i) {
+      const uint32_t dst = ring + dst0 + i * (RPI * D * 2) + ((lch ^ ((lrow + RPI * i) & 7)) << 4);
+      if (P16) {
+        if (rest >= 16) {
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(base + i * RPI * stride)
+                       : "memory");
+        } else {
+          const bool in = lrow + RPI * i < rest;
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n"
+                       ::"r"(dst), "l"(in ? base + i * RPI * stride : pool), "r"(in ? 16 : 0) : "memory");
         }
       } else {
-        const int valid = t.len - t.n * kTile;
-        for (int i = 0; i < kTile / RPP; ++i) {
-          const int row = lrow + i * RPP, dst = ldst + i * RPP * CH;
-          const longlong2 o = sm.off[l_it & 1][row / ROWS];
-          const bool in = row < valid && o.x >= 0;
-          cp_async16(vs + dst, p.c.v + (in ? o.y + vthr : 0), in ? 16 : 0);
-          if (row < valid && o.x == -2) {
-            ks[dst] = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
-          } else {
-            cp_async16(ks + dst, p.c.k + (in ? o.x + kthr : 0), in ? 16 : 0);
-          }
+        const int64_t o = __shfl_sync(0xffffffffu, off, lrow + RPI * i);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n"
+                     ::"r"(dst), "l"(o >= 0 ? pool + (o + lch * 16) : pool), "r"(o >= 0 ? 16 : 0) : "memory");
+      }
+    }
+  };
+  auto load_k = [&]() {  // unit nx; its V rows follow one unit later
+    if (k_it < count) {
+      bool bad = false;
+      if (P16) {
+        if (rows.fresh) {
+          const bool ok = rows.entry >= 0 && rows.entry < p.c.n_pages;
+          const int64_t pg = ok ? rows.entry : 0;
+          kbase = p.c.k + (lrow + rows.slot) * p.c.ksn + lch * 16 + nx.h * p.c.ksh + pg * p.c.ksp;
+          vbase = p.c.v + (lrow + rows.slot) * p.c.vsn + lch * 16 + nx.h * p.c.vsh + pg * p.c.vsp;
+          left = ok ? 16 : 0;
+        } else {
+          kbase += p.k16;
+          vbase += p.v16;
         }
+        bad = left == 0;
+        vnext = vbase;
+        vleft = bad ? 0 : nx.len - nx.n * 16;
+        copy(ring_k + (k_it & 1) * (D * 32), kbase, p.c.k, 0, p.c.ksn, vleft);
+      } else {
+        const bool in = nx.n * 16 + (lane & 15) < nx.len;
+        const bool ok = rows.entry >= 0 && rows.entry < p.c.n_pages;
+        koff = in && ok ? rows.entry * p.c.ksp + nx.h * p.c.ksh + rows.slot * p.c.ksn : -1;
+        vonext = in && ok ? rows.entry * p.c.vsp + nx.h * p.c.vsh + rows.slot * p.c.vsn : -1;
+        bad = __any_sync(0xffffffffu, in && !ok);
+        copy(ring_k + (k_it & 1) * (D * 32), nullptr, p.c.k, koff, 0, 16);
+      }
+      if (bad) {  // the whole unit: every output of the sequence is NaN
+        asm volatile("cp.async.wait_all;\n" ::: "memory");
+        if (lane == 0) atomicCAS(p.err, 0, kErrPageDecode);
+        for (int i = lane; i < 16 * CH; i += 32)
+          sm.k[warp][k_it & 1][i] = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+      }
+      if (k_it + 1 < count) {
+        step(p, nx);
+        lookup(false);
       }
     }
     asm volatile("cp.async.commit_group;\n" ::: "memory");
-    ++l_it;
+    ++k_it;
   };
-  // ---- queries of a tile: rotated by p_i - p_0, stored as B fragments.  From tile to tile of a
-  // segment the angle moves by a constant step.
-  const int qf = 2 * (tid % HP), qg = tid / HP;  // frequencies qf, qf + 1; heads qg + i * (128 / HP)
-  float q1[QH][2], q2[QH][2], qc[2], qs[2], dc[2], ds[2];
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    turn(-(double)kTile * (p.L > 0 ? 1.0 : p.pos_scale), __ldg(p.inv_freq + qf + e), dc[e], ds[e]);
-    qc[e] = 1.f;
-    qs[e] = 0.f;
-  }
-  auto queries = [&]() {
-    if (q_it < count) {
-      const TileInfo t = sm.info[q_it % S::RING];
-      if (t.b & kStart) {
-        const int gbase = (t.hg % p.NG) * GT, h0 = (t.hg / p.NG) * p.G + gbase;
-#pragma unroll
-        for (int i = 0; i < QH; ++i) {
-          const int g = qg + i * (kDecThreads / HP);
-          const bool in = gbase + g < p.G;
-          const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.q) +
-                                     (int64_t)(t.b & kSeq) * p.qsb + (h0 + g) * p.qsh + qf;
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            q1[i][e] = in ? __bfloat162float(src[e]) * p.qscale : 0.f;
-            q2[i][e] = in ? __bfloat162float(src[e + HALF]) * p.qscale : 0.f;
-          }
-        }
-      }
-      if (t.b & kFresh) {
-        const double at = query_offset(p, t.len, t.n);
-        turn(at, __ldg(p.inv_freq + qf), qc[0], qs[0]);
-        turn(at, __ldg(p.inv_freq + qf + 1), qc[1], qs[1]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float c = qc[e] * dc[e] - qs[e] * ds[e];
-          qs[e] = qs[e] * dc[e] + qc[e] * ds[e];
-          qc[e] = c;
-        }
-      }
-      const int ks = qf / 16, reg = (qf % 16) / 8, fc = (qf % 8) / 2;
-#pragma unroll
-      for (int i = 0; i < QH; ++i) {
-        const int g = qg + i * (kDecThreads / HP);
-        float r1[2], r2[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          r1[e] = q1[i][e] * qc[e] - q2[i][e] * qs[e];
-          r2[e] = q2[i][e] * qc[e] + q1[i][e] * qs[e];
-        }
-        uint32_t hi, lo;
-        pack_split(r1[0], r1[1], hi, lo);
-        uint32_t* d = reinterpret_cast<uint32_t*>(&sm.q[q_it & 1][g / 8][ks][(g % 8) * 4 + fc]);
-        d[reg] = hi;
-        d[2 + reg] = lo;
-        pack_split(r2[0], r2[1], hi, lo);
-        d += KS / 2 * 32 * 4;
-        d[reg] = hi;
-        d[2 + reg] = lo;
-      }
-    }
-    ++q_it;
+  auto load_v = [&](int it, const char* base, int64_t off, int rest) {
+    if (it < count) copy(ring_v, base, p.c.v, off, p.c.vsn, rest);
+    asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
 
-#pragma unroll
-  for (int i = 0; i < ST - 1; ++i) {
-    lookup();
-    publish();
-    __syncthreads();
-    loads();
+  const char* vcur = p.c.v;   // the V rows that follow next
+  int64_t vocur = 0;
+  int vlcur = 0;
+  if (count > 0) {
+    lookup(true);
+    load_k();
+    vcur = vnext; vocur = vonext; vlcur = vleft;
+    load_v(0, vcur, vocur, vlcur);
+    load_k();
+    vcur = vnext; vocur = vonext; vlcur = vleft;
   }
-  lookup();
-  publish();
-  queries();
-  // cos / sin of this thread's key offsets, in the order of its A fragment's elements
-  const int fr = lane >> 2, fc = lane & 3;
-  f32x2 rc[KS / 2][4], rs[KS / 2][4], rn[KS / 2][4];  // cos, sin, -sin
+  // ---- cos / sin of the key offsets t * pos_scale, t = 0 .. 63, by all warps
+  for (int i = threadIdx.x; i < 4 * NH * 4 * 32; i += NW * 32) {
+    const int l = i & 31, r = (i >> 5) & 3, ks = (i >> 7) % NH, u = i / (128 * NH);
+    const int t = u * 16 + (l >> 2) + (r & 1) * 8, f = ks * 16 + (l & 3) * 2 + (r >> 1) * 8;
+    float4 x;
+    turn((double)t * p.pos_scale, __ldg(p.inv_freq + f), x.x, x.z);
+    turn((double)t * p.pos_scale, __ldg(p.inv_freq + f + 1), x.y, x.w);
+    sm.rot[u][ks][r][l] = x;
+  }
+  __syncthreads();
+  if (count == 0) return;
+
+  // ---- the query's angle at a tile, this lane's frequencies; it moves by a constant from tile to
+  // tile of a segment (of a chunk)
+  float ac[FPL], as[FPL], dc[FPL], ds[FPL];
+#pragma unroll
+  for (int e = 0; e < FPL; ++e) {
+    turn(-(double)kTile * p.pos_scale, __ldg(p.inv_freq + lane * FPL + e), dc[e], ds[e]);
+    ac[e] = as[e] = 0.f;
+  }
+  uint32_t qb[NT][2 * NH][4];      // B fragments of a k step: hi b0, hi b1, lo b0, lo b1
   const f32x2 minus_one = pair(-1.f, -1.f);
-#pragma unroll
-  for (int ks = 0; ks < KS / 2; ++ks)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int t = warp * 16 + fr + (r & 1) * 8, f = ks * 16 + fc * 2 + (r >> 1) * 8;
-      const double at = (double)t * (p.L > 0 ? 1.0 : p.pos_scale);
-      float c[2], s[2];
-      turn(at, __ldg(p.inv_freq + f), c[0], s[0]);
-      turn(at, __ldg(p.inv_freq + f + 1), c[1], s[1]);
-      rc[ks][r] = pair(c[0], c[1]);
-      rs[ks][r] = pair(s[0], s[1]);
-      rn[ks][r] = pair(-s[0], -s[1]);
-    }
 
   float acc[NT][MT][4];
-  float mx[NT][2], mref[NT][2], sum[NT][2];  // of heads 8 nt + 2 fc + {0, 1}; sums of this thread's keys
+  float mx[NT][2], mref[NT][2], sum[NT][2];  // of heads 8 nt + 2 fc + {0, 1}; sums of this lane's keys
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -301,72 +279,126 @@ __global__ void __launch_bounds__(kDecThreads) paged_decode_bf16_kernel(const PD
     mx[nt][0] = mx[nt][1] = -INFINITY;
     mref[nt][0] = mref[nt][1] = sum[nt][0] = sum[nt][1] = 0.f;
   }
-  // ldmatrix lane addresses inside a stage (bytes)
-  const uint32_t k_row = (uint32_t)(warp * 16 + (lane & 15)) * (D * 2), sw = lane & 7;
-  const uint32_t v_row = (uint32_t)(warp * 16 + (lane & 7) + ((lane >> 4) << 3)) * (D * 2);
+  // ldmatrix lane addresses inside a unit (bytes)
+  const uint32_t k_row = (uint32_t)(lane & 15) * (D * 2), sw = lane & 7;
+  const uint32_t v_row = (uint32_t)((lane & 7) + ((lane >> 4) << 3)) * (D * 2);
 
+  int seg = -1, len = 0;           // the segment in hand and its length
+  bool fresh_seg = true;
+#pragma unroll 1
   for (int it = 0; it < count; ++it) {
-    asm volatile("cp.async.wait_group %0;\n" ::"n"(ST - 2) : "memory");
-    __syncthreads();
-    loads();
-    lookup();
-    const TileInfo cur = sm.info[it % S::RING];
-    const int cur_b = (int)(cur.b & kSeq);
-    const uint32_t kb = smem_u32(sm.kv[it % ST][0]), vb = smem_u32(sm.kv[it % ST][1]);
+    asm volatile("cp.async.wait_group 2;\n" ::: "memory");
+    __syncwarp();
+    if (fresh_seg) {
+      ++seg;
+      len = sm.seg[warp][seg & 3].w;
+    }
+    // ---- queries, once per tile
+    if (it == 0 || (n & 3) == 0) {
+      const int4 at = sm.seg[warp][seg & 3];
+      const int tile = n >> 2;
+      if (it == 0 || tile % kRenew == 0 || (p.L > 0 && tile * kTile % p.L == 0)) {
+        const double x = query_offset(p, len, tile);
+#pragma unroll
+        for (int e = 0; e < FPL; ++e) turn(x, __ldg(p.inv_freq + lane * FPL + e), ac[e], as[e]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < FPL; ++e) {
+          const float c = ac[e] * dc[e] - as[e] * ds[e];
+          as[e] = as[e] * dc[e] + ac[e] * ds[e];
+          ac[e] = c;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < FPL; ++e) sm.ang[warp][lane * FPL + e] = make_float2(ac[e], as[e]);
+      __syncwarp();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const int g = at.z * GT + nt * 8 + fr;
+        const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.q) + at.x * p.qsb +
+                                   (at.y * p.G + g) * p.qsh + fc * 2;
+#pragma unroll
+        for (int ks = 0; ks < NH; ++ks)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int d = ks * 16 + b * 8;
+            const float4 cs = *reinterpret_cast<const float4*>(&sm.ang[warp][d + fc * 2]);
+            float x1[2] = {0.f, 0.f}, x2[2] = {0.f, 0.f};
+            if (g < p.G) {
+#pragma unroll
+              for (int e = 0; e < 2; ++e) {
+                x1[e] = __bfloat162float(src[d + e]) * p.qscale;
+                x2[e] = __bfloat162float(src[d + e + HALF]) * p.qscale;
+              }
+            }
+            pack_split(x1[0] * cs.x - x2[0] * cs.y, x1[1] * cs.z - x2[1] * cs.w, qb[nt][ks][b], qb[nt][ks][2 + b]);
+            pack_split(x2[0] * cs.x + x1[0] * cs.y, x2[1] * cs.z + x1[1] * cs.w, qb[nt][ks + NH][b],
+                       qb[nt][ks + NH][2 + b]);
+          }
+      }
+      __syncwarp();
+    }
     // ---- S^T
-    float sc[NT][4][4];
+    float sc[NT][2][4];
+    const float4* rot = &sm.rot[n & 3][0][0][lane];
+    const uint32_t kb = ring_k + (it & 1) * (D * 32) + k_row;
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) sc[nt][i][x] = 0.f;
-#pragma unroll
-    for (int ks = 0; ks < KS / 2; ++ks) {
+    for (int ks = 0; ks < NH; ++ks) {
       uint32_t a[4], b[4], ah[4], al[4], bh[4], bl[4];
       const uint32_t ch = 2 * ks + (lane >> 4);
-      ldsm_x4(kb + k_row + ((ch ^ sw) << 4), a[0], a[1], a[2], a[3]);
-      ldsm_x4(kb + k_row + (((ch + CH / 2) ^ sw) << 4), b[0], b[1], b[2], b[3]);
+      ldsm_x4(kb + ((ch ^ sw) << 4), a[0], a[1], a[2], a[3]);
+      ldsm_x4(kb + (((ch + CH / 2) ^ sw) << 4), b[0], b[1], b[2], b[3]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const f32x2 x1 = widen(a[r]), x2 = widen(b[r]);
-        split_cut(fma2(x2, rn[ks][r], mul2(x1, rc[ks][r])), minus_one, ah[r], al[r]);
-        split_cut(fma2(x1, rs[ks][r], mul2(x2, rc[ks][r])), minus_one, bh[r], bl[r]);
+        const float4 cs = rot[(ks * 4 + r) * 32];
+        const f32x2 c = pair(cs.x, cs.y), s = pair(cs.z, cs.w);
+        split_cut(fma2(mul2(x2, s), minus_one, mul2(x1, c)), minus_one, ah[r], al[r]);
+        split_cut(fma2(x1, s, mul2(x2, c)), minus_one, bh[r], bl[r]);
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        const uint4 qa4 = sm.q[it & 1][nt][ks][lane], qb4 = sm.q[it & 1][nt][ks + KS / 2][lane];
-        mma_bf16(sc[nt][0], ah, qa4.x, qa4.y);
-        mma_bf16(sc[nt][1], ah, qa4.z, qa4.w);
-        mma_bf16(sc[nt][2], al, qa4.x, qa4.y);
-        mma_bf16(sc[nt][3], al, qa4.z, qa4.w);
-        mma_bf16(sc[nt][0], bh, qb4.x, qb4.y);
-        mma_bf16(sc[nt][1], bh, qb4.z, qb4.w);
-        mma_bf16(sc[nt][2], bl, qb4.x, qb4.y);
-        mma_bf16(sc[nt][3], bl, qb4.z, qb4.w);
+        const uint32_t(&qa)[4] = qb[nt][ks];
+        const uint32_t(&qc)[4] = qb[nt][ks + NH];
+        if (ks == 0) {
+          mma_bf16_first(sc[nt][0], ah, qa[0], qa[1]);
+          mma_bf16_first(sc[nt][1], ah, qa[2], qa[3]);
+        } else {
+          mma_bf16(sc[nt][0], ah, qa[0], qa[1]);
+          mma_bf16(sc[nt][1], ah, qa[2], qa[3]);
+        }
+        mma_bf16(sc[nt][0], al, qa[0], qa[1]);
+        mma_bf16(sc[nt][1], al, qa[2], qa[3]);
+        mma_bf16(sc[nt][0], bh, qc[0], qc[1]);
+        mma_bf16(sc[nt][1], bh, qc[2], qc[3]);
+        mma_bf16(sc[nt][0], bl, qc[0], qc[1]);
+        mma_bf16(sc[nt][1], bl, qc[2], qc[3]);
       }
     }
-    // ---- online softmax over this warp's 16 keys (rows fr and fr + 8 of the fragment)
+    // ---- the K rows of the unit after the next, into the place just read
+    __syncwarp();
+    load_k();
+    // ---- online softmax over the 16 keys
     uint32_t ph[NT][2], pl[NT][2];
     bool grow = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int x = 0; x < 4; ++x)
-        sc[nt][0][x] = sc[nt][0][x] + ((sc[nt][1][x] + sc[nt][2][x]) + sc[nt][3][x]);
-    if (!(cur.b & kFull)) {
-      const int left = cur.len - cur.n * kTile - warp * 16 - fr;
+        sc[nt][0][x] += sc[nt][1][x];
+    if (n * 16 + 16 > len) {
+      const int rest = len - n * 16 - fr;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int x = 0; x < 4; ++x)
-          if ((x < 2 ? 0 : 8) >= left) sc[nt][0][x] = -INFINITY;
+          if ((x < 2 ? 0 : 8) >= rest) sc[nt][0][x] = -INFINITY;
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int c = 0; c < 2; ++c) grow |= fmaxf(sc[nt][0][c], sc[nt][0][c + 2]) > mx[nt][c];
-    if (__any_sync(0xffffffffu, grow)) {  // rare after the first tiles of a segment
+    if (__any_sync(0xffffffffu, grow)) {  // rare after the first units of a segment
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -387,14 +419,15 @@ __global__ void __launch_bounds__(kDecThreads) paged_decode_bf16_kernel(const PD
         }
     }
     if (p.scores) {
-      float* out = p.scores +
-          (((int64_t)cur_b * p.c.Hkv * p.NG + cur.hg) * p.cap_tiles + cur.n) * GT * kTile + warp * 16 + fr;
+      const int4 at = sm.seg[warp][seg & 3];
+      float* out = p.scores + ((((int64_t)at.x * p.c.Hkv + at.y) * p.NG + at.z) * p.cap_tiles + (n >> 2)) *
+                                  GT * kTile + (n & 3) * 16 + fr;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
           const int g = nt * 8 + fc * 2 + (x & 1);
-          if ((cur.hg % p.NG) * GT + g < p.G) out[g * kTile + (x >> 1) * 8] = sc[nt][0][x];
+          if (at.z * GT + g < p.G) out[g * kTile + (x >> 1) * 8] = sc[nt][0][x];
         }
     }
 #pragma unroll
@@ -414,22 +447,31 @@ __global__ void __launch_bounds__(kDecThreads) paged_decode_bf16_kernel(const PD
       }
     }
     // ---- O^T += V^T . P^T
+    asm volatile("cp.async.wait_group 1;\n" ::: "memory");
+    __syncwarp();
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       uint32_t a[4];
       const uint32_t ch = 2 * mt + ((lane >> 3) & 1);
-      ldsm_x4_t(vb + v_row + ((ch ^ sw) << 4), a[0], a[1], a[2], a[3]);
+      ldsm_x4_t(ring_v + v_row + ((ch ^ sw) << 4), a[0], a[1], a[2], a[3]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         mma_bf16(acc[nt][mt], a, ph[nt][0], ph[nt][1]);
         mma_bf16(acc[nt][mt], a, pl[nt][0], pl[nt][1]);
       }
     }
-    const bool seg_end = cur.n == n_tiles(cur.len) - 1;
-    if (seg_end || it == count - 1) {
-      // the warps' partial results of this segment, joined (in the stage just used) and stored
-      float* part_acc = reinterpret_cast<float*>(sm.kv[it % ST][0]);  // [warp][head][d]
-      __syncthreads();
+    __syncwarp();
+    load_v(it + 1, vcur, vocur, vlcur);
+    vcur = vnext;
+    vocur = vonext;
+    vlcur = vleft;
+    fresh_seg = n * 16 + 16 >= len;
+    if (fresh_seg || it + 1 == count) {
+      // the share's part of this segment: the result itself, or a partial
+      const int4 at = sm.seg[warp][seg & 3];
+      const bool started = n <= it;  // the segment's first unit lies in this share
+      const bool whole = fresh_seg && started;
+      const int64_t slot = 2 * me + (started ? 1 : 0);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -438,74 +480,64 @@ __global__ void __launch_bounds__(kDecThreads) paged_decode_bf16_kernel(const PD
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
           const int g = nt * 8 + fc * 2 + c;
-          if (fr == 0) {
-            sm.m[warp][g] = mx[nt][c];
-            sm.l[warp][g] = l;
+          if (at.z * GT + g < p.G) {
+            const int64_t head = (int64_t)at.x * p.H + at.y * p.G + at.z * GT + g;
+            if (whole) {
+              __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out) + head * D + fr;
+              const float f = 1.f / l;
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                out[mt * 16] = __float2bfloat16_rn(acc[nt][mt][c] * f);
+                out[mt * 16 + 8] = __float2bfloat16_rn(acc[nt][mt][c + 2] * f);
+              }
+              if (fr == 0) p.ml[head] = make_float2(mref[nt][c], f);
+            } else {
+              float* part = p.part + (slot * GT + g) * D + fr;
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt) {
+                part[mt * 16] = acc[nt][mt][c];
+                part[mt * 16 + 8] = acc[nt][mt][c + 2];
+              }
+              if (fr == 0) p.part_ml[slot * GT + g] = make_float2(mx[nt][c], l);
+            }
           }
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            part_acc[(warp * GT + g) * D + mt * 16 + fr] = acc[nt][mt][c];
-            part_acc[(warp * GT + g) * D + mt * 16 + fr + 8] = acc[nt][mt][c + 2];
-            acc[nt][mt][c] = acc[nt][mt][c + 2] = 0.f;
-          }
+          for (int mt = 0; mt < MT; ++mt) acc[nt][mt][c] = acc[nt][mt][c + 2] = 0.f;
           mx[nt][c] = -INFINITY;
           mref[nt][c] = sum[nt][c] = 0.f;
         }
-      __syncthreads();
-      const bool started = cur.n <= it;  // the segment's first tile lies in this share
-      const bool whole = seg_end && started;
-      const int slot = 2 * blockIdx.x + (started ? 1 : 0);
-      const int gbase = (cur.hg % p.NG) * GT, h0 = (cur.hg / p.NG) * p.G + gbase;
-      const int heads = min(GT, p.G - gbase);
-      for (int i = tid; i < heads * D; i += kDecThreads) {
-        const int g = i / D, d = i % D;
-        float M = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) M = fmaxf(M, sm.m[w][g]);
-        const float ms = M == -INFINITY ? 0.f : M;
-        float L = 0.f, o = 0.f;
-#pragma unroll
-        for (int w = 0; w < kDecWarps; ++w) {
-          const float f = exp2f(sm.m[w][g] - ms);
-          L += sm.l[w][g] * f;
-          o += part_acc[(w * GT + g) * D + d] * f;
-        }
-        if (whole) {
-          store_out(static_cast<__nv_bfloat16*>(p.out) + ((int64_t)cur_b * p.H + h0 + g) * D + d, o / L);
-          if (d == 0) p.ml[(int64_t)cur_b * p.H + h0 + g] = make_float2(ms, 1.f / L);
-        } else {
-          p.part[((int64_t)slot * GT + g) * D + d] = o;
-          if (d == 0) p.part_ml[(int64_t)slot * GT + g] = make_float2(M, L);
-        }
-      }
     }
-    publish();
-    queries();
+    n = fresh_seg ? 0 : n + 1;
   }
 }
 
-template <int D, int NT, int ROWS>
-int launch(const PDecP& p, int W, cudaStream_t st) {
-  constexpr int bytes = (int)sizeof(SmemB<D, NT>);
-  const cudaError_t e = cudaFuncSetAttribute(paged_decode_bf16_kernel<D, NT, ROWS>,
+template <int D, int NT, bool P16>
+int launch(const PDecP& p, cudaStream_t st) {
+  constexpr int bytes = (int)sizeof(SmemB<D, NT>), NW = Cfg<D, NT>::NW;
+  const cudaError_t e = cudaFuncSetAttribute(paged_decode_bf16_kernel<D, NT, P16>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(STA_ERR_CUDA, cudaGetErrorString(e));
-  paged_decode_bf16_kernel<D, NT, ROWS><<<W, kDecThreads, bytes, st>>>(p);
+  // shares go to the CTAs in turn, so few shares spread over the SMs
+  const int grid = p.W < p.sms * Cfg<D, NT>::CTAS ? p.W : p.sms * Cfg<D, NT>::CTAS;
+  paged_decode_bf16_kernel<D, NT, P16><<<grid, NW * 32, bytes, st>>>(p);
   return STA_OK;
 }
 
 template <int D, int NT>
-int launch(const PDecP& p, int W, cudaStream_t st) {
-  return p.c.page % 8 == 0 ? launch<D, NT, 8>(p, W, st) : launch<D, NT, 1>(p, W, st);
+int launch(const PDecP& p, cudaStream_t st) {
+  return p.c.page % 16 == 0 ? launch<D, NT, true>(p, st) : launch<D, NT, false>(p, st);
 }
 
 }  // namespace
 
-int paged_decode_bf16_ctas(int d, int GT) { return d == 128 && GT == 16 ? 1 : 2; }
+int paged_decode_bf16_shares(int d, int GT) {
+  if (d == 128) return GT == 8 ? Cfg<128, 1>::NW * Cfg<128, 1>::CTAS : Cfg<128, 2>::NW * Cfg<128, 2>::CTAS;
+  return GT == 8 ? Cfg<64, 1>::NW * Cfg<64, 1>::CTAS : Cfg<64, 2>::NW * Cfg<64, 2>::CTAS;
+}
 
-int launch_paged_decode_bf16(const PDecP& p, int d, int W, cudaStream_t st) {
-  if (d == 128) return p.GT == 8 ? launch<128, 1>(p, W, st) : launch<128, 2>(p, W, st);
-  return p.GT == 8 ? launch<64, 1>(p, W, st) : launch<64, 2>(p, W, st);
+int launch_paged_decode_bf16(const PDecP& p, int d, cudaStream_t st) {
+  if (d == 128) return p.GT == 8 ? launch<128, 1>(p, st) : launch<128, 2>(p, st);
+  return p.GT == 8 ? launch<64, 1>(p, st) : launch<64, 2>(p, st);
 }
 
 }  // namespace sta
