@@ -39,7 +39,8 @@ struct SmemB {
   uint4 k[NW][2][16 * D / 8];             // K rows of two units
   uint4 v[NW][16 * D / 8];                // V rows of one
   float4 rot[4][D / 32][4][32];           // (cos, cos, sin, sin) of two dims: unit, k step, register, lane
-  float2 ang[NW][D / 2];                  // cos / sin of the query's angle at this tile
+  float4 ang[NW][D / 4];                  // (cos, cos, sin, sin) of the query's angle, two dims, times the scale
+  uint4 q[NW][NT][D / 32][32];            // a lane's raw queries of a k step: dims 0, 8, d/2, d/2 + 8 on, two each
   int4 seg[NW][4];                        // segments entered by the loads: sequence, kv head, group, length
 };
 
@@ -100,6 +101,15 @@ __device__ __forceinline__ void split_cut(f32x2 x, f32x2 minus_one, uint32_t& hi
   lo = pack_bf16(a, b);
 }
 
+// both pieces rounded
+__device__ __forceinline__ void split_round(f32x2 x, f32x2 minus_one, uint32_t& hi, uint32_t& lo) {
+  float a, b;
+  unpair(x, a, b);
+  hi = pack_bf16(a, b);
+  unpair(fma2(widen(hi), minus_one, x), a, b);
+  lo = pack_bf16(a, b);
+}
+
 // Where the 16 keys of a unit lie: entry of the page table and slot in that page (of this lane's
 // row where the page size is no multiple of 16).
 struct Rows {
@@ -108,14 +118,18 @@ struct Rows {
   bool fresh;  // another page than the unit before
 };
 
-// P16: the page size is a multiple of 16, so that 16 keys share one page.
-template <int D, int NT, bool P16>
+// How a unit's 16 rows lie: anywhere; in one page (its size is a multiple of 16); in one page,
+// one behind the other.
+enum RowMode { kAnyRows, kPageRows, kDenseRows };
+
+template <int D, int NT, RowMode MODE>
 __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
     paged_decode_bf16_kernel(const PDecP p) {
   using S = SmemB<D, NT>;
   constexpr int HALF = D / 2, CH = D / 8, NW = Cfg<D, NT>::NW, NH = D / 32, MT = D / 16, GT = 8 * NT;
   constexpr int FPL = D / 64;      // frequencies of a lane in the angles
   constexpr int RPI = 32 / CH;     // rows that one copy of the warp covers
+  constexpr bool P16 = MODE != kAnyRows;
   extern __shared__ __align__(128) unsigned char smem_raw[];
   S& sm = *reinterpret_cast<S*>(smem_raw);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -165,27 +179,38 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
   // ---- copies.  Rows without data are zero; of a bad page, K is NaN.
   const int lch = lane % CH, lrow = lane / CH;
   const uint32_t ring_k = smem_u32(sm.k[warp][0]), ring_v = smem_u32(sm.v[warp]);
-  const uint32_t dst0 = (uint32_t)lrow * (D * 2);
+  uint32_t dst0[8 / RPI];  // this lane's chunk of the first 8 rows, chunks swizzled by row
+#pragma unroll
+  for (int i = 0; i < 8 / RPI; ++i) {
+    const int row = lrow + RPI * i;
+    dst0[i] = (uint32_t)(row * (D * 2) + ((lch ^ row) << 4));
+  }
   const char *kbase = p.c.k, *vbase = p.c.v, *vnext = p.c.v;  // P16: this lane's first row
   int64_t koff = 0, voff = 0, vonext = 0;  // otherwise: of row (lane & 15); -1: no row, -2: bad page
   int left = 0, vleft = 0;                 // keys of the unit from its first on; 0: a bad page
   auto copy = [&](uint32_t ring, const char* base, const char* pool, int64_t off, int64_t stride, int rest) {
+    uint32_t to[8 / RPI];
 #pragma unroll
-    for (int i = 0; i < 16 / RPI; ++i) {
-      const uint32_t dst = ring + dst0 + i * (RPI * D * 2) + ((lch ^ ((lrow + RPI * i) & 7)) << 4);
-      if (P16) {
-        if (rest >= 16) {
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(base + i * RPI * stride)
-                       : "memory");
-        } else {
-          const bool in = lrow + RPI * i < rest;
-          asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n"
-                       ::"r"(dst), "l"(in ? base + i * RPI * stride : pool), "r"(in ? 16 : 0) : "memory");
+    for (int i = 0; i < 8 / RPI; ++i) to[i] = ring + dst0[i];
+    if (P16 && rest >= 16) {
+#pragma unroll
+      for (int i = 0; i < 16 / RPI; ++i)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n"
+                     ::"r"(to[i % (8 / RPI)] + i / (8 / RPI) * (8 * D * 2)),
+                       "l"(base + i * RPI * (MODE == kDenseRows ? D * 2 : stride)) : "memory");
+    } else {
+#pragma unroll
+      for (int i = 0; i < 16 / RPI; ++i) {
+        const uint32_t dst = to[i % (8 / RPI)] + i / (8 / RPI) * (8 * D * 2);
+        const char* src = base + i * RPI * stride;
+        bool in = lrow + RPI * i < rest;
+        if (!P16) {
+          const int64_t o = __shfl_sync(0xffffffffu, off, lrow + RPI * i);
+          in = o >= 0;
+          src = pool + (o + lch * 16);
         }
-      } else {
-        const int64_t o = __shfl_sync(0xffffffffu, off, lrow + RPI * i);
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;\n"
-                     ::"r"(dst), "l"(o >= 0 ? pool + (o + lch * 16) : pool), "r"(o >= 0 ? 16 : 0) : "memory");
+                     ::"r"(dst), "l"(in ? src : pool), "r"(in ? 16 : 0) : "memory");
       }
     }
   };
@@ -213,7 +238,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
         koff = in && ok ? rows.entry * p.c.ksp + nx.h * p.c.ksh + rows.slot * p.c.ksn : -1;
         vonext = in && ok ? rows.entry * p.c.vsp + nx.h * p.c.vsh + rows.slot * p.c.vsn : -1;
         bad = __any_sync(0xffffffffu, in && !ok);
-        copy(ring_k + (k_it & 1) * (D * 32), nullptr, p.c.k, koff, 0, 16);
+        copy(ring_k + (k_it & 1) * (D * 32), p.c.k, p.c.k, koff, 0, 16);
       }
       if (bad) {  // the whole unit: every output of the sequence is NaN
         asm volatile("cp.async.wait_all;\n" ::: "memory");
@@ -279,9 +304,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
     mx[nt][0] = mx[nt][1] = -INFINITY;
     mref[nt][0] = mref[nt][1] = sum[nt][0] = sum[nt][1] = 0.f;
   }
-  // ldmatrix lane addresses inside a unit (bytes)
-  const uint32_t k_row = (uint32_t)(lane & 15) * (D * 2), sw = lane & 7;
-  const uint32_t v_row = (uint32_t)((lane & 7) + ((lane >> 4) << 3)) * (D * 2);
+  // ldmatrix lane addresses of a unit's first chunks; chunk c lies c * 16 bytes on, by exclusive or
+  const uint32_t k_lane = ring_k + (lane & 15) * (D * 2) + (((lane >> 4) ^ (lane & 7)) << 4);
+  const uint32_t v_lane = ring_v + ((lane & 7) + ((lane >> 4) << 3)) * (D * 2) +
+                          ((((lane >> 3) & 1) ^ (lane & 7)) << 4);
 
   int seg = -1, len = 0;           // the segment in hand and its length
   bool fresh_seg = true;
@@ -309,45 +335,57 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
           ac[e] = c;
         }
       }
+      if (fresh_seg) {
 #pragma unroll
-      for (int e = 0; e < FPL; ++e) sm.ang[warp][lane * FPL + e] = make_float2(ac[e], as[e]);
-      __syncwarp();
+        for (int nt = 0; nt < NT; ++nt) {
+          const int g = at.z * GT + nt * 8 + fr;
+          const uint16_t* src = static_cast<const uint16_t*>(p.q) + at.x * p.qsb + (at.y * p.G + g) * p.qsh + fc * 2;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        const int g = at.z * GT + nt * 8 + fr;
-        const __nv_bfloat16* src = static_cast<const __nv_bfloat16*>(p.q) + at.x * p.qsb +
-                                   (at.y * p.G + g) * p.qsh + fc * 2;
-#pragma unroll
-        for (int ks = 0; ks < NH; ++ks)
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const int d = ks * 16 + b * 8;
-            const float4 cs = *reinterpret_cast<const float4*>(&sm.ang[warp][d + fc * 2]);
-            float x1[2] = {0.f, 0.f}, x2[2] = {0.f, 0.f};
+          for (int ks = 0; ks < NH; ++ks) {
+            uint32_t x[4] = {0u, 0u, 0u, 0u};
             if (g < p.G) {
 #pragma unroll
-              for (int e = 0; e < 2; ++e) {
-                x1[e] = __bfloat162float(src[d + e]) * p.qscale;
-                x2[e] = __bfloat162float(src[d + e + HALF]) * p.qscale;
+              for (int i = 0; i < 4; ++i) {
+                const int d = ks * 16 + (i & 1) * 8 + (i >> 1) * HALF;
+                x[i] = src[d] | (uint32_t)src[d + 1] << 16;
               }
             }
-            pack_split(x1[0] * cs.x - x2[0] * cs.y, x1[1] * cs.z - x2[1] * cs.w, qb[nt][ks][b], qb[nt][ks][2 + b]);
-            pack_split(x2[0] * cs.x + x1[0] * cs.y, x2[1] * cs.z + x1[1] * cs.w, qb[nt][ks + NH][b],
-                       qb[nt][ks + NH][2 + b]);
+            sm.q[warp][nt][ks][lane] = make_uint4(x[0], x[1], x[2], x[3]);
           }
+        }
       }
+#pragma unroll
+      for (int e = 0; e < FPL; ++e) {
+        float* x = reinterpret_cast<float*>(&sm.ang[warp][(lane * FPL + e) / 2]) + ((lane * FPL + e) & 1);
+        x[0] = ac[e] * p.qscale;
+        x[2] = as[e] * p.qscale;
+      }
+      __syncwarp();
+#pragma unroll
+      for (int ks = 0; ks < NH; ++ks)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const uint4 raw = sm.q[warp][nt][ks][lane];
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const float4 cs = sm.ang[warp][ks * 8 + b * 4 + fc];
+            const f32x2 c = pair(cs.x, cs.y), s = pair(cs.z, cs.w);
+            const f32x2 x1 = widen(b == 0 ? raw.x : raw.y), x2 = widen(b == 0 ? raw.z : raw.w);
+            split_round(fma2(mul2(x2, s), minus_one, mul2(x1, c)), minus_one, qb[nt][ks][b], qb[nt][ks][2 + b]);
+            split_round(fma2(x1, s, mul2(x2, c)), minus_one, qb[nt][ks + NH][b], qb[nt][ks + NH][2 + b]);
+          }
+        }
       __syncwarp();
     }
     // ---- S^T
     float sc[NT][2][4];
     const float4* rot = &sm.rot[n & 3][0][0][lane];
-    const uint32_t kb = ring_k + (it & 1) * (D * 32) + k_row;
+    const uint32_t kb = k_lane + (it & 1) * (D * 32);
 #pragma unroll
     for (int ks = 0; ks < NH; ++ks) {
       uint32_t a[4], b[4], ah[4], al[4], bh[4], bl[4];
-      const uint32_t ch = 2 * ks + (lane >> 4);
-      ldsm_x4(kb + ((ch ^ sw) << 4), a[0], a[1], a[2], a[3]);
-      ldsm_x4(kb + (((ch + CH / 2) ^ sw) << 4), b[0], b[1], b[2], b[3]);
+      ldsm_x4(kb ^ (ks * 32), a[0], a[1], a[2], a[3]);
+      ldsm_x4(kb ^ (ks * 32 + D), b[0], b[1], b[2], b[3]);
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         const f32x2 x1 = widen(a[r]), x2 = widen(b[r]);
@@ -441,7 +479,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         uint32_t hi, lo;
-        pack_split(e[2 * r], e[2 * r + 1], hi, lo);
+        split_round(pair(e[2 * r], e[2 * r + 1]), minus_one, hi, lo);
         ph[nt][r] = transpose8x8(hi);
         pl[nt][r] = transpose8x8(lo);
       }
@@ -452,8 +490,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       uint32_t a[4];
-      const uint32_t ch = 2 * mt + ((lane >> 3) & 1);
-      ldsm_x4_t(ring_v + v_row + ((ch ^ sw) << 4), a[0], a[1], a[2], a[3]);
+      ldsm_x4_t(v_lane ^ (mt * 32), a[0], a[1], a[2], a[3]);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         mma_bf16(acc[nt][mt], a, ph[nt][0], ph[nt][1]);
@@ -511,21 +548,23 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
   }
 }
 
-template <int D, int NT, bool P16>
+template <int D, int NT, RowMode MODE>
 int launch(const PDecP& p, cudaStream_t st) {
   constexpr int bytes = (int)sizeof(SmemB<D, NT>), NW = Cfg<D, NT>::NW;
-  const cudaError_t e = cudaFuncSetAttribute(paged_decode_bf16_kernel<D, NT, P16>,
+  const cudaError_t e = cudaFuncSetAttribute(paged_decode_bf16_kernel<D, NT, MODE>,
                                              cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e != cudaSuccess) return fail(STA_ERR_CUDA, cudaGetErrorString(e));
   // shares go to the CTAs in turn, so few shares spread over the SMs
   const int grid = p.W < p.sms * Cfg<D, NT>::CTAS ? p.W : p.sms * Cfg<D, NT>::CTAS;
-  paged_decode_bf16_kernel<D, NT, P16><<<grid, NW * 32, bytes, st>>>(p);
+  paged_decode_bf16_kernel<D, NT, MODE><<<grid, NW * 32, bytes, st>>>(p);
   return STA_OK;
 }
 
 template <int D, int NT>
 int launch(const PDecP& p, cudaStream_t st) {
-  return p.c.page % 16 == 0 ? launch<D, NT, true>(p, st) : launch<D, NT, false>(p, st);
+  if (p.c.page % 16 != 0) return launch<D, NT, kAnyRows>(p, st);
+  if (p.c.ksn == 2 * D && p.c.vsn == 2 * D) return launch<D, NT, kDenseRows>(p, st);
+  return launch<D, NT, kPageRows>(p, st);
 }
 
 }  // namespace
