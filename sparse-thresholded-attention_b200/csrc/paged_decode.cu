@@ -78,10 +78,11 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
   extern __shared__ __align__(128) unsigned char smem_raw[];
   S& sm = *reinterpret_cast<S*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  grid_dependents();
   const int64_t total = scan_lengths(p, 0, nullptr), shares = n_shares(p, total);
   if (blockIdx.x >= shares) return;
-  const int64_t t0 = total * blockIdx.x / shares, t1 = total * (blockIdx.x + 1) / shares;
-  const int count = (int)(t1 - t0);
+  const int64_t t0 = share_begin(total, blockIdx.x, shares);
+  const int count = (int)(share_begin(total, blockIdx.x + 1, shares) - t0);
   Place cur = find_unit(p, t0);
   Place qa = cur, oa = cur;  // where queries and row offsets stand
   int q_it = 0, l_it = 0, o_it = 0;
@@ -323,144 +324,157 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
   }
 }
 
-constexpr int kFinish = 256;   // threads of the finishing kernel
-constexpr int kKeysPer = 4;    // keys of a thread in the weights update
+constexpr int kJoin = 512;      // threads of the joining kernel
+constexpr int kUpd = 256;       // threads of the weights update, kKeysPer keys each
+constexpr int kKeysPer = 4;
 
-// The shares [w0, w1] of W that cut a segment; one share (w0 == w1) has finished it.
+// The shares [w0, w1] that cut a segment; one share (w0 == w1) has finished it.  Of the others, w0
+// holds its first unit and left partial 2 w0 + 1; share w behind it left partial 2 w.
 struct Cut {
-  int64_t total, W, s0, w0, w1;
+  int64_t w0, w1;
 };
 
-__device__ __forceinline__ Cut cut_of(const PDecP& p, int b, int hg, int64_t units) {
-  Cut c;
+// the share of unit t: share_begin(w) <= t < share_begin(w + 1), decided without a division
+__device__ __forceinline__ int64_t share_of(int64_t total, int64_t t, int64_t W) {
+  int64_t w = (int64_t)((double)t * (double)W / (double)total);
+  while (total * (w + 1) < (t + 1) * W) ++w;
+  while (total * w >= (t + 1) * W) --w;
+  return w;
+}
+
+__device__ __forceinline__ Cut cut_of(const PDecP& p, int b, int hg, int units) {
   int64_t before;
-  c.total = scan_lengths(p, b, &before);
-  c.W = n_shares(p, c.total);
-  c.s0 = before + hg * units;
-  const int64_t last = c.s0 + units - 1;
-  c.w0 = c.s0 * c.W / c.total;
-  c.w1 = last * c.W / c.total;
-  while (c.total * (c.w0 + 1) / c.W <= c.s0) ++c.w0;
-  while (c.total * (c.w1 + 1) / c.W <= last) ++c.w1;
-  return c;
+  const int64_t total = scan_lengths(p, b, &before), W = n_shares(p, total);
+  const int64_t s0 = before + (int64_t)hg * units;
+  return {share_of(total, s0, W), share_of(total, s0 + units - 1, W)};
 }
 
-// the partial that share w left of the segment (no share is empty: W is at most the units)
-__device__ __forceinline__ int64_t slot_of(const Cut& c, int64_t w) {
-  return 2 * w + (c.total * w / c.W <= c.s0 ? 1 : 0);
-}
+__device__ __forceinline__ int64_t slot_of(const Cut& c, int64_t w) { return 2 * w + (w == c.w0 ? 1 : 0); }
 
-// max and sum of one head over the partials of a segment, by one warp
-__device__ __forceinline__ void join_ml(const PDecP& p, const Cut& c, int g, float& M, float& L) {
-  const int lane = threadIdx.x & 31;
-  M = -INFINITY;
-  L = 0.f;
-  for (int64_t w = c.w0 + lane; w <= c.w1; w += 32) {
-    const float2 ml = p.part_ml[slot_of(c, w) * p.GT + g];
-    const float mn = fmaxf(M, ml.x), ms = mn == -INFINITY ? 0.f : mn;
-    L = L * exp2f(M - ms) + ml.y * exp2f(ml.x - ms);
-    M = mn;
-  }
-#pragma unroll
-  for (int o = 16; o >= 1; o >>= 1) {
-    const float m = __shfl_xor_sync(0xffffffffu, M, o), l = __shfl_xor_sync(0xffffffffu, L, o);
-    const float mn = fmaxf(M, m), ms = mn == -INFINITY ? 0.f : mn;
-    L = L * exp2f(M - ms) + l * exp2f(m - ms);
-    M = mn;
-  }
-  if (M == -INFINITY) M = 0.f;
-}
-
-// One block per (sequence, q head) joins the partials of the shares that cut its segment: a warp
-// takes every eighth partial, so that their loads are in flight together.  Empty sequences give
-// zeros.  With weights, blocks behind those update 1024 keys of a (sequence, kv head) each:
-// weights_out[j] = weights[j] + sum_g exp2(s_gj - M_g) / L_g, where they form M and L themselves.
+// One block per (sequence, q head) joins the partials of the shares that cut its segment: each of
+// 16 warps joins every 16th, eight of them in flight, then the warps' results are joined.  Empty
+// sequences give zeros.
 template <int D, typename TV>
-__global__ void __launch_bounds__(kFinish) paged_finish_kernel(const PDecP p) {
-  constexpr int NW = kFinish / 32, V = D / 32;
+__global__ void __launch_bounds__(kJoin) paged_join_kernel(const PDecP p) {
+  constexpr int NW = kJoin / 32, V = D / 32, U = 8;
   __shared__ float s_o[NW][D];
-  __shared__ float2 s_ml[128];
+  __shared__ float2 s_ml[NW];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t joins = (int64_t)p.c.B * p.H;
-  if (blockIdx.x < joins) {
-    const int b = blockIdx.x / p.H, h = blockIdx.x % p.H;
-    const int g0 = h % p.G, hg = h / p.G * p.NG + g0 / p.GT, g = g0 % p.GT;
-    const int units = n_units(p, paged_len(p.c, b));
-    TV* out = static_cast<TV*>(p.out) + (int64_t)blockIdx.x * D;
-    if (units == 0) {
-      if (tid < D) store_out(out + tid, 0.f);
-      return;
-    }
-    const Cut c = cut_of(p, b, hg, units);
-    if (c.w0 == c.w1) return;
-    float M, L;
-    join_ml(p, c, g, M, L);
-    float o[V];
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = 0.f;
-#pragma unroll 4
-    for (int64_t w = c.w0 + warp; w <= c.w1; w += NW) {
-      const int64_t slot = slot_of(c, w);
-      const float f = exp2f(p.part_ml[slot * p.GT + g].x - M);
-      const float* part = p.part + (slot * p.GT + g) * D + lane * V;
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = fmaf(part[i], f, o[i]);
-    }
-#pragma unroll
-    for (int i = 0; i < V; ++i) s_o[warp][lane * V + i] = o[i];
-    __syncthreads();
-    if (tid < D) {
-      float x = 0.f;
-#pragma unroll
-      for (int i = 0; i < NW; ++i) x += s_o[i][tid];
-      store_out(out + tid, x / L);
-    }
+  grid_dependents();
+  const int b = blockIdx.x / p.H, h = blockIdx.x % p.H;
+  const int g0 = h % p.G, hg = h / p.G * p.NG + g0 / p.GT, g = g0 % p.GT;
+  const int units = n_units(p, paged_len(p.c, b));
+  TV* out = static_cast<TV*>(p.out) + (int64_t)blockIdx.x * D;
+  if (units == 0) {
+    grid_wait();
+    if (tid < D) store_out(out + tid, 0.f);
     return;
   }
-  const int64_t chunks = (p.c.cap + kFinish * kKeysPer - 1) / (kFinish * kKeysPer);
-  const int64_t at = blockIdx.x - joins, seg = at / chunks;
+  const Cut c = cut_of(p, b, hg, units);
+  grid_wait();
+  if (c.w0 == c.w1) return;
+  float M = -INFINITY, L = 0.f, o[V];
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = 0.f;
+  for (int64_t w = c.w0 + warp; w <= c.w1; w += NW * U) {
+    float x[U][V];
+    float2 ml[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const bool in = w + u * NW <= c.w1;
+      const int64_t at = slot_of(c, in ? w + u * NW : w) * p.GT + g;
+      ml[u] = p.part_ml[at];
+      if (!in) ml[u].x = -INFINITY;
+      const float* part = p.part + at * D + lane * V;
+      if (V == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(part);
+        x[u][0] = y.x; x[u][1] = y.y; x[u][V - 2] = y.z; x[u][V - 1] = y.w;
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(part);
+        x[u][0] = y.x; x[u][V - 1] = y.y;
+      }
+    }
+    float mn = M;
+#pragma unroll
+    for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
+    const float ms = mn == -INFINITY ? 0.f : mn, a = exp2f(M - ms);
+    L *= a;
+#pragma unroll
+    for (int i = 0; i < V; ++i) o[i] *= a;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      if (w + u * NW > c.w1) break;
+      const float f = exp2f(ml[u].x - ms);
+      L = fmaf(ml[u].y, f, L);
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] = fmaf(x[u][i], f, o[i]);
+    }
+    M = mn;
+  }
+#pragma unroll
+  for (int i = 0; i < V; ++i) s_o[warp][lane * V + i] = o[i];
+  if (lane == 0) s_ml[warp] = make_float2(M, L);
+  __syncthreads();
+  if (tid < D) {
+    float m = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) m = fmaxf(m, s_ml[i].x);
+    const float ms = m == -INFINITY ? 0.f : m;
+    float x = 0.f, l = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      const float f = exp2f(s_ml[i].x - ms);
+      l = fmaf(s_ml[i].y, f, l);
+      x = fmaf(s_o[i][tid], f, x);
+    }
+    store_out(out + tid, x / l);
+    if (tid == 0) p.ml[blockIdx.x] = make_float2(ms, 1.f / l);
+  }
+}
+
+// weights_out[j] = weights[j] + sum_g exp2(s_gj - M_g) / L_g, 1024 keys of a (sequence, kv head)
+// per block.
+__global__ void __launch_bounds__(kUpd) paged_weights_kernel(const PDecP p) {
+  const int64_t chunks = (p.c.cap + kUpd * kKeysPer - 1) / (kUpd * kKeysPer), seg = blockIdx.x / chunks;
   const int b = (int)(seg / p.c.Hkv), h = (int)(seg % p.c.Hkv);
   const int len = paged_len(p.c, b);
-  const int64_t j0 = (at % chunks) * (kFinish * kKeysPer) + tid;
-  if (at % chunks * (kFinish * kKeysPer) >= len) return;
-  float sum[kKeysPer];
-#pragma unroll
-  for (int i = 0; i < kKeysPer; ++i) sum[i] = 0.f;
-  for (int grp = 0; grp < p.NG; ++grp) {
-    const int hg = h * p.NG + grp, heads = min(p.GT, p.G - grp * p.GT);
-    const Cut c = cut_of(p, b, hg, n_units(p, len));
-    for (int g = warp; g < heads; g += NW) {
-      float2 ml;
-      if (c.w0 == c.w1) {
-        ml = p.ml[(int64_t)b * p.H + h * p.G + grp * p.GT + g];
-      } else {
-        join_ml(p, c, g, ml.x, ml.y);
-        ml.y = 1.f / ml.y;
-      }
-      if (lane == 0) s_ml[g] = ml;
-    }
-    __syncthreads();
-    const float* sc = p.scores + ((int64_t)b * p.c.Hkv * p.NG + hg) * p.cap_tiles * p.GT * kTile;
-    for (int g = 0; g < heads; ++g) {
-      const float2 ml = s_ml[g];
-#pragma unroll
-      for (int i = 0; i < kKeysPer; ++i) {
-        const int64_t j = j0 + i * kFinish;
-        if (j < len) sum[i] += exp2f(sc[(j / kTile * p.GT + g) * kTile + j % kTile] - ml.x) * ml.y;
-      }
-    }
-    __syncthreads();
+  const int j0 = (int)(blockIdx.x % chunks) * (kUpd * kKeysPer) + threadIdx.x;
+  if (j0 - (int)threadIdx.x >= len) {
+    grid_wait();  // no block of a chain of programmatic launches ends before the kernel ahead has
+    return;
   }
+  float sum[kKeysPer], old[kKeysPer];
+  int64_t to[kKeysPer];
 #pragma unroll
   for (int i = 0; i < kKeysPer; ++i) {
-    const int64_t j = j0 + i * kFinish;
-    if (j >= len) break;
-    const uint32_t t = (uint32_t)j / p.c.page;
-    const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
-    if (pg < 0) continue;
-    const int64_t w = pg * p.c.wsp + h * p.c.wsh + ((uint32_t)j - t * p.c.page);
-    p.w_out[w] = p.c.w[w] + sum[i];
+    const int j = j0 + i * kUpd;
+    sum[i] = old[i] = 0.f;
+    to[i] = -1;
+    if (j < len) {
+      const uint32_t t = (uint32_t)j / p.c.page;
+      const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
+      if (pg >= 0) to[i] = pg * p.c.wsp + h * p.c.wsh + ((uint32_t)j - t * p.c.page);
+    }
   }
+#pragma unroll
+  for (int i = 0; i < kKeysPer; ++i)
+    if (to[i] >= 0) old[i] = p.c.w[to[i]];
+  grid_wait();
+  const float2* ml = p.ml + (int64_t)b * p.H + h * p.G;
+  const float* sc = p.scores + ((int64_t)b * p.c.Hkv + h) * p.NG * p.cap_tiles * p.GT * kTile;
+#pragma unroll 4
+  for (int g = 0; g < p.G; ++g) {
+    const float2 x = ml[g];
+    const int64_t row = (int64_t)(g / p.GT) * p.cap_tiles * p.GT + g % p.GT;
+#pragma unroll
+    for (int i = 0; i < kKeysPer; ++i) {
+      const int j = j0 + i * kUpd;
+      if (j < len) sum[i] += exp2f(sc[(row + (int64_t)(j / kTile) * p.GT) * kTile + j % kTile] - x.x) * x.y;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kKeysPer; ++i)
+    if (to[i] >= 0) p.w_out[to[i]] = old[i] + sum[i];
 }
 
 struct PLayout {
@@ -554,13 +568,32 @@ int launch_f32(const PDecP& p, cudaStream_t st) {
   return launch_f32<D, 8>(p, st);
 }
 
+// Launches a kernel that may begin before the one ahead of it in the stream has ended (it waits
+// for that kernel's results itself), so that its launch does not add to the call.
+template <typename K>
+cudaError_t launch_behind(K kernel, int64_t grid, int threads, const PDecP& p, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 template <typename TV>
-void launch_finish(const PDecP& p, int d, cudaStream_t st) {
-  int64_t grid = (int64_t)p.c.B * p.H;
-  if (p.scores)
-    grid += (int64_t)p.c.B * p.c.Hkv * ((p.c.cap + kFinish * kKeysPer - 1) / (kFinish * kKeysPer));
-  if (d == 128) paged_finish_kernel<128, TV><<<(unsigned)grid, kFinish, 0, st>>>(p);
-  else paged_finish_kernel<64, TV><<<(unsigned)grid, kFinish, 0, st>>>(p);
+cudaError_t launch_finish(const PDecP& p, int d, cudaStream_t st) {
+  const int64_t heads = (int64_t)p.c.B * p.H;
+  cudaError_t e = d == 128 ? launch_behind(paged_join_kernel<128, TV>, heads, kJoin, p, st)
+                           : launch_behind(paged_join_kernel<64, TV>, heads, kJoin, p, st);
+  if (e == cudaSuccess && p.scores) {
+    const int64_t chunks = (p.c.cap + kUpd * kKeysPer - 1) / (kUpd * kKeysPer);
+    e = launch_behind(paged_weights_kernel, (int64_t)p.c.B * p.c.Hkv * chunks, kUpd, p, st);
+  }
+  return e;
 }
 
 }  // namespace
@@ -610,9 +643,9 @@ int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void*
   if (f32) rc = c->d == 128 ? launch_f32<128>(p, st) : launch_f32<64>(p, st);
   else rc = launch_paged_decode_bf16(p, c->d, st);
   if (rc != STA_OK) return rc;
-  if (f32) launch_finish<float>(p, c->d, st);
-  else launch_finish<__nv_bfloat16>(p, c->d, st);
-  const cudaError_t e = cudaGetLastError();
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess)
+    e = f32 ? launch_finish<float>(p, c->d, st) : launch_finish<__nv_bfloat16>(p, c->d, st);
   return e == cudaSuccess ? STA_OK : fail(STA_ERR_CUDA, cudaGetErrorString(e));
 }
 

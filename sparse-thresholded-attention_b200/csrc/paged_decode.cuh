@@ -31,6 +31,11 @@ struct PDecP {
   int* err;
 };
 
+// Programmatic launch: the next kernel of the stream may be set up from here on / its inputs, the
+// results of the kernel ahead, are complete from here on.
+__device__ __forceinline__ void grid_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 __device__ __forceinline__ int n_units(const PDecP& p, int len) {
   return (int)(((uint32_t)len + (1u << p.unit) - 1u) >> p.unit);
 }
@@ -54,10 +59,16 @@ __device__ __forceinline__ int64_t scan_lengths(const PDecP& p, int until, int64
   return all * hg;
 }
 
-// Shares that the units are cut into: share w holds the units [total w / W, total (w + 1) / W).
+// Shares that the units are cut into: share w holds the units from share_begin(w) = total w / W
+// (rounded down) to share_begin(w + 1).
 __device__ __forceinline__ int64_t n_shares(const PDecP& p, int64_t total) {
   const int64_t w = (total + p.min_units - 1) / p.min_units;
   return w < p.W ? w : p.W;
+}
+
+__device__ __forceinline__ int64_t share_begin(int64_t total, int64_t w, int64_t W) {
+  const int64_t x = total * w;
+  return (x >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)W) : x / W;
 }
 
 // A place in the list of units.

@@ -135,14 +135,15 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int fr = lane >> 2, fc = lane & 3;
 
+  grid_dependents();
   const int64_t total = scan_lengths(p, 0, nullptr);
   const int64_t shares = n_shares(p, total), me = (int64_t)warp * gridDim.x + blockIdx.x;
   int count = 0;
   Place nx{};                       // the unit whose K rows are loaded next
   Rows rows{-1, 0, 0, true};
   if (me < shares) {
-    const int64_t t0 = total * me / shares;
-    count = (int)(total * (me + 1) / shares - t0);
+    const int64_t t0 = share_begin(total, me, shares);
+    count = (int)(share_begin(total, me + 1, shares) - t0);
     nx = find_unit(p, t0);
   }
   int segs = 0, k_it = 0;           // segments entered, units whose K rows are loaded
