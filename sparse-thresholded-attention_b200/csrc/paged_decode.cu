@@ -79,11 +79,10 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
   S& sm = *reinterpret_cast<S*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_dependents();
-  const int64_t total = scan_lengths(p, 0, nullptr), shares = n_shares(p, total);
-  if (blockIdx.x >= shares) return;
-  const int64_t t0 = share_begin(total, blockIdx.x, shares);
-  const int count = (int)(share_begin(total, blockIdx.x + 1, shares) - t0);
-  Place cur = find_unit(p, t0);
+  const Share share = find_share(p, blockIdx.x, first_len(p.c));
+  const int count = share.count;
+  if (count == 0) return;
+  Place cur = share.at;
   Place qa = cur, oa = cur;  // where queries and row offsets stand
   int q_it = 0, l_it = 0, o_it = 0;
 
@@ -616,6 +615,7 @@ int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void*
   PDecP p;
   p.c = paged_view(c);
   p.q = a->q; p.qsb = a->q_stride_b; p.qsh = a->q_stride_h;
+  p.q_words = (reinterpret_cast<uintptr_t>(a->q) & 3) == 0 && a->q_stride_b % 2 == 0 && a->q_stride_h % 2 == 0;
   p.out = a->out;
   p.H = (int)a->n_heads;
   p.G = (int)(a->n_heads / c->n_kv_heads);
@@ -623,7 +623,7 @@ int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void*
   p.GT = L.GT;
   p.unit = L.unit;
   p.W = L.W;
-  p.min_units = f32 ? 1 : 2;
+  p.min_log = f32 ? 0 : 1;
   p.sms = sm_count();
   p.k16 = 16 * p.c.ksn;
   p.v16 = 16 * p.c.vsn;

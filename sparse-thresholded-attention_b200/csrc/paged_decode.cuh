@@ -12,10 +12,11 @@ struct PDecP {
   PagedView c;
   const void* q;
   int64_t qsb, qsh;  // elements
+  int q_words;       // 16-bit queries start on 4-byte boundaries
   void* out;
   int H, G, NG, GT;  // q heads, per kv head, groups of GT of them
   int unit;          // log2 of the keys of a unit of work
-  int W, min_units;  // shares at most, units of a share at least
+  int W, min_log;    // shares at most, log2 of the units of a share at least
   int sms;
   int64_t k16, v16;  // bytes of 16 rows
   const float* inv_freq;
@@ -62,13 +63,16 @@ __device__ __forceinline__ int64_t scan_lengths(const PDecP& p, int until, int64
 // Shares that the units are cut into: share w holds the units from share_begin(w) = total w / W
 // (rounded down) to share_begin(w + 1).
 __device__ __forceinline__ int64_t n_shares(const PDecP& p, int64_t total) {
-  const int64_t w = (total + p.min_units - 1) / p.min_units;
+  const int64_t w = (total + (1 << p.min_log) - 1) >> p.min_log;
   return w < p.W ? w : p.W;
 }
 
+// x / y for x >= 0, y > 0; 64-bit divisions are long, and seldom needed
+__device__ __forceinline__ int64_t div_fast(int64_t x, int64_t y) {
+  return ((x | y) >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)y) : x / y;
+}
 __device__ __forceinline__ int64_t share_begin(int64_t total, int64_t w, int64_t W) {
-  const int64_t x = total * w;
-  return (x >> 32) == 0 ? (int64_t)((uint32_t)x / (uint32_t)W) : x / W;
+  return div_fast(total * w, W);
 }
 
 // A place in the list of units.
@@ -97,37 +101,63 @@ __device__ __forceinline__ void step(const PDecP& p, Place& a) {
   seek_sequence(p, a);
 }
 
-// The place of unit t (t < the number of units), found by a warp.
-__device__ __forceinline__ Place find_unit(const PDecP& p, int64_t t) {
+// What share `me` holds: `count` units from the place `at` on (count 0: nothing).  Found by a warp;
+// `len` is the length of sequence `lane` (0 beyond the batch), loaded by the caller ahead of time.
+struct Share {
+  int count;
+  Place at;
+};
+
+__device__ __forceinline__ Share find_share(const PDecP& p, int64_t me, int len) {
   const int lane = threadIdx.x & 31;
   const int64_t hg = (int64_t)p.c.Hkv * p.NG;
-  int64_t base = 0;
-  Place a{};
-  for (int b0 = 0; b0 < p.c.B; b0 += 32) {
-    const int b = b0 + lane;
-    const int64_t mine = b < p.c.B ? (int64_t)n_units(p, paged_len(p.c, b)) * hg : 0;
-    int64_t inc = mine;
+  int64_t mine = n_units(p, len) * hg, inc = mine;  // of the first 32 sequences
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += y;
+  }
+  int64_t base = 0, total = __shfl_sync(0xffffffffu, inc, 31);
+  const int64_t head = total;
+  if (p.c.B > 32) {
+    int64_t more = 0;
+    for (int b = 32 + lane; b < p.c.B; b += 32) more += n_units(p, paged_len(p.c, b));
+#pragma unroll
+    for (int o = 16; o >= 1; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+    total += more * hg;
+  }
+  const int64_t shares = n_shares(p, total);
+  Share s{};
+  if (me >= shares) return s;
+  const int64_t t = share_begin(total, me, shares);
+  s.count = (int)(share_begin(total, me + 1, shares) - t);
+  int b0 = 0;
+  while (t >= base + (b0 == 0 ? head : __shfl_sync(0xffffffffu, inc, 31))) {  // (t < total: ends)
+    base += b0 == 0 ? head : __shfl_sync(0xffffffffu, inc, 31);
+    b0 += 32;
+    len = b0 + lane < p.c.B ? paged_len(p.c, b0 + lane) : 0;
+    inc = mine = n_units(p, len) * hg;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int64_t y = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += y;
     }
-    const uint32_t hit = __ballot_sync(0xffffffffu, mine > 0 && t >= base + inc - mine && t < base + inc);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      const int64_t rest = t - __shfl_sync(0xffffffffu, base + inc - mine, src);
-      a.b = b0 + src;
-      a.len = paged_len(p.c, a.b);
-      a.units = n_units(p, a.len);
-      const int g = (int)(rest / a.units);
-      a.n = (int)(rest - (int64_t)g * a.units);
-      a.h = g / p.NG;
-      a.grp = g - a.h * p.NG;
-      return a;
-    }
-    base += __shfl_sync(0xffffffffu, inc, 31);
   }
-  return a;
+  const int src = __ffs(__ballot_sync(0xffffffffu, t < base + inc)) - 1;
+  const int64_t rest = t - base - __shfl_sync(0xffffffffu, inc - mine, src);
+  s.at.b = b0 + src;
+  s.at.len = __shfl_sync(0xffffffffu, len, src);
+  s.at.units = n_units(p, s.at.len);
+  const int g = (int)div_fast(rest, s.at.units);
+  s.at.n = (int)(rest - (int64_t)g * s.at.units);
+  s.at.h = p.NG == 1 ? g : g / p.NG;
+  s.at.grp = g - s.at.h * p.NG;
+  return s;
+}
+
+__device__ __forceinline__ int first_len(const PagedView& c) {
+  const int lane = threadIdx.x & 31;
+  return lane < c.B ? paged_len(c, lane) : 0;
 }
 
 // cos / sin of pos * inv_freq: the angle in turns is formed and reduced in 64 bits

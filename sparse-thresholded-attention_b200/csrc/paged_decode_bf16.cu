@@ -41,6 +41,7 @@ struct SmemB {
   float4 rot[4][D / 32][4][32];           // (cos, cos, sin, sin) of two dims: unit, k step, register, lane
   float4 ang[NW][D / 4];                  // (cos, cos, sin, sin) of the query's angle, two dims, times the scale
   uint4 q[NW][NT][D / 32][32];            // a lane's raw queries of a k step: dims 0, 8, d/2, d/2 + 8 on, two each
+  float2 turns[16][D / 2];                // cos / sin of turns by 0 .. 7 and by 0, 8 .. 56 positions
   int4 seg[NW][4];                        // segments entered by the loads: sequence, kv head, group, length
 };
 
@@ -136,16 +137,18 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
   const int fr = lane >> 2, fc = lane & 3;
 
   grid_dependents();
-  const int64_t total = scan_lengths(p, 0, nullptr);
-  const int64_t shares = n_shares(p, total), me = (int64_t)warp * gridDim.x + blockIdx.x;
-  int count = 0;
-  Place nx{};                       // the unit whose K rows are loaded next
-  Rows rows{-1, 0, 0, true};
-  if (me < shares) {
-    const int64_t t0 = share_begin(total, me, shares);
-    count = (int)(share_begin(total, me + 1, shares) - t0);
-    nx = find_unit(p, t0);
+  // ---- cos / sin of the key offsets t * pos_scale, t = 0 .. 63, by all warps: t = 8 i + j as the
+  // product of the turns by 8 i and by j (16 sincos per frequency instead of 64)
+  const int len0 = first_len(p.c);
+  for (int i = threadIdx.x; i < 16 * HALF; i += NW * 32) {
+    const int f = i % HALF, t = i / HALF;
+    turn((double)(t < 8 ? t : (t - 8) * 8) * p.pos_scale, __ldg(p.inv_freq + f), sm.turns[t][f].x, sm.turns[t][f].y);
   }
+  const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;
+  const Share share = find_share(p, me, len0);
+  const int count = share.count;
+  Place nx = share.at;              // the unit whose K rows are loaded next
+  Rows rows{-1, 0, 0, true};
   int segs = 0, k_it = 0;           // segments entered, units whose K rows are loaded
   int n = nx.n;                     // the unit in hand, of its segment
 
@@ -260,25 +263,49 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
 
+  // ---- a segment's raw queries, as the lanes rotate them
+  auto raw_queries = [&](const int4& at) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int g = at.z * GT + nt * 8 + fr;
+      const uint16_t* src = static_cast<const uint16_t*>(p.q) + at.x * p.qsb + (at.y * p.G + g) * p.qsh + fc * 2;
+#pragma unroll
+      for (int ks = 0; ks < NH; ++ks) {
+        uint32_t x[4] = {0u, 0u, 0u, 0u};
+        if (g < p.G) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int d = ks * 16 + (i & 1) * 8 + (i >> 1) * HALF;
+            x[i] = p.q_words ? *reinterpret_cast<const uint32_t*>(src + d) : src[d] | (uint32_t)src[d + 1] << 16;
+          }
+        }
+        sm.q[warp][nt][ks][lane] = make_uint4(x[0], x[1], x[2], x[3]);
+      }
+    }
+  };
   const char* vcur = p.c.v;   // the V rows that follow next
   int64_t vocur = 0;
   int vlcur = 0;
   if (count > 0) {
     lookup(true);
+    // (ahead of the rows: what is asked for behind them waits until they have come)
+    raw_queries(make_int4(share.at.b, share.at.h, share.at.grp, 0));
+  }
+  __syncthreads();
+  if (count > 0) {
     load_k();
     vcur = vnext; vocur = vonext; vlcur = vleft;
     load_v(0, vcur, vocur, vlcur);
     load_k();
     vcur = vnext; vocur = vonext; vlcur = vleft;
   }
-  // ---- cos / sin of the key offsets t * pos_scale, t = 0 .. 63, by all warps
   for (int i = threadIdx.x; i < 4 * NH * 4 * 32; i += NW * 32) {
     const int l = i & 31, r = (i >> 5) & 3, ks = (i >> 7) % NH, u = i / (128 * NH);
-    const int t = u * 16 + (l >> 2) + (r & 1) * 8, f = ks * 16 + (l & 3) * 2 + (r >> 1) * 8;
-    float4 x;
-    turn((double)t * p.pos_scale, __ldg(p.inv_freq + f), x.x, x.z);
-    turn((double)t * p.pos_scale, __ldg(p.inv_freq + f + 1), x.y, x.w);
-    sm.rot[u][ks][r][l] = x;
+    const int f = ks * 16 + (l & 3) * 2 + (r >> 1) * 8;
+    const float4 a = *reinterpret_cast<const float4*>(&sm.turns[l >> 2][f]);
+    const float4 b = *reinterpret_cast<const float4*>(&sm.turns[8 + 2 * u + (r & 1)][f]);
+    sm.rot[u][ks][r][l] = make_float4(a.x * b.x - a.y * b.y, a.z * b.z - a.w * b.w,
+                                      a.x * b.y + a.y * b.x, a.z * b.w + a.w * b.z);
   }
   __syncthreads();
   if (count == 0) return;
@@ -314,8 +341,6 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
   bool fresh_seg = true;
 #pragma unroll 1
   for (int it = 0; it < count; ++it) {
-    asm volatile("cp.async.wait_group 2;\n" ::: "memory");
-    __syncwarp();
     if (fresh_seg) {
       ++seg;
       len = sm.seg[warp][seg & 3].w;
@@ -336,25 +361,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
           ac[e] = c;
         }
       }
-      if (fresh_seg) {
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          const int g = at.z * GT + nt * 8 + fr;
-          const uint16_t* src = static_cast<const uint16_t*>(p.q) + at.x * p.qsb + (at.y * p.G + g) * p.qsh + fc * 2;
-#pragma unroll
-          for (int ks = 0; ks < NH; ++ks) {
-            uint32_t x[4] = {0u, 0u, 0u, 0u};
-            if (g < p.G) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int d = ks * 16 + (i & 1) * 8 + (i >> 1) * HALF;
-                x[i] = src[d] | (uint32_t)src[d + 1] << 16;
-              }
-            }
-            sm.q[warp][nt][ks][lane] = make_uint4(x[0], x[1], x[2], x[3]);
-          }
-        }
-      }
+      if (fresh_seg && it > 0) raw_queries(at);
 #pragma unroll
       for (int e = 0; e < FPL; ++e) {
         float* x = reinterpret_cast<float*>(&sm.ang[warp][(lane * FPL + e) / 2]) + ((lane * FPL + e) & 1);
@@ -379,6 +386,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
       __syncwarp();
     }
     // ---- S^T
+    asm volatile("cp.async.wait_group 2;\n" ::: "memory");
+    __syncwarp();
     float sc[NT][2][4];
     const float4* rot = &sm.rot[n & 3][0][0][lane];
     const uint32_t kb = k_lane + (it & 1) * (D * 32);
