@@ -53,6 +53,17 @@ __device__ __forceinline__ int64_t paged_page(const PagedView& c, const int32_t*
   return pg >= 0 && pg < c.n_pages ? pg : -1;
 }
 
+// Lets a kernel have `bytes` of dynamic shared memory; asked for once per device (`ready`).
+template <typename K>
+inline cudaError_t allow_smem(K kernel, int bytes, bool (&ready)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < 64 && ready[dev])) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess && dev < 64) ready[dev] = true;
+  return e;
+}
+
 inline int paged_check(const sta_paged_cache* c) {
   if (!c || !c->k || !c->v || !c->table || !c->lens)
     return fail(STA_ERR_ARG, "sta_paged: null pointer");

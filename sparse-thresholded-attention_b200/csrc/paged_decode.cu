@@ -552,8 +552,8 @@ int check(const sta_paged_cache* c, const sta_paged_decode_args* a) {
 template <int D, int GT>
 int launch_f32(const PDecP& p, cudaStream_t st) {
   constexpr int bytes = (int)sizeof(Smem<D, GT>);
-  const cudaError_t e = cudaFuncSetAttribute(paged_decode_f32_kernel<D, GT>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static bool ready[64];
+  const cudaError_t e = allow_smem(paged_decode_f32_kernel<D, GT>, bytes, ready);
   if (e != cudaSuccess) return fail(STA_ERR_CUDA, cudaGetErrorString(e));
   paged_decode_f32_kernel<D, GT><<<p.W, kF32Threads, bytes, st>>>(p);
   return STA_OK;

@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
     dst0[i] = (uint32_t)(row * (D * 2) + ((lch ^ row) << 4));
   }
   const char *kbase = p.c.k, *vbase = p.c.v, *vnext = p.c.v;  // P16: this lane's first row
-  int64_t koff = 0, voff = 0, vonext = 0;  // otherwise: of row (lane & 15); -1: no row, -2: bad page
+  int64_t koff = 0, vonext = 0;            // otherwise: of row (lane & 15); -1: no row, -2: bad page
   int left = 0, vleft = 0;                 // keys of the unit from its first on; 0: a bad page
   auto copy = [&](uint32_t ring, const char* base, const char* pool, int64_t off, int64_t stride, int rest) {
     uint32_t to[8 / RPI];
@@ -561,8 +561,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
 template <int D, int NT, RowMode MODE>
 int launch(const PDecP& p, cudaStream_t st) {
   constexpr int bytes = (int)sizeof(SmemB<D, NT>), NW = Cfg<D, NT>::NW;
-  const cudaError_t e = cudaFuncSetAttribute(paged_decode_bf16_kernel<D, NT, MODE>,
-                                             cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  static bool ready[64];
+  const cudaError_t e = allow_smem(paged_decode_bf16_kernel<D, NT, MODE>, bytes, ready);
   if (e != cudaSuccess) return fail(STA_ERR_CUDA, cudaGetErrorString(e));
   // shares go to the CTAs in turn, so few shares spread over the SMs
   const int grid = p.W < p.sms * Cfg<D, NT>::CTAS ? p.W : p.sms * Cfg<D, NT>::CTAS;

@@ -1,19 +1,31 @@
 // Eviction from a paged cache by accumulated attention weight.
 //
-// Per (sequence, kv head): the min(len, budget) slots to keep are the forced ones (first
-// n_global, last n_local) and the heaviest others, ties to the lowest slot -- an order statistic
-// over order-preserving integer keys, found by radix selection (4 rounds of 8 bits), then a
-// compaction in slot order.  A second launch copies the kept rows of K, V and weights into the
-// new pages; source and destination pages are disjoint, so rows move independently of each other.
+// Per (sequence, kv head) the min(len, budget) slots to keep are the forced ones (first n_global,
+// last n_local) and the heaviest others, ties to the lowest slot.  One cluster of up to 8 CTAs
+// does all of it for one (sequence, kv head); each CTA holds a contiguous slice of the slots:
+//   1. the weights become order-preserving integer keys in shared memory;
+//   2. the key of the last kept slot is found by radix selection (11 + 11 + 10 bits): every CTA
+//      counts its slice, then reads all CTAs' counts (distributed shared memory) and finds the
+//      digit, so that no CTA waits for a result of another beyond one cluster barrier per digit;
+//   3. each CTA compacts its slice, and copies the rows of K, V and weights that it keeps into the
+//      new pages.  Source and destination pages are disjoint: rows move independently.
+// The kept rows (read and written once) bound it: the selection reads 4 bytes per slot.
+#include <cooperative_groups.h>
+
 #include "paged.cuh"
+
+namespace cg = cooperative_groups;
 
 namespace sta {
 
 namespace {
 
-constexpr int kSel = 1024;
-constexpr int kCopy = 256;
-constexpr int kIter = 4;
+constexpr int kThreads = 512;
+constexpr int kWarps = kThreads / 32;
+constexpr int kBins = 2048;
+constexpr int kItems = 8;              // consecutive slots of a thread in the compaction
+constexpr int kChunk = kThreads * kItems;
+constexpr int kSliceSmem = 20 * 1024;  // slots of a slice whose keys fit shared memory (80 KB)
 
 struct EvP {
   PagedView c;
@@ -23,8 +35,19 @@ struct EvP {
   uint32_t cap_out;
   int32_t* kept;
   int32_t* lens_out;
-  uint32_t* keys;  // (B, Hkv, cap) order-preserving keys
+  uint32_t* keys;     // (B, Hkv, cap) where a slice exceeds shared memory, else null
   int* err;
+};
+
+struct Counts {
+  int above, equal;
+};
+
+struct SmemE {
+  uint32_t hist[3][kBins];  // of each digit (others may still read the one before)
+  uint32_t scan[kWarps];
+  uint32_t digit, rest;  // the digit found and how many of its slots are kept
+  Counts counts;
 };
 
 // larger weight, larger key; NaN below everything, forced slots above everything
@@ -34,143 +57,212 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-__device__ __forceinline__ int block_excl_sum(int x, int* sh, int& total) {
+__device__ __forceinline__ uint32_t block_excl_sum(uint32_t x, uint32_t* sh, uint32_t& total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  int inc = x;
+  uint32_t inc = x;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, inc, o);
+    const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
     if (lane >= o) inc += y;
   }
   if (lane == 31) sh[w] = inc;
   __syncthreads();
-  int base = 0, all = 0;
-  for (int i = 0; i < kSel / 32; ++i) {
-    if (i < w) base += sh[i];
-    all += sh[i];
+  uint32_t base = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    const uint32_t y = sh[i];
+    if (i < w) base += y;
+    all += y;
   }
   __syncthreads();
   total = all;
   return base + inc - x;
 }
 
-__global__ void __launch_bounds__(kSel) paged_evict_select_kernel(const EvP p) {
-  __shared__ uint32_t hist[256];
-  __shared__ int sh[kSel / 32];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_k;
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-  const int len = paged_len(p.c, b);
-  const int n = (int)min((int64_t)len, p.budget);
-  int32_t* kept = p.kept + ((int64_t)b * p.c.Hkv + h) * p.budget;
-  if (h == 0 && tid == 0) p.lens_out[b] = n;
-  for (int64_t r = n + tid; r < p.budget; r += kSel) kept[r] = -1;
-  if (len <= p.budget) {
-    for (int r = tid; r < n; r += kSel) kept[r] = r;
-    return;
-  }
-  uint32_t* keys = p.keys + ((int64_t)b * p.c.Hkv + h) * p.c.cap;
-  for (int j = tid; j < len; j += kSel) {
-    uint32_t key;
-    if (j < p.n_global || j >= len - p.n_local) {
-      key = 0xffffffffu;
-    } else {
-      const uint32_t t = (uint32_t)j / p.c.page;
-      const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
-      if (pg < 0) atomicCAS(p.err, 0, kErrPageEvict);
-      key = pg < 0 ? 0u : weight_key(p.c.w[pg * p.c.wsp + h * p.c.wsh + ((uint32_t)j - t * p.c.page)]);
-    }
-    keys[j] = key;
-  }
-  // the n-th largest key and how many of its equals are kept
-  if (tid == 0) {
-    s_prefix = 0u;
-    s_k = n;
-  }
-  uint32_t mask = 0u;
-  for (int round = 0; round < 4; ++round) {
-    const int shift = 24 - 8 * round;
-    if (tid < 256) hist[tid] = 0u;
-    __syncthreads();
-    const uint32_t prefix = s_prefix;
-    for (int j = tid; j < len; j += kSel) {
-      const uint32_t key = keys[j];
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255u], 1u);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      int kk = s_k, d = 255;
-      for (; d > 0; --d) {
-        if ((int)hist[d] >= kk) break;
-        kk -= (int)hist[d];
-      }
-      s_k = kk;
-      s_prefix = prefix | ((uint32_t)d << shift);
-    }
-    __syncthreads();
-    mask |= 255u << shift;
-  }
-  const uint32_t cut = s_prefix;
-  const int equals = s_k;
-  int carry = 0, tie_carry = 0;
-  for (int j0 = 0; j0 < len; j0 += kSel) {
-    const int j = j0 + tid;
-    const uint32_t key = j < len ? keys[j] : 0u;
-    const int tie = j < len && key == cut;
-    int ties, all;
-    const int tr = block_excl_sum(tie, sh, ties);
-    const int keep = j < len && (key > cut || (tie && tie_carry + tr < equals));
-    const int r = carry + block_excl_sum(keep, sh, all);
-    if (keep) kept[r] = j;
-    carry += all;
-    tie_carry += ties;
-  }
-}
-
-// One unit: the K and V row of one kept slot; 16-byte chunks, all loads before the stores.
+// 32 kept rows of a warp: lane l has slot j (its rank r = r0 + l); `n` of them are rows.  A row's K
+// and V are LPU lanes' 16-byte chunks; four of a lane's loads are in flight.
 template <int CH>
-__global__ void __launch_bounds__(kCopy) paged_evict_copy_kernel(const EvP p) {
-  constexpr int UNITS = kCopy / (2 * CH);
-  const int tid = threadIdx.x;
-  const int ch = tid % CH, is_v = (tid / CH) & 1, sub = tid / (2 * CH);
-  const int h = blockIdx.y, b = blockIdx.z;
-  const int n = (int)min((int64_t)paged_len(p.c, b), p.budget);
-  const int r0 = (int)blockIdx.x * (UNITS * kIter) + sub;
-  if (r0 >= n) return;
-  const int32_t* kept = p.kept + ((int64_t)b * p.c.Hkv + h) * p.budget;
-  uint4 x[kIter];
-  float w[kIter];
-  char* dst[kIter];
-  float* wdst[kIter];
-#pragma unroll
-  for (int i = 0; i < kIter; ++i) {
-    const int r = r0 + i * UNITS;
-    dst[i] = nullptr;
-    wdst[i] = nullptr;
-    if (r >= n) continue;
-    const uint32_t j = (uint32_t)kept[r];
-    const uint32_t t = j / p.c.page, to = (uint32_t)r / p.c.page;
+__device__ __forceinline__ void copy_rows(const EvP& p, int b, int h, int j, int r, int n) {
+  constexpr int LPU = 2 * CH < 32 ? 2 * CH : 32, PER = 32 / LPU, PASS = 2 * CH / LPU, U = 4 / PASS;
+  const int lane = threadIdx.x & 31;
+  int64_t ks = -1, vs = 0, kd = 0, vd = 0;
+  if (lane < n) {
+    const uint32_t t = (uint32_t)j / p.c.page, to = (uint32_t)r / p.c.page;
     const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
     const int64_t pd = (uint32_t)r < p.cap_out ? paged_page(p.c, p.table_out, p.tos, b, to) : -1;
     if (pg < 0 || pd < 0) {
-      if (ch == 0) atomicCAS(p.err, 0, kErrPageEvict);
-      continue;
-    }
-    const uint32_t slot = j - t * p.c.page, ds = (uint32_t)r - to * p.c.page;
-    const char* s = is_v ? p.c.v + pg * p.c.vsp + h * p.c.vsh + slot * p.c.vsn
-                         : p.c.k + pg * p.c.ksp + h * p.c.ksh + slot * p.c.ksn;
-    dst[i] = (is_v ? p.c.v + pd * p.c.vsp + h * p.c.vsh + ds * p.c.vsn
-                   : p.c.k + pd * p.c.ksp + h * p.c.ksh + ds * p.c.ksn) + ch * 16;
-    x[i] = *reinterpret_cast<const uint4*>(s + ch * 16);
-    if (is_v && ch == 0) {
-      wdst[i] = p.c.w + pd * p.c.wsp + h * p.c.wsh + ds;
-      w[i] = p.c.w[pg * p.c.wsp + h * p.c.wsh + slot];
+      atomicCAS(p.err, 0, kErrPageEvict);
+    } else {
+      const int64_t slot = (uint32_t)j - t * p.c.page, ds = (uint32_t)r - to * p.c.page;
+      ks = pg * p.c.ksp + h * p.c.ksh + slot * p.c.ksn;
+      vs = pg * p.c.vsp + h * p.c.vsh + slot * p.c.vsn;
+      kd = pd * p.c.ksp + h * p.c.ksh + ds * p.c.ksn;
+      vd = pd * p.c.vsp + h * p.c.vsh + ds * p.c.vsn;
+      p.c.w[pd * p.c.wsp + h * p.c.wsh + ds] = p.c.w[pg * p.c.wsp + h * p.c.wsh + slot];
     }
   }
+  const int sub = lane / LPU, ch = lane % CH;
+  const bool is_v = PASS == 1 && (lane / CH) % 2 == 1;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += U * PER) {
+    uint4 x[U][PASS];
+    char* to[U][PASS];
 #pragma unroll
-  for (int i = 0; i < kIter; ++i) {
-    if (dst[i]) *reinterpret_cast<uint4*>(dst[i]) = x[i];
-    if (wdst[i]) *wdst[i] = w[i];
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * PER + sub;
+      const int64_t a = __shfl_sync(0xffffffffu, ks, i & 31), c = __shfl_sync(0xffffffffu, kd, i & 31);
+      const int64_t d = __shfl_sync(0xffffffffu, vs, i & 31), e = __shfl_sync(0xffffffffu, vd, i & 31);
+#pragma unroll
+      for (int q = 0; q < PASS; ++q) {
+        const bool v = PASS == 1 ? is_v : q == 1;
+        to[u][q] = i < n && a >= 0 ? (v ? p.c.v + e : p.c.k + c) + ch * 16 : nullptr;
+        if (to[u][q]) x[u][q] = __ldcs(reinterpret_cast<const uint4*>((v ? p.c.v + d : p.c.k + a) + ch * 16));
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int q = 0; q < PASS; ++q)
+        if (to[u][q]) *reinterpret_cast<uint4*>(to[u][q]) = x[u][q];
+  }
+}
+
+template <int CH>
+__global__ void __launch_bounds__(kThreads, 2) paged_evict_kernel(const EvP p) {
+  extern __shared__ uint32_t s_keys[];
+  __shared__ SmemE sm;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int rank = blockIdx.x, CL = gridDim.x;  // the cluster is the grid's first dimension
+  const int h = blockIdx.y, b = blockIdx.z;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int len = paged_len(p.c, b);
+  const int n = (int)min((int64_t)len, p.budget);
+  int32_t* kept = p.kept + ((int64_t)b * p.c.Hkv + h) * p.budget;
+  if (rank == 0 && h == 0 && tid == 0) p.lens_out[b] = n;
+  for (int64_t r = n + (int64_t)rank * kThreads + tid; r < p.budget; r += (int64_t)CL * kThreads) kept[r] = -1;
+  const int per = (len + CL - 1) / CL;
+  const int lo = min(rank * per, len), cnt = min(per, len - lo);  // this CTA's slots
+  if (len <= p.budget) {  // (the same for all CTAs of the cluster)
+    for (int i0 = warp * 32; i0 < cnt; i0 += kThreads) {
+      const int j = lo + i0 + lane;
+      if (i0 + lane < cnt) kept[j] = j;
+      copy_rows<CH>(p, b, h, j, j, min(32, cnt - i0));
+    }
+    return;
+  }
+  uint32_t* keys = p.keys ? p.keys + ((int64_t)b * p.c.Hkv + h) * p.c.cap + lo : s_keys;
+
+  // ---- keys
+  for (int i = tid; i < 3 * kBins; i += kThreads) sm.hist[0][i] = 0u;
+#pragma unroll 4
+  for (int i = tid; i < cnt; i += kThreads) {
+    const int j = lo + i;
+    const uint32_t t = (uint32_t)j / p.c.page;
+    const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
+    uint32_t key = 0u;
+    if (pg < 0) atomicCAS(p.err, 0, kErrPageEvict);
+    else key = weight_key(p.c.w[pg * p.c.wsp + h * p.c.wsh + ((uint32_t)j - t * p.c.page)]);
+    if (j < p.n_global || j >= len - p.n_local) key = 0xffffffffu;
+    keys[i] = key;
+  }
+  __syncthreads();
+
+  // ---- the n-th largest key of all slices, and how many of its equals are kept
+  uint32_t prefix = 0u, mask = 0u, need = (uint32_t)n;
+#pragma unroll 1
+  for (int round = 0; round < 3; ++round) {
+    const int bits = round < 2 ? 11 : 10, shift = round == 0 ? 21 : (round == 1 ? 10 : 0);
+    uint32_t* hist = sm.hist[round];
+    for (int i = tid; i < cnt; i += kThreads) {
+      const uint32_t key = keys[i];
+      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1u)], 1u);
+    }
+    cluster.sync();
+    // this thread's bins of all slices, largest digit first
+    constexpr int PB = kBins / kThreads;
+    uint32_t c[PB], sum = 0;
+#pragma unroll
+    for (int i = 0; i < PB; ++i) c[i] = 0u;
+    const int top = (1 << bits) - 1 - tid * PB;  // digits top, top - 1, ..
+    if (top >= 0)
+      for (int q = 0; q < CL; ++q) {
+        const uint32_t* far = CL == 1 ? hist : cluster.map_shared_rank(hist, q);
+#pragma unroll
+        for (int i = 0; i < PB; ++i) c[i] += far[top - i];
+      }
+#pragma unroll
+    for (int i = 0; i < PB; ++i) sum += c[i];
+    uint32_t all;
+    uint32_t before = block_excl_sum(sum, sm.scan, all);
+#pragma unroll
+    for (int i = 0; i < PB; ++i) {
+      if (before < need && before + c[i] >= need) {
+        sm.digit = (uint32_t)(top - i);
+        sm.rest = need - before;
+      }
+      before += c[i];
+    }
+    __syncthreads();
+    prefix |= sm.digit << shift;
+    mask |= ((1u << bits) - 1u) << shift;
+    need = sm.rest;
+    __syncthreads();
+  }
+
+  // ---- where this slice's kept slots go
+  uint32_t above = 0, equal = 0;
+  for (int i = tid; i < cnt; i += kThreads) {
+    above += keys[i] > prefix;
+    equal += keys[i] == prefix;
+  }
+  uint32_t all_above, all_equal;
+  block_excl_sum(above, sm.scan, all_above);
+  block_excl_sum(equal, sm.scan, all_equal);
+  if (tid == 0) sm.counts = {(int)all_above, (int)all_equal};
+  cluster.sync();
+  int base = 0, ties = (int)need;  // rank of the first kept slot, equals left for this slice and those behind
+  for (int q = 0; q < rank; ++q) {
+    const Counts c = *cluster.map_shared_rank(&sm.counts, q);
+    const int take = min(c.equal, ties);
+    base += c.above + take;
+    ties -= take;
+  }
+  ties = min(ties, (int)all_equal);
+  cluster.sync();  // no CTA ends while another may read its counts
+
+  // ---- compaction in slot order, in place: entry i of the list never lies behind the keys read
+  const int mine = (int)all_above + ties;
+  uint32_t done_above = 0, done_equal = 0;
+  for (int i0 = 0; i0 < cnt; i0 += kChunk) {
+    const int i = i0 + tid * kItems;
+    uint32_t key[kItems], x = 0;
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      key[k] = i + k < cnt ? keys[i + k] : 0u;
+      if (i + k < cnt) x += key[k] > prefix ? 1u : (key[k] == prefix ? 1u << 16 : 0u);
+    }
+    uint32_t all;
+    const uint32_t at = block_excl_sum(x, sm.scan, all);  // (ends behind a barrier: all keys are read)
+    uint32_t a = done_above + (at & 0xffffu), e = done_equal + (at >> 16);
+#pragma unroll
+    for (int k = 0; k < kItems; ++k) {
+      if (i + k >= cnt) break;
+      const bool tie = key[k] == prefix;
+      if (key[k] > prefix || (tie && e < (uint32_t)ties)) keys[a + min(e, (uint32_t)ties)] = (uint32_t)(lo + i + k);
+      a += key[k] > prefix;
+      e += tie;
+    }
+    done_above += all & 0xffffu;
+    done_equal += all >> 16;
+    __syncthreads();
+  }
+
+  // ---- rows
+  for (int i0 = warp * 32; i0 < mine; i0 += kThreads) {
+    const bool in = i0 + lane < mine;
+    const int j = in ? (int)keys[i0 + lane] : 0, r = base + i0 + lane;
+    if (in) kept[r] = j;
+    copy_rows<CH>(p, b, h, j, r, min(32, mine - i0));
   }
 }
 
@@ -196,11 +288,46 @@ int check(const sta_paged_cache* c, const sta_paged_evict_args* a) {
   return STA_OK;
 }
 
+// CTAs of a cluster: enough to fill the GPU (two CTAs per SM) and to hold the keys in shared
+// memory, but slices of 128 slots at least.
+int cluster_size(const sta_paged_cache* c) {
+  const int64_t cap = c->table_width * c->page_size, segs = c->batch * c->n_kv_heads;
+  int cl = 1;
+  while (cl < 8 && cap / cl >= 256 && (segs * cl < 296 || cap / cl > kSliceSmem)) cl *= 2;
+  return cl;
+}
+
+bool keys_in_smem(const sta_paged_cache* c) {
+  const int64_t cap = c->table_width * c->page_size;
+  return (cap + cluster_size(c) - 1) / cluster_size(c) <= kSliceSmem;
+}
+
+template <int CH>
+cudaError_t launch(const EvP& p, int cl, int64_t cap, cudaStream_t st) {
+  const int bytes = p.keys ? 0 : (int)(((cap + cl - 1) / cl) * 4);
+  static bool ready[64];
+  const cudaError_t e = allow_smem(paged_evict_kernel<CH>, kSliceSmem * 4, ready);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)cl, (unsigned)p.c.Hkv, (unsigned)p.c.B);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = (size_t)bytes;
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)cl;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, paged_evict_kernel<CH>, p);
+}
+
 }  // namespace
 
 size_t paged_evict_workspace_bytes(const sta_paged_cache* c, const sta_paged_evict_args* a) {
   if (check(c, a) != STA_OK) return 0;
-  return (size_t)(c->batch * c->n_kv_heads) * (c->table_width * c->page_size) * 4 + 256;
+  const size_t keys = (size_t)(c->batch * c->n_kv_heads) * (c->table_width * c->page_size) * 4;
+  return (keys_in_smem(c) ? 0 : keys) + 256;
 }
 
 int paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* ws, size_t ws_len,
@@ -220,18 +347,13 @@ int paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* w
   p.kept = a->kept;
   p.lens_out = a->lens_out;
   uint8_t* w = static_cast<uint8_t*>(ws);
-  p.keys = reinterpret_cast<uint32_t*>(w + (256 - reinterpret_cast<uintptr_t>(w) % 256) % 256);
+  p.keys = keys_in_smem(c) ? nullptr
+                           : reinterpret_cast<uint32_t*>(w + (256 - reinterpret_cast<uintptr_t>(w) % 256) % 256);
   p.err = device_error_word();
   if (!p.err) return fail(STA_ERR_CUDA, "sta_paged_evict: no device");
-  paged_evict_select_kernel<<<dim3((unsigned)p.c.Hkv, (unsigned)p.c.B), kSel, 0, st>>>(p);
-  const int ch = c->d * (c->dtype == STA_DTYPE_F32 ? 4 : 2) / 16;
-  const int64_t per = (int64_t)kCopy / (2 * ch) * kIter;
-  const int64_t most = p.c.cap < a->budget ? p.c.cap : a->budget;
-  const dim3 grid((unsigned)((most + per - 1) / per), (unsigned)p.c.Hkv, (unsigned)p.c.B);
-  if (ch == 8) paged_evict_copy_kernel<8><<<grid, kCopy, 0, st>>>(p);
-  else if (ch == 16) paged_evict_copy_kernel<16><<<grid, kCopy, 0, st>>>(p);
-  else paged_evict_copy_kernel<32><<<grid, kCopy, 0, st>>>(p);
-  const cudaError_t e = cudaGetLastError();
+  const int ch = c->d * (c->dtype == STA_DTYPE_F32 ? 4 : 2) / 16, cl = cluster_size(c);
+  const cudaError_t e = ch == 8 ? launch<8>(p, cl, p.c.cap, st)
+                                : (ch == 16 ? launch<16>(p, cl, p.c.cap, st) : launch<32>(p, cl, p.c.cap, st));
   return e == cudaSuccess ? STA_OK : fail(STA_ERR_CUDA, cudaGetErrorString(e));
 }
 

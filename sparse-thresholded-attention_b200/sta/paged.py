@@ -18,11 +18,19 @@ import math
 import torch
 
 from . import _lib as L
-from .core import Geometry, _rows, _stream, dtype_code
+from .core import Geometry, dtype_code
 
 
 def _on(t, dev, dtype, shape, name):
     """t is a tensor of this device, type and shape (None entries: any) with a dense last dim."""
+    if torch.is_tensor(t) and t.dtype is dtype and t.device == dev and t.dim() == len(shape):
+        s = t.shape
+        for i, n in enumerate(shape):
+            if n is not None and s[i] != n:
+                break
+        else:
+            if not s or s[-1] <= 1 or t.stride(-1) == 1:
+                return
     if not torch.is_tensor(t) or t.device != dev:
         raise ValueError(f"{name} must be a tensor on {dev}")
     if t.dtype != dtype:
@@ -31,6 +39,31 @@ def _on(t, dev, dtype, shape, name):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"the last dimension of {name} must be contiguous")
+
+
+def _run(cache, name, *args):
+    """Call a library entry with the cache, on the current stream of the cache's device."""
+    dev = cache.device.index
+    if torch._C._cuda_getDevice() == dev:
+        rc = getattr(L.lib(), name)(cache._ref, *args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            rc = getattr(L.lib(), name)(cache._ref, *args, torch._C._cuda_getCurrentRawStream(dev))
+    if rc:
+        L.check(rc, name)
+
+
+def _workspace(cache, name, key, ref):
+    """Scratch of one call (its size depends on the shapes alone and is asked for once).  Every call
+    has its own: torch's allocator keeps it from other streams and from other captured graphs."""
+    n = cache._sizes.get(key)
+    if n is None:
+        with torch.cuda.device(cache.device):
+            n = getattr(L.lib(), name + "_workspace_bytes")(cache._ref, ref)
+        if n == 0:
+            L.check(1, name)
+        cache._sizes[key] = n
+    return torch.empty(n, dtype=torch.uint8, device=cache.device), n
 
 
 class PagedCache:
@@ -48,7 +81,7 @@ class PagedCache:
     outside the pool never faults: its sequence's result is NaN, its rows are dropped, and
     ``core.device_error()`` is 201 (append), 202 (decode) or 203 (evict)."""
 
-    __slots__ = ("k", "v", "table", "lens", "weights", "device", "_args", "_ref")
+    __slots__ = ("k", "v", "table", "lens", "weights", "device", "_args", "_ref", "_sizes")
 
     def __init__(self, k, v, table, lens, weights=None):
         if not (torch.is_tensor(k) and k.is_cuda):
@@ -74,7 +107,7 @@ class PagedCache:
         a.dtype, a.d = code, d
         a.n_pages, a.n_kv_heads, a.page_size = n_pages, hk, page
         a.batch, a.table_width = table.shape
-        self._args, self._ref = a, ctypes.byref(a)
+        self._args, self._ref, self._sizes = a, ctypes.byref(a), {}
 
     @property
     def batch(self):
@@ -83,6 +116,16 @@ class PagedCache:
     def with_pages(self, table, lens):
         """The same pool under other page tables / lengths."""
         return PagedCache(self.k, self.v, table, lens, weights=self.weights)
+
+    def _moved(self, table, lens):
+        """with_pages for a table and lengths that have been checked."""
+        c = PagedCache.__new__(PagedCache)
+        c.k, c.v, c.table, c.lens, c.weights, c.device = self.k, self.v, table, lens, self.weights, self.device
+        a = L.PagedCacheArgs.from_buffer_copy(self._args)
+        a.table, a.table_stride, a.lens = table.data_ptr(), table.stride(0), lens.data_ptr()
+        a.batch, a.table_width = table.shape
+        c._args, c._ref, c._sizes = a, ctypes.byref(a), {}
+        return c
 
 
 def append(cache: PagedCache, k, v, *, counts=None, lens_out=None):
@@ -93,21 +136,29 @@ def append(cache: PagedCache, k, v, *, counts=None, lens_out=None):
     dropped and reported by ``core.device_error()``."""
     a = cache._args
     dev = cache.device
-    shape = (a.batch, a.n_kv_heads, None, a.d)
-    k, v = _rows(k), _rows(v)
-    _on(k, dev, cache.k.dtype, shape, "k")
-    _on(v, dev, cache.k.dtype, k.shape, "v")
+    if not (torch.is_tensor(k) and torch.is_tensor(v)):
+        raise ValueError("k and v must be tensors")
+    shape = (a.batch, a.n_kv_heads, k.shape[2] if k.dim() == 4 else None, a.d)
+    if k.dim() == 4 and k.stride(3) != 1:
+        k = k.contiguous()
+    if v.dim() == 4 and v.stride(3) != 1:
+        v = v.contiguous()
+    dt = cache.k.dtype
+    if not (k.shape == shape and v.shape == shape and k.dtype is dt and v.dtype is dt
+            and k.device == dev and v.device == dev):
+        _on(k, dev, dt, shape, "k")
+        _on(v, dev, dt, shape, "v")
     if counts is not None:
         _on(counts, dev, torch.int32, (a.batch,), "counts")
     if lens_out is None:
         lens_out = cache.lens
     else:
         _on(lens_out, dev, torch.int32, (a.batch,), "lens_out")
-    b = L.PagedAppendArgs(k.data_ptr(), k.stride(0), k.stride(1), k.stride(2),
-                          v.data_ptr(), v.stride(0), v.stride(1), v.stride(2), k.shape[2],
+    kb, kh, kn, _ = k.stride()
+    vb, vh, vn, _ = v.stride()
+    b = L.PagedAppendArgs(k.data_ptr(), kb, kh, kn, v.data_ptr(), vb, vh, vn, shape[2],
                           None if counts is None else counts.data_ptr(), lens_out.data_ptr())
-    with torch.cuda.device(dev):
-        L.check(L.lib().sta_paged_append(cache._ref, ctypes.byref(b), _stream()), "sta_paged_append")
+    _run(cache, "sta_paged_append", ctypes.byref(b))
     return lens_out
 
 
@@ -126,13 +177,14 @@ def decode(q, cache: PagedCache, geometry: Geometry, *, sm_scale=None, weights_o
     dev = cache.device
     _on(q, dev, cache.k.dtype, (a.batch, None, a.d), "q")
     inv = geometry.inv_freq
-    if inv.dtype != torch.float32 or inv.device != dev or not inv.is_contiguous():
+    if inv.dtype is not torch.float32 or inv.device != dev or not inv.is_contiguous():
         inv = inv.to(device=dev, dtype=torch.float32).contiguous()
     if inv.numel() != a.d // 2:
         raise ValueError("inv_freq must have head_dim/2 entries")
     H = q.shape[1]
-    out = torch.empty((a.batch, H, a.d), dtype=q.dtype, device=dev)
-    b = L.PagedDecodeArgs(q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), H, inv.data_ptr(),
+    out = q.new_empty((a.batch, H, a.d))
+    qb, qh, _ = q.stride()
+    b = L.PagedDecodeArgs(q.data_ptr(), qb, qh, out.data_ptr(), H, inv.data_ptr(),
                           geometry.pos_scale, geometry.rope_scale,
                           1.0 / math.sqrt(a.d) if sm_scale is None else sm_scale)
     if geometry.dca is not None:
@@ -146,13 +198,9 @@ def decode(q, cache: PagedCache, geometry: Geometry, *, sm_scale=None, weights_o
         if weights_out.stride() != cache.weights.stride():
             raise ValueError("weights_out must have the strides of the cache's weights")
         b.weights_out = weights_out.data_ptr()
-    lib, ref = L.lib(), ctypes.byref(b)
-    with torch.cuda.device(dev):
-        n = lib.sta_paged_decode_workspace_bytes(cache._ref, ref)
-        if n == 0:
-            L.check(1, "sta_paged_decode")
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        L.check(lib.sta_paged_decode(cache._ref, ref, ws.data_ptr(), n, _stream()), "sta_paged_decode")
+    ref = ctypes.byref(b)
+    ws, n = _workspace(cache, "sta_paged_decode", (H, weights_out is not None), ref)
+    _run(cache, "sta_paged_decode", ref, ws.data_ptr(), n)
     return out
 
 
@@ -171,15 +219,11 @@ def evict(cache: PagedCache, budget: int, table_out, *, n_global=32, n_local=32)
     _on(table_out, dev, torch.int32, (a.batch, None), "table_out")
     if budget <= 0:
         raise ValueError("budget must be positive")
-    kept = torch.empty((a.batch, a.n_kv_heads, budget), dtype=torch.int32, device=dev)
-    lens = torch.empty((a.batch,), dtype=torch.int32, device=dev)
+    kept = table_out.new_empty((a.batch, a.n_kv_heads, budget))
+    lens = table_out.new_empty((a.batch,))
     b = L.PagedEvictArgs(budget, int(n_global), int(n_local), table_out.data_ptr(),
                          table_out.stride(0), table_out.shape[1], kept.data_ptr(), lens.data_ptr())
-    lib, ref = L.lib(), ctypes.byref(b)
-    with torch.cuda.device(dev):
-        n = lib.sta_paged_evict_workspace_bytes(cache._ref, ref)
-        if n == 0:
-            L.check(1, "sta_paged_evict")
-        ws = torch.empty(n, dtype=torch.uint8, device=dev)
-        L.check(lib.sta_paged_evict(cache._ref, ref, ws.data_ptr(), n, _stream()), "sta_paged_evict")
-    return cache.with_pages(table_out, lens), kept
+    ref = ctypes.byref(b)
+    ws, n = _workspace(cache, "sta_paged_evict", ("evict", budget, b.n_global, b.n_local, b.table_out_width), ref)
+    _run(cache, "sta_paged_evict", ref, ws.data_ptr(), n)
+    return cache._moved(table_out, lens), kept
