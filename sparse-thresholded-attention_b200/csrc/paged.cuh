@@ -53,6 +53,77 @@ __device__ __forceinline__ int64_t paged_page(const PagedView& c, const int32_t*
   return pg >= 0 && pg < c.n_pages ? pg : -1;
 }
 
+// Moves up to 32 rows of K and V by one warp: lane l has row l's byte offsets (ks < 0: no row), `n`
+// rows in all.  Neighbouring lanes hold the 16-byte chunks (CH of a row) of K, then of V; eight
+// rows are loaded before the first is stored, which keeps 4 to 8 KB per warp in flight.  VEC:
+// sources lie on 16-byte boundaries; otherwise they are read by elements of `es` bytes.
+template <int CH, bool VEC>
+__device__ __forceinline__ void move_rows(const char* ksrc, const char* vsrc, char* kdst, char* vdst,
+                                          int64_t ks, int64_t vs, int64_t kd, int64_t vd, int n, int es) {
+  constexpr int LPU = 2 * CH < 32 ? 2 * CH : 32;  // lanes of a row
+  constexpr int PER = 32 / LPU, PASS = 2 * CH / LPU, U = 8 / PER / PASS;
+  const int lane = threadIdx.x & 31, sub = lane / LPU, ch = lane % CH;
+  const bool is_v = PASS == 1 && (lane / CH) % 2 == 1;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += U * PER) {
+    uint4 x[U][PASS];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * PER + sub;
+      const int64_t a = __shfl_sync(0xffffffffu, ks, i & 31), c = __shfl_sync(0xffffffffu, vs, i & 31);
+#pragma unroll
+      for (int q = 0; q < PASS; ++q) {
+        const bool v = PASS == 1 ? is_v : q == 1;
+        const char* s = (v ? vsrc + c : ksrc + a) + ch * 16;
+        if (i >= n || a < 0) continue;
+        if (VEC) {
+          x[u][q] = __ldcs(reinterpret_cast<const uint4*>(s));
+        } else if (es == 4) {
+          const uint32_t* e = reinterpret_cast<const uint32_t*>(s);
+          x[u][q] = make_uint4(e[0], e[1], e[2], e[3]);
+        } else {
+          const uint16_t* e = reinterpret_cast<const uint16_t*>(s);
+          x[u][q] = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
+                               e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
+        }
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * PER + sub;
+      const int64_t a = __shfl_sync(0xffffffffu, kd, i & 31), c = __shfl_sync(0xffffffffu, vd, i & 31);
+      const int64_t from = __shfl_sync(0xffffffffu, ks, i & 31);  // (by all lanes, rows or not)
+      const bool in = i < n && from >= 0;
+#pragma unroll
+      for (int q = 0; q < PASS; ++q) {
+        const bool v = PASS == 1 ? is_v : q == 1;
+        if (in) *reinterpret_cast<uint4*>((v ? vdst + c : kdst + a) + ch * 16) = x[u][q];
+      }
+    }
+  }
+}
+
+// Programmatic launch: the next kernel of the stream may be set up from here on / its inputs, the
+// results of the kernel ahead, are complete from here on.
+__device__ __forceinline__ void grid_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Launches a kernel that may begin before the one ahead of it in the stream has ended (it waits
+// for that kernel's results itself), so that its launch does not add to the call.
+template <typename K, typename P>
+inline cudaError_t launch_behind(K kernel, dim3 grid, int threads, const P& p, cudaStream_t st) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.stream = st;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
 // Lets a kernel have `bytes` of dynamic shared memory; asked for once per device (`ready`).
 template <typename K>
 inline cudaError_t allow_smem(K kernel, int bytes, bool (&ready)[64]) {
@@ -82,7 +153,8 @@ inline int paged_check(const sta_paged_cache* c) {
   const int64_t strides[6] = {c->k_stride_p, c->k_stride_h, c->k_stride_n,
                               c->v_stride_p, c->v_stride_h, c->v_stride_n};
   for (int64_t s : strides)
-    if (s * es % 16) return fail(STA_ERR_ARG, "sta_paged: K / V strides must be multiples of 16 bytes");
+    if (s < 0 || s * es % 16)
+      return fail(STA_ERR_ARG, "sta_paged: K / V strides must be non-negative multiples of 16 bytes");
   if ((reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v)) & 15u)
     return fail(STA_ERR_ARG, "sta_paged: K / V must start on a 16-byte boundary");
   return STA_OK;

@@ -1,10 +1,12 @@
 // Rows of new tokens into the pages of their sequences.
 //
 // A pure copy: every row is read once and written once (2 * d * element size bytes each for K
-// and V), so HBM bounds it for prompts and launch latency for single tokens.  One thread moves
-// kIter 16-byte chunks whose loads are all in flight before the first store; chunks of a row lie
-// in neighbouring threads, kv heads of a token in neighbouring rows (the order in which a
-// projection leaves them).  Sources that are not 16-byte aligned take element loads.
+// and V), so HBM bounds it for prompts and launch latency for single tokens.  A warp takes 32
+// (token, kv head) rows, kv heads of a token next to each other (the order in which a projection
+// leaves them): each lane looks up one row's page, then the warp moves the rows.  Sources that
+// are not 16-byte aligned take element loads.
+#include <initializer_list>
+
 #include "paged.cuh"
 
 namespace sta {
@@ -12,7 +14,7 @@ namespace sta {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kIter = 4;
+constexpr int kUnits = kThreads;  // (token, kv head) rows of a block: 32 per warp
 
 struct AppP {
   PagedView c;
@@ -33,59 +35,36 @@ __device__ __forceinline__ int new_len(const AppP& p, int b, int len, int& cnt) 
   return (uint32_t)len + (uint32_t)cnt > p.c.cap ? (int)p.c.cap : len + cnt;
 }
 
-template <bool VEC>
-__device__ __forceinline__ uint4 load_chunk(const char* s, int es) {
-  if (VEC) return *reinterpret_cast<const uint4*>(s);
-  uint4 u;
-  if (es == 4) {
-    const uint32_t* e = reinterpret_cast<const uint32_t*>(s);
-    u = make_uint4(e[0], e[1], e[2], e[3]);
-  } else {
-    const uint16_t* e = reinterpret_cast<const uint16_t*>(s);
-    u = make_uint4(e[0] | (uint32_t)e[1] << 16, e[2] | (uint32_t)e[3] << 16,
-                   e[4] | (uint32_t)e[5] << 16, e[6] | (uint32_t)e[7] << 16);
-  }
-  return u;
-}
-
-// CH: 16-byte chunks of a row (8, 16 or 32); a unit is the K and V row of one (token, kv head).
+// CH: 16-byte chunks of a row (8, 16 or 32)
 template <int CH, bool VEC>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(const AppP p) {
-  constexpr int UNITS = kThreads / (2 * CH);  // units that one pass of the block moves
-  const int tid = threadIdx.x;
-  const int ch = tid % CH, is_v = (tid / CH) & 1, sub = tid / (2 * CH);
+  const int tid = threadIdx.x, lane = tid & 31;
   for (int b = blockIdx.y; b < p.c.B; b += gridDim.y) {
     const int len = paged_len(p.c, b);
     int cnt;
     const int total = new_len(p, b, len, cnt);
-    const int64_t units = (int64_t)cnt * p.c.Hkv;
-    const int64_t u0 = (int64_t)blockIdx.x * (UNITS * kIter) + sub;
-    uint4 x[kIter];
-    char* dst[kIter];
-#pragma unroll
-    for (int i = 0; i < kIter; ++i) {
-      const int64_t u = u0 + i * UNITS;
-      dst[i] = nullptr;
-      if (u >= units) continue;
-      const uint32_t r = (uint32_t)(u / p.c.Hkv), h = (uint32_t)(u - (int64_t)r * p.c.Hkv);
-      const uint32_t j = (uint32_t)len + r;
-      const uint32_t t = j / p.c.page;
-      const int64_t pg = j < p.c.cap ? paged_page(p.c, p.c.table, p.c.ts, b, t) : -1;
-      if (pg < 0) {
-        if (ch == 0) atomicCAS(p.err, 0, kErrPageAppend);
-        continue;
+    const int64_t units = (int64_t)cnt * p.c.Hkv, u0 = (int64_t)blockIdx.x * kUnits + (tid & ~31);
+    const int64_t u = u0 + lane;
+    if (u0 < units) {
+      int64_t ks = -1, vs = 0, kd = 0, vd = 0;
+      if (u < units) {
+        const uint32_t r = (units >> 32) == 0 ? (uint32_t)u / (uint32_t)p.c.Hkv : (uint32_t)(u / p.c.Hkv);
+        const uint32_t h = (uint32_t)(u - (int64_t)r * p.c.Hkv), j = (uint32_t)len + r, t = j / p.c.page;
+        const int64_t pg = j < p.c.cap ? paged_page(p.c, p.c.table, p.c.ts, b, t) : -1;
+        if (pg < 0) {
+          atomicCAS(p.err, 0, kErrPageAppend);
+        } else {
+          const uint32_t slot = j - t * p.c.page;
+          ks = h * p.ksh + r * p.ksn;
+          vs = h * p.vsh + r * p.vsn;
+          kd = pg * p.c.ksp + h * p.c.ksh + slot * p.c.ksn;
+          vd = pg * p.c.vsp + h * p.c.vsh + slot * p.c.vsn;
+          if (p.c.w) p.c.w[pg * p.c.wsp + h * p.c.wsh + slot] = 0.f;
+        }
       }
-      const uint32_t slot = j - t * p.c.page;
-      const char* s = is_v ? p.v + b * p.vsb + h * p.vsh + r * p.vsn
-                           : p.k + b * p.ksb + h * p.ksh + r * p.ksn;
-      dst[i] = (is_v ? p.c.v + pg * p.c.vsp + h * p.c.vsh + slot * p.c.vsn
-                     : p.c.k + pg * p.c.ksp + h * p.c.ksh + slot * p.c.ksn) + ch * 16;
-      x[i] = load_chunk<VEC>(s + ch * 16, p.es);
-      if (p.c.w && ch == 0 && is_v) p.c.w[pg * p.c.wsp + h * p.c.wsh + slot] = 0.f;
+      move_rows<CH, VEC>(p.k + b * p.ksb, p.v + b * p.vsb, p.c.k, p.c.v, ks, vs, kd, vd,
+                         (int)min((int64_t)32, units - u0), p.es);
     }
-#pragma unroll
-    for (int i = 0; i < kIter; ++i)
-      if (dst[i]) *reinterpret_cast<uint4*>(dst[i]) = x[i];
     if (p.store_lens && blockIdx.x == 0) {
       __syncthreads();  // lens_out may be lens: every thread of the (then only) block has read it
       if (tid == 0) p.lens_out[b] = total;
@@ -113,6 +92,8 @@ int paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, cudaS
   if (rc != STA_OK) return rc;
   if (!a || !a->lens_out) return fail(STA_ERR_ARG, "sta_paged_append: null pointer");
   if (a->n < 0 || a->n > ((int64_t)1 << 31) - 65) return fail(STA_ERR_ARG, "sta_paged_append: bad n");
+  for (int64_t x : {a->k_stride_h, a->k_stride_n, a->v_stride_h, a->v_stride_n})
+    if (x < 0) return fail(STA_ERR_ARG, "sta_paged_append: negative stride");
   if (a->n > 0 && (!a->k || !a->v)) return fail(STA_ERR_ARG, "sta_paged_append: null pointer");
   if (a->lens_out != c->lens && a->lens_out < c->lens + c->batch && c->lens < a->lens_out + c->batch)
     return fail(STA_ERR_ARG, "sta_paged_append: lens_out overlaps lens without being it");
@@ -132,8 +113,7 @@ int paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, cudaS
   const bool vec = ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | p.ksb |
                      p.ksh | p.ksn | p.vsb | p.vsh | p.vsn) & 15) == 0;
   const int ch = c->d * p.es / 16;
-  const int64_t per_block = (int64_t)kThreads / (2 * ch) * kIter;
-  const int64_t gx = (a->n * c->n_kv_heads + per_block - 1) / per_block;
+  const int64_t gx = (a->n * c->n_kv_heads + kUnits - 1) / kUnits;
   if (gx > ((int64_t)1 << 31) - 1) return fail(STA_ERR_UNSUPPORTED, "sta_paged_append: too many rows");
   const dim3 grid((unsigned)(gx > 0 ? gx : 1), (unsigned)(c->batch < 65535 ? c->batch : 65535));
   // a length that is overwritten in place is read by one block only, or stored by a second launch

@@ -567,30 +567,14 @@ int launch_f32(const PDecP& p, cudaStream_t st) {
   return launch_f32<D, 8>(p, st);
 }
 
-// Launches a kernel that may begin before the one ahead of it in the stream has ended (it waits
-// for that kernel's results itself), so that its launch does not add to the call.
-template <typename K>
-cudaError_t launch_behind(K kernel, int64_t grid, int threads, const PDecP& p, cudaStream_t st) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, p);
-}
-
 template <typename TV>
 cudaError_t launch_finish(const PDecP& p, int d, cudaStream_t st) {
   const int64_t heads = (int64_t)p.c.B * p.H;
-  cudaError_t e = d == 128 ? launch_behind(paged_join_kernel<128, TV>, heads, kJoin, p, st)
-                           : launch_behind(paged_join_kernel<64, TV>, heads, kJoin, p, st);
+  cudaError_t e = d == 128 ? launch_behind(paged_join_kernel<128, TV>, dim3((unsigned)heads), kJoin, p, st)
+                           : launch_behind(paged_join_kernel<64, TV>, dim3((unsigned)heads), kJoin, p, st);
   if (e == cudaSuccess && p.scores) {
     const int64_t chunks = (p.c.cap + kUpd * kKeysPer - 1) / (kUpd * kKeysPer);
-    e = launch_behind(paged_weights_kernel, (int64_t)p.c.B * p.c.Hkv * chunks, kUpd, p, st);
+    e = launch_behind(paged_weights_kernel, dim3((unsigned)(p.c.B * p.c.Hkv * chunks)), kUpd, p, st);
   }
   return e;
 }

@@ -32,11 +32,6 @@ struct PDecP {
   int* err;
 };
 
-// Programmatic launch: the next kernel of the stream may be set up from here on / its inputs, the
-// results of the kernel ahead, are complete from here on.
-__device__ __forceinline__ void grid_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 __device__ __forceinline__ int n_units(const PDecP& p, int len) {
   return (int)(((uint32_t)len + (1u << p.unit) - 1u) >> p.unit);
 }

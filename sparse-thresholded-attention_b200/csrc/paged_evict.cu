@@ -1,15 +1,18 @@
 // Eviction from a paged cache by accumulated attention weight.
 //
 // Per (sequence, kv head) the min(len, budget) slots to keep are the forced ones (first n_global,
-// last n_local) and the heaviest others, ties to the lowest slot.  One cluster of up to 8 CTAs
-// does all of it for one (sequence, kv head); each CTA holds a contiguous slice of the slots:
-//   1. the weights become order-preserving integer keys in shared memory;
-//   2. the key of the last kept slot is found by radix selection (11 + 11 + 10 bits): every CTA
-//      counts its slice, then reads all CTAs' counts (distributed shared memory) and finds the
-//      digit, so that no CTA waits for a result of another beyond one cluster barrier per digit;
-//   3. each CTA compacts its slice, and copies the rows of K, V and weights that it keeps into the
-//      new pages.  Source and destination pages are disjoint: rows move independently.
-// The kept rows (read and written once) bound it: the selection reads 4 bytes per slot.
+// last n_local) and the heaviest others, ties to the lowest slot.  Two launches:
+//
+// Selection, one CTA per (sequence, kv head), or a cluster of up to 8 where the slots exceed 8192
+// per CTA; each CTA holds a contiguous slice.  The weights become order-preserving integer keys in
+// shared memory; the key of the last kept slot is found by radix selection (11 + 11 + 10 bits):
+// every CTA counts its slice, reads all CTAs' counts (distributed shared memory) and finds the
+// digit, one cluster barrier per digit; then each CTA writes its kept slots in order.  It reads 4
+// bytes per slot and is bound by latency.
+//
+// Copy of the kept rows of K, V and weights into the new pages, 8 to 32 rows per warp wherever
+// they come from, set up while the selection runs (programmatic launch).  Source and destination pages
+// are disjoint, so rows move independently.  Bound by HBM: rows are read and written once.
 #include <cooperative_groups.h>
 
 #include "paged.cuh"
@@ -23,6 +26,8 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
+constexpr int kSlice = 8192;           // slots of a CTA that call for a larger cluster
+constexpr int kCopy = 256;             // threads of the copy
 constexpr int kItems = 8;              // consecutive slots of a thread in the compaction
 constexpr int kChunk = kThreads * kItems;
 constexpr int kSliceSmem = 20 * 1024;  // slots of a slice whose keys fit shared memory (80 KB)
@@ -35,19 +40,17 @@ struct EvP {
   uint32_t cap_out;
   int32_t* kept;
   int32_t* lens_out;
+  int rows;           // rows of a warp in the copy: 8, 16 or 32
+  int quads;          // weights of four neighbouring slots may be loaded at once
   uint32_t* keys;     // (B, Hkv, cap) where a slice exceeds shared memory, else null
   int* err;
 };
 
-struct Counts {
-  int above, equal;
-};
-
-struct SmemE {
+struct __align__(16) SmemE {
   uint32_t hist[3][kBins];  // of each digit (others may still read the one before)
   uint32_t scan[kWarps];
   uint32_t digit, rest;  // the digit found and how many of its slots are kept
-  Counts counts;
+  __align__(16) uint32_t counts[4];  // slots of the slice above the last kept key, and equal to it
 };
 
 // larger weight, larger key; NaN below everything, forced slots above everything
@@ -79,92 +82,73 @@ __device__ __forceinline__ uint32_t block_excl_sum(uint32_t x, uint32_t* sh, uin
   return base + inc - x;
 }
 
-// 32 kept rows of a warp: lane l has slot j (its rank r = r0 + l); `n` of them are rows.  A row's K
-// and V are LPU lanes' 16-byte chunks; four of a lane's loads are in flight.
-template <int CH>
-__device__ __forceinline__ void copy_rows(const EvP& p, int b, int h, int j, int r, int n) {
-  constexpr int LPU = 2 * CH < 32 ? 2 * CH : 32, PER = 32 / LPU, PASS = 2 * CH / LPU, U = 4 / PASS;
-  const int lane = threadIdx.x & 31;
-  int64_t ks = -1, vs = 0, kd = 0, vd = 0;
-  if (lane < n) {
-    const uint32_t t = (uint32_t)j / p.c.page, to = (uint32_t)r / p.c.page;
-    const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
-    const int64_t pd = (uint32_t)r < p.cap_out ? paged_page(p.c, p.table_out, p.tos, b, to) : -1;
-    if (pg < 0 || pd < 0) {
-      atomicCAS(p.err, 0, kErrPageEvict);
-    } else {
-      const int64_t slot = (uint32_t)j - t * p.c.page, ds = (uint32_t)r - to * p.c.page;
-      ks = pg * p.c.ksp + h * p.c.ksh + slot * p.c.ksn;
-      vs = pg * p.c.vsp + h * p.c.vsh + slot * p.c.vsn;
-      kd = pd * p.c.ksp + h * p.c.ksh + ds * p.c.ksn;
-      vd = pd * p.c.vsp + h * p.c.vsh + ds * p.c.vsn;
-      p.c.w[pd * p.c.wsp + h * p.c.wsh + ds] = p.c.w[pg * p.c.wsp + h * p.c.wsh + slot];
-    }
-  }
-  const int sub = lane / LPU, ch = lane % CH;
-  const bool is_v = PASS == 1 && (lane / CH) % 2 == 1;
-#pragma unroll 1
-  for (int i0 = 0; i0 < n; i0 += U * PER) {
-    uint4 x[U][PASS];
-    char* to[U][PASS];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int i = i0 + u * PER + sub;
-      const int64_t a = __shfl_sync(0xffffffffu, ks, i & 31), c = __shfl_sync(0xffffffffu, kd, i & 31);
-      const int64_t d = __shfl_sync(0xffffffffu, vs, i & 31), e = __shfl_sync(0xffffffffu, vd, i & 31);
-#pragma unroll
-      for (int q = 0; q < PASS; ++q) {
-        const bool v = PASS == 1 ? is_v : q == 1;
-        to[u][q] = i < n && a >= 0 ? (v ? p.c.v + e : p.c.k + c) + ch * 16 : nullptr;
-        if (to[u][q]) x[u][q] = __ldcs(reinterpret_cast<const uint4*>((v ? p.c.v + d : p.c.k + a) + ch * 16));
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-#pragma unroll
-      for (int q = 0; q < PASS; ++q)
-        if (to[u][q]) *reinterpret_cast<uint4*>(to[u][q]) = x[u][q];
-  }
+// four words of CTA q's shared memory
+__device__ __forceinline__ uint4 far_words(const uint32_t* mine, int q) {
+  uint32_t a;
+  uint4 x;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_u32(mine)), "r"(q));
+  asm volatile("ld.shared::cluster.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w) : "r"(a));
+  return x;
 }
 
-template <int CH>
-__global__ void __launch_bounds__(kThreads, 2) paged_evict_kernel(const EvP p) {
+__global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP p) {
   extern __shared__ uint32_t s_keys[];
   __shared__ SmemE sm;
   cg::cluster_group cluster = cg::this_cluster();
+  grid_dependents();
   const int rank = blockIdx.x, CL = gridDim.x;  // the cluster is the grid's first dimension
   const int h = blockIdx.y, b = blockIdx.z;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, lane = tid & 31;
   const int len = paged_len(p.c, b);
   const int n = (int)min((int64_t)len, p.budget);
   int32_t* kept = p.kept + ((int64_t)b * p.c.Hkv + h) * p.budget;
   if (rank == 0 && h == 0 && tid == 0) p.lens_out[b] = n;
   for (int64_t r = n + (int64_t)rank * kThreads + tid; r < p.budget; r += (int64_t)CL * kThreads) kept[r] = -1;
-  const int per = (len + CL - 1) / CL;
+  const int per = ((len + CL - 1) / CL + 3) & ~3;
   const int lo = min(rank * per, len), cnt = min(per, len - lo);  // this CTA's slots
   if (len <= p.budget) {  // (the same for all CTAs of the cluster)
-    for (int i0 = warp * 32; i0 < cnt; i0 += kThreads) {
-      const int j = lo + i0 + lane;
-      if (i0 + lane < cnt) kept[j] = j;
-      copy_rows<CH>(p, b, h, j, j, min(32, cnt - i0));
-    }
+    for (int i = tid; i < cnt; i += kThreads) kept[lo + i] = lo + i;
     return;
   }
   uint32_t* keys = p.keys ? p.keys + ((int64_t)b * p.c.Hkv + h) * p.c.cap + lo : s_keys;
 
   // ---- keys
   for (int i = tid; i < 3 * kBins; i += kThreads) sm.hist[0][i] = 0u;
+  auto key_of = [&](int j, float w) {
+    return j < p.n_global || j >= len - p.n_local ? 0xffffffffu : weight_key(w);
+  };
+  if (p.quads) {  // four neighbouring slots share a page and a 16-byte load
 #pragma unroll 4
-  for (int i = tid; i < cnt; i += kThreads) {
-    const int j = lo + i;
-    const uint32_t t = (uint32_t)j / p.c.page;
-    const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
-    uint32_t key = 0u;
-    if (pg < 0) atomicCAS(p.err, 0, kErrPageEvict);
-    else key = weight_key(p.c.w[pg * p.c.wsp + h * p.c.wsh + ((uint32_t)j - t * p.c.page)]);
-    if (j < p.n_global || j >= len - p.n_local) key = 0xffffffffu;
-    keys[i] = key;
+    for (int i = tid * 4; i < cnt; i += kThreads * 4) {
+      const int j = lo + i;
+      const uint32_t t = (uint32_t)j / p.c.page;
+      const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
+      float4 w = make_float4(__int_as_float(0x7fffffff), 0.f, 0.f, 0.f);
+      if (pg < 0) {
+        atomicCAS(p.err, 0, kErrPageEvict);
+        w.y = w.z = w.w = w.x;
+      } else {
+        w = *reinterpret_cast<const float4*>(p.c.w + pg * p.c.wsp + h * p.c.wsh + ((uint32_t)j - t * p.c.page));
+      }
+      const float x[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (i + k < cnt) keys[i + k] = key_of(j + k, x[k]);
+    }
+  } else {
+#pragma unroll 4
+    for (int i = tid; i < cnt; i += kThreads) {
+      const int j = lo + i;
+      const uint32_t t = (uint32_t)j / p.c.page;
+      const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
+      float w = __int_as_float(0x7fffffff);  // of a bad page: the smallest
+      if (pg < 0) atomicCAS(p.err, 0, kErrPageEvict);
+      else w = p.c.w[pg * p.c.wsp + h * p.c.wsh + ((uint32_t)j - t * p.c.page)];
+      keys[i] = key_of(j, w);
+    }
   }
+  if (tid < 4) sm.counts[tid] = 0u;
   __syncthreads();
 
   // ---- the n-th largest key of all slices, and how many of its equals are kept
@@ -175,29 +159,30 @@ __global__ void __launch_bounds__(kThreads, 2) paged_evict_kernel(const EvP p) {
     uint32_t* hist = sm.hist[round];
     for (int i = tid; i < cnt; i += kThreads) {
       const uint32_t key = keys[i];
-      if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & ((1u << bits) - 1u)], 1u);
+      if ((key & mask) == prefix) atomicAdd(&hist[~(key >> shift) & ((1u << bits) - 1u)], 1u);
     }
     cluster.sync();
-    // this thread's bins of all slices, largest digit first
-    constexpr int PB = kBins / kThreads;
-    uint32_t c[PB], sum = 0;
+    // this thread's four bins (bin i counts digit bins - 1 - i) of all slices
+    uint32_t c[4] = {0u, 0u, 0u, 0u};
+    if (tid * 4 < (1 << bits)) {
+      uint4 x[8];
 #pragma unroll
-    for (int i = 0; i < PB; ++i) c[i] = 0u;
-    const int top = (1 << bits) - 1 - tid * PB;  // digits top, top - 1, ..
-    if (top >= 0)
-      for (int q = 0; q < CL; ++q) {
-        const uint32_t* far = CL == 1 ? hist : cluster.map_shared_rank(hist, q);
+      for (int q = 0; q < 8; ++q) x[q] = q < CL ? far_words(hist + tid * 4, q) : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
-        for (int i = 0; i < PB; ++i) c[i] += far[top - i];
+      for (int q = 0; q < 8; ++q) {
+        c[0] += x[q].x;
+        c[1] += x[q].y;
+        c[2] += x[q].z;
+        c[3] += x[q].w;
       }
-#pragma unroll
-    for (int i = 0; i < PB; ++i) sum += c[i];
+    }
+    const uint32_t sum = c[0] + c[1] + c[2] + c[3];
     uint32_t all;
     uint32_t before = block_excl_sum(sum, sm.scan, all);
 #pragma unroll
-    for (int i = 0; i < PB; ++i) {
+    for (int i = 0; i < 4; ++i) {
       if (before < need && before + c[i] >= need) {
-        sm.digit = (uint32_t)(top - i);
+        sm.digit = (uint32_t)((1 << bits) - 1 - tid * 4 - i);
         sm.rest = need - before;
       }
       before += c[i];
@@ -215,23 +200,35 @@ __global__ void __launch_bounds__(kThreads, 2) paged_evict_kernel(const EvP p) {
     above += keys[i] > prefix;
     equal += keys[i] == prefix;
   }
-  uint32_t all_above, all_equal;
-  block_excl_sum(above, sm.scan, all_above);
-  block_excl_sum(equal, sm.scan, all_equal);
-  if (tid == 0) sm.counts = {(int)all_above, (int)all_equal};
-  cluster.sync();
-  int base = 0, ties = (int)need;  // rank of the first kept slot, equals left for this slice and those behind
-  for (int q = 0; q < rank; ++q) {
-    const Counts c = *cluster.map_shared_rank(&sm.counts, q);
-    const int take = min(c.equal, ties);
-    base += c.above + take;
-    ties -= take;
+  above = __reduce_add_sync(0xffffffffu, above);
+  equal = __reduce_add_sync(0xffffffffu, equal);
+  if (lane == 0) {
+    atomicAdd(&sm.counts[0], above);
+    atomicAdd(&sm.counts[1], equal);
   }
-  ties = min(ties, (int)all_equal);
-  cluster.sync();  // no CTA ends while another may read its counts
+  cluster.sync();
+  // lane q: slots of slice q above and equal; the equals go to the slices in order
+  uint4 c = lane < CL ? far_words(sm.counts, lane) : make_uint4(0u, 0u, 0u, 0u);
+  cluster.barrier_arrive();  // (waited for at the end: no CTA goes while another may read its counts)
+  uint32_t eq = c.y;
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, eq, o);
+    if (lane >= o) eq += y;
+  }
+  const uint32_t eq_before = eq - c.y, take = eq_before >= need ? 0u : min(c.y, need - eq_before);
+  const uint32_t holds = c.x + take;  // kept slots of slice q
+  uint32_t upto = holds;
+#pragma unroll
+  for (int o = 1; o < 8; o <<= 1) {
+    const uint32_t y = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += y;
+  }
+  const int base = (int)__shfl_sync(0xffffffffu, upto - holds, rank);
+  const uint32_t ties = __shfl_sync(0xffffffffu, take, rank);
+  const int mine = (int)__shfl_sync(0xffffffffu, holds, rank);
 
-  // ---- compaction in slot order, in place: entry i of the list never lies behind the keys read
-  const int mine = (int)all_above + ties;
+  // ---- the kept slots in order
   uint32_t done_above = 0, done_equal = 0;
   for (int i0 = 0; i0 < cnt; i0 += kChunk) {
     const int i = i0 + tid * kItems;
@@ -242,28 +239,54 @@ __global__ void __launch_bounds__(kThreads, 2) paged_evict_kernel(const EvP p) {
       if (i + k < cnt) x += key[k] > prefix ? 1u : (key[k] == prefix ? 1u << 16 : 0u);
     }
     uint32_t all;
-    const uint32_t at = block_excl_sum(x, sm.scan, all);  // (ends behind a barrier: all keys are read)
+    const uint32_t at = block_excl_sum(x, sm.scan, all);
     uint32_t a = done_above + (at & 0xffffu), e = done_equal + (at >> 16);
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
       if (i + k >= cnt) break;
       const bool tie = key[k] == prefix;
-      if (key[k] > prefix || (tie && e < (uint32_t)ties)) keys[a + min(e, (uint32_t)ties)] = (uint32_t)(lo + i + k);
+      if (key[k] > prefix || (tie && e < ties)) kept[base + a + min(e, ties)] = lo + i + k;
       a += key[k] > prefix;
       e += tie;
     }
     done_above += all & 0xffffu;
     done_equal += all >> 16;
-    __syncthreads();
   }
+  cluster.barrier_wait();
+}
 
-  // ---- rows
-  for (int i0 = warp * 32; i0 < mine; i0 += kThreads) {
-    const bool in = i0 + lane < mine;
-    const int j = in ? (int)keys[i0 + lane] : 0, r = base + i0 + lane;
-    if (in) kept[r] = j;
-    copy_rows<CH>(p, b, h, j, r, min(32, mine - i0));
+template <int CH>
+__global__ void __launch_bounds__(kCopy) paged_evict_copy_kernel(const EvP p) {
+  const int lane = threadIdx.x & 31, h = blockIdx.y, b = blockIdx.z;
+  const int n = (int)min((int64_t)paged_len(p.c, b), p.budget);
+  const int r0 = (int)(blockIdx.x * (kCopy / 32) + threadIdx.x / 32) * p.rows, r = r0 + lane;
+  const int end = min(n, r0 + p.rows);
+  int64_t kd = 0, vd = 0, wd = -1;
+  if (r < end) {
+    const uint32_t to = (uint32_t)r / p.c.page, ds = (uint32_t)r - to * p.c.page;
+    const int64_t pd = (uint32_t)r < p.cap_out ? paged_page(p.c, p.table_out, p.tos, b, to) : -1;
+    if (pd >= 0) {
+      kd = pd * p.c.ksp + h * p.c.ksh + ds * p.c.ksn;
+      vd = pd * p.c.vsp + h * p.c.vsh + ds * p.c.vsn;
+      wd = pd * p.c.wsp + h * p.c.wsh + ds;
+    }
   }
+  grid_wait();
+  if (r0 >= n) return;
+  int64_t ks = -1, vs = 0;
+  if (r < end) {
+    const uint32_t j = (uint32_t)p.kept[((int64_t)b * p.c.Hkv + h) * p.budget + r];
+    const uint32_t t = j / p.c.page, slot = j - t * p.c.page;
+    const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
+    if (pg < 0 || wd < 0) {
+      atomicCAS(p.err, 0, kErrPageEvict);
+    } else {
+      ks = pg * p.c.ksp + h * p.c.ksh + slot * p.c.ksn;
+      vs = pg * p.c.vsp + h * p.c.vsh + slot * p.c.vsn;
+      p.c.w[wd] = p.c.w[pg * p.c.wsp + h * p.c.wsh + slot];
+    }
+  }
+  move_rows<CH, true>(p.c.k, p.c.v, p.c.k, p.c.v, ks, vs, kd, vd, end - r0, 0);
 }
 
 int check(const sta_paged_cache* c, const sta_paged_evict_args* a) {
@@ -288,30 +311,26 @@ int check(const sta_paged_cache* c, const sta_paged_evict_args* a) {
   return STA_OK;
 }
 
-// CTAs of a cluster: enough to fill the GPU (two CTAs per SM) and to hold the keys in shared
-// memory, but slices of 128 slots at least.
 int cluster_size(const sta_paged_cache* c) {
-  const int64_t cap = c->table_width * c->page_size, segs = c->batch * c->n_kv_heads;
+  const int64_t cap = c->table_width * c->page_size;
   int cl = 1;
-  while (cl < 8 && cap / cl >= 256 && (segs * cl < 296 || cap / cl > kSliceSmem)) cl *= 2;
+  while (cl < 8 && cap / cl > kSlice) cl *= 2;
   return cl;
 }
 
 bool keys_in_smem(const sta_paged_cache* c) {
   const int64_t cap = c->table_width * c->page_size;
-  return (cap + cluster_size(c) - 1) / cluster_size(c) <= kSliceSmem;
+  return (cap + cluster_size(c) - 1) / cluster_size(c) + 3 <= kSliceSmem;
 }
 
-template <int CH>
-cudaError_t launch(const EvP& p, int cl, int64_t cap, cudaStream_t st) {
-  const int bytes = p.keys ? 0 : (int)(((cap + cl - 1) / cl) * 4);
+cudaError_t launch_select(const EvP& p, int cl, cudaStream_t st) {
   static bool ready[64];
-  const cudaError_t e = allow_smem(paged_evict_kernel<CH>, kSliceSmem * 4, ready);
+  const cudaError_t e = allow_smem(paged_evict_select_kernel, kSliceSmem * 4, ready);
   if (e != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)cl, (unsigned)p.c.Hkv, (unsigned)p.c.B);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = (size_t)bytes;
+  cfg.dynamicSmemBytes = p.keys ? 0 : ((size_t)(p.c.cap + cl - 1) / cl + 3) * 4;
   cfg.stream = st;
   cudaLaunchAttribute attr;
   attr.id = cudaLaunchAttributeClusterDimension;
@@ -319,7 +338,7 @@ cudaError_t launch(const EvP& p, int cl, int64_t cap, cudaStream_t st) {
   attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_evict_kernel<CH>, p);
+  return cudaLaunchKernelEx(&cfg, paged_evict_select_kernel, p);
 }
 
 }  // namespace
@@ -349,11 +368,21 @@ int paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* w
   uint8_t* w = static_cast<uint8_t*>(ws);
   p.keys = keys_in_smem(c) ? nullptr
                            : reinterpret_cast<uint32_t*>(w + (256 - reinterpret_cast<uintptr_t>(w) % 256) % 256);
+  p.quads = p.c.page % 4 == 0 && (reinterpret_cast<uintptr_t>(p.c.w) & 15) == 0 && p.c.wsp % 4 == 0 && p.c.wsh % 4 == 0;
   p.err = device_error_word();
   if (!p.err) return fail(STA_ERR_CUDA, "sta_paged_evict: no device");
-  const int ch = c->d * (c->dtype == STA_DTYPE_F32 ? 4 : 2) / 16, cl = cluster_size(c);
-  const cudaError_t e = ch == 8 ? launch<8>(p, cl, p.c.cap, st)
-                                : (ch == 16 ? launch<16>(p, cl, p.c.cap, st) : launch<32>(p, cl, p.c.cap, st));
+  const int ch = c->d * (c->dtype == STA_DTYPE_F32 ? 4 : 2) / 16;
+  const int64_t most = p.c.cap < a->budget ? p.c.cap : a->budget;
+  // a warp has few rows where that is what it takes to give 16 warps to every SM
+  p.rows = 32;
+  while (p.rows > 8 && most * p.c.Hkv * p.c.B < (int64_t)p.rows * 16 * 148) p.rows /= 2;
+  const int64_t per = (int64_t)p.rows * (kCopy / 32);
+  const dim3 grid((unsigned)((most + per - 1) / per), (unsigned)p.c.Hkv, (unsigned)p.c.B);
+  cudaError_t e = launch_select(p, cluster_size(c), st);
+  if (e == cudaSuccess)
+    e = ch == 8 ? launch_behind(paged_evict_copy_kernel<8>, grid, kCopy, p, st)
+                : (ch == 16 ? launch_behind(paged_evict_copy_kernel<16>, grid, kCopy, p, st)
+                            : launch_behind(paged_evict_copy_kernel<32>, grid, kCopy, p, st));
   return e == cudaSuccess ? STA_OK : fail(STA_ERR_CUDA, cudaGetErrorString(e));
 }
 

@@ -118,12 +118,12 @@ class PagedCache:
         return PagedCache(self.k, self.v, table, lens, weights=self.weights)
 
     def _moved(self, table, lens):
-        """with_pages for a table and lengths that have been checked."""
+        """with_pages for a table (of the same batch) and lengths that have been checked."""
         c = PagedCache.__new__(PagedCache)
         c.k, c.v, c.table, c.lens, c.weights, c.device = self.k, self.v, table, lens, self.weights, self.device
         a = L.PagedCacheArgs.from_buffer_copy(self._args)
-        a.table, a.table_stride, a.lens = table.data_ptr(), table.stride(0), lens.data_ptr()
-        a.batch, a.table_width = table.shape
+        a.table, a.lens = table.data_ptr(), lens.data_ptr()
+        a.table_stride, a.table_width = table.stride(0), table.shape[1]
         c._args, c._ref, c._sizes = a, ctypes.byref(a), {}
         return c
 
