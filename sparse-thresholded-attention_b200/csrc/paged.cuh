@@ -19,7 +19,7 @@ struct PagedView {
   int64_t ts;
   const int32_t* lens;
   int64_t n_pages;
-  uint32_t page, cap;                    // page size, slots that a table row can name
+  uint32_t page, width, cap;             // page size, entries of a table row, slots it can name
   int B, Hkv;
 };
 
@@ -35,6 +35,7 @@ inline PagedView paged_view(const sta_paged_cache* c) {
   v.lens = c->lens;
   v.n_pages = c->n_pages;
   v.page = (uint32_t)c->page_size;
+  v.width = (uint32_t)c->table_width;
   v.cap = (uint32_t)(c->table_width * c->page_size);
   v.B = (int)c->batch;
   v.Hkv = (int)c->n_kv_heads;

@@ -323,9 +323,7 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
   }
 }
 
-constexpr int kJoin = 512;      // threads of the joining kernel
-constexpr int kUpd = 256;       // threads of the weights update, kKeysPer keys each
-constexpr int kKeysPer = 4;
+constexpr int kUpd = 256;       // threads of the weights update, four keys each
 
 // The shares [w0, w1] that cut a segment; one share (w0 == w1) has finished it.  Of the others, w0
 // holds its first unit and left partial 2 w0 + 1; share w behind it left partial 2 w.
@@ -351,11 +349,11 @@ __device__ __forceinline__ Cut cut_of(const PDecP& p, int b, int hg, int units) 
 __device__ __forceinline__ int64_t slot_of(const Cut& c, int64_t w) { return 2 * w + (w == c.w0 ? 1 : 0); }
 
 // One block per (sequence, q head) joins the partials of the shares that cut its segment: each of
-// 16 warps joins every 16th, eight of them in flight, then the warps' results are joined.  Empty
+// NW warps joins every NW-th, eight of them in flight, then the warps' results are joined.  Empty
 // sequences give zeros.
-template <int D, typename TV>
-__global__ void __launch_bounds__(kJoin) paged_join_kernel(const PDecP p) {
-  constexpr int NW = kJoin / 32, V = D / 32, U = 8;
+template <int D, typename TV, int NW>
+__global__ void __launch_bounds__(NW * 32) paged_join_kernel(const PDecP p) {
+  constexpr int V = D / 32, U = 8;
   __shared__ float s_o[NW][D];
   __shared__ float2 s_ml[NW];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -414,7 +412,7 @@ __global__ void __launch_bounds__(kJoin) paged_join_kernel(const PDecP p) {
   for (int i = 0; i < V; ++i) s_o[warp][lane * V + i] = o[i];
   if (lane == 0) s_ml[warp] = make_float2(M, L);
   __syncthreads();
-  if (tid < D) {
+  if (tid < D) {  // (NW >= 4: there are that many threads)
     float m = -INFINITY;
 #pragma unroll
     for (int i = 0; i < NW; ++i) m = fmaxf(m, s_ml[i].x);
@@ -432,48 +430,66 @@ __global__ void __launch_bounds__(kJoin) paged_join_kernel(const PDecP p) {
 }
 
 // weights_out[j] = weights[j] + sum_g exp2(s_gj - M_g) / L_g, 1024 keys of a (sequence, kv head)
-// per block.
+// per block.  QUADS: a thread's four neighbouring keys share a page and 16-byte accesses (page size
+// and strides multiples of four); otherwise each key is looked up.
+template <bool QUADS>
 __global__ void __launch_bounds__(kUpd) paged_weights_kernel(const PDecP p) {
-  const int64_t chunks = (p.c.cap + kUpd * kKeysPer - 1) / (kUpd * kKeysPer), seg = blockIdx.x / chunks;
-  const int b = (int)(seg / p.c.Hkv), h = (int)(seg % p.c.Hkv);
+  const int64_t chunks = (p.c.cap + kUpd * 4 - 1) / (kUpd * 4), seg = div_fast(blockIdx.x, chunks);
+  const int b = (int)div_fast(seg, p.c.Hkv), h = (int)(seg - (int64_t)b * p.c.Hkv);
   const int len = paged_len(p.c, b);
-  const int j0 = (int)(blockIdx.x % chunks) * (kUpd * kKeysPer) + threadIdx.x;
-  if (j0 - (int)threadIdx.x >= len) {
+  const int j = ((int)(blockIdx.x - seg * chunks) * kUpd + (int)threadIdx.x) * 4;  // this thread's first key
+  if (j >= len) {
     grid_wait();  // no block of a chain of programmatic launches ends before the kernel ahead has
     return;
   }
-  float sum[kKeysPer], old[kKeysPer];
-  int64_t to[kKeysPer];
+  int64_t to[QUADS ? 1 : 4];
 #pragma unroll
-  for (int i = 0; i < kKeysPer; ++i) {
-    const int j = j0 + i * kUpd;
-    sum[i] = old[i] = 0.f;
+  for (int i = 0; i < (QUADS ? 1 : 4); ++i) {
     to[i] = -1;
-    if (j < len) {
-      const uint32_t t = (uint32_t)j / p.c.page;
-      const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
-      if (pg >= 0) to[i] = pg * p.c.wsp + h * p.c.wsh + ((uint32_t)j - t * p.c.page);
-    }
+    if (j + i >= len) continue;
+    const uint32_t t = (uint32_t)(j + i) / p.c.page;
+    const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
+    if (pg >= 0) to[i] = pg * p.c.wsp + h * p.c.wsh + ((uint32_t)(j + i) - t * p.c.page);
   }
-#pragma unroll
-  for (int i = 0; i < kKeysPer; ++i)
-    if (to[i] >= 0) old[i] = p.c.w[to[i]];
+  float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (QUADS) {
+    if (to[0] >= 0) w = *reinterpret_cast<const float4*>(p.c.w + to[0]);
+  } else {
+    if (to[0] >= 0) w.x = p.c.w[to[0]];
+    if (to[QUADS ? 0 : 1] >= 0) w.y = p.c.w[to[QUADS ? 0 : 1]];
+    if (to[QUADS ? 0 : 2] >= 0) w.z = p.c.w[to[QUADS ? 0 : 2]];
+    if (to[QUADS ? 0 : 3] >= 0) w.w = p.c.w[to[QUADS ? 0 : 3]];
+  }
   grid_wait();
   const float2* ml = p.ml + (int64_t)b * p.H + h * p.G;
-  const float* sc = p.scores + ((int64_t)b * p.c.Hkv + h) * p.NG * p.cap_tiles * p.GT * kTile;
+  const float* sc = p.scores + (((int64_t)b * p.c.Hkv + h) * p.NG * p.cap_tiles + j / kTile) * p.GT * kTile + j % kTile;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int grp = 0; grp < p.NG; ++grp, sc += p.cap_tiles * p.GT * kTile) {
+    const int heads = min(p.GT, p.G - grp * p.GT);
 #pragma unroll 4
-  for (int g = 0; g < p.G; ++g) {
-    const float2 x = ml[g];
-    const int64_t row = (int64_t)(g / p.GT) * p.cap_tiles * p.GT + g % p.GT;
-#pragma unroll
-    for (int i = 0; i < kKeysPer; ++i) {
-      const int j = j0 + i * kUpd;
-      if (j < len) sum[i] += exp2f(sc[(row + (int64_t)(j / kTile) * p.GT) * kTile + j % kTile] - x.x) * x.y;
+    for (int g = 0; g < heads; ++g) {
+      const float2 x = ml[grp * p.GT + g];
+      const float4 s = *reinterpret_cast<const float4*>(sc + g * kTile);
+      sum.x = fmaf(exp2f(s.x - x.x), x.y, sum.x);
+      sum.y = fmaf(exp2f(s.y - x.x), x.y, sum.y);
+      sum.z = fmaf(exp2f(s.z - x.x), x.y, sum.z);
+      sum.w = fmaf(exp2f(s.w - x.x), x.y, sum.w);
     }
   }
+  w.x += sum.x;
+  w.y += sum.y;
+  w.z += sum.z;
+  w.w += sum.w;
+  if (QUADS && j + 4 <= len) {
+    if (to[0] >= 0) *reinterpret_cast<float4*>(p.w_out + to[0]) = w;
+    return;
+  }
+  const float x[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-  for (int i = 0; i < kKeysPer; ++i)
-    if (to[i] >= 0) p.w_out[to[i]] = old[i] + sum[i];
+  for (int i = 0; i < 4; ++i) {
+    const int64_t at = QUADS ? (to[0] >= 0 && j + i < len ? to[0] + i : -1) : to[QUADS ? 0 : i];
+    if (at >= 0) p.w_out[at] = x[i];
+  }
 }
 
 struct PLayout {
@@ -567,14 +583,26 @@ int launch_f32(const PDecP& p, cudaStream_t st) {
   return launch_f32<D, 8>(p, st);
 }
 
+template <int D, typename TV>
+cudaError_t launch_join(const PDecP& p, cudaStream_t st) {
+  const dim3 grid((unsigned)((int64_t)p.c.B * p.H));
+  // partials of a segment, where all sequences are alike: 16 warps join them for a few long
+  // sequences, 4 where there are many segments and few partials of each
+  const int64_t each = p.W / ((int64_t)p.c.B * p.c.Hkv * p.NG);
+  return each > 32 ? launch_behind(paged_join_kernel<D, TV, 16>, grid, 512, p, st)
+                   : launch_behind(paged_join_kernel<D, TV, 4>, grid, 128, p, st);
+}
+
 template <typename TV>
 cudaError_t launch_finish(const PDecP& p, int d, cudaStream_t st) {
-  const int64_t heads = (int64_t)p.c.B * p.H;
-  cudaError_t e = d == 128 ? launch_behind(paged_join_kernel<128, TV>, dim3((unsigned)heads), kJoin, p, st)
-                           : launch_behind(paged_join_kernel<64, TV>, dim3((unsigned)heads), kJoin, p, st);
+  cudaError_t e = d == 128 ? launch_join<128, TV>(p, st) : launch_join<64, TV>(p, st);
   if (e == cudaSuccess && p.scores) {
-    const int64_t chunks = (p.c.cap + kUpd * kKeysPer - 1) / (kUpd * kKeysPer);
-    e = launch_behind(paged_weights_kernel, dim3((unsigned)(p.c.B * p.c.Hkv * chunks)), kUpd, p, st);
+    const int64_t chunks = (p.c.cap + kUpd * 4 - 1) / (kUpd * 4);
+    const dim3 grid((unsigned)(p.c.B * p.c.Hkv * chunks));
+    const bool quads = p.c.page % 4 == 0 && p.c.wsp % 4 == 0 && p.c.wsh % 4 == 0 &&
+                       ((reinterpret_cast<uintptr_t>(p.c.w) | reinterpret_cast<uintptr_t>(p.w_out)) & 15) == 0;
+    e = quads ? launch_behind(paged_weights_kernel<true>, grid, kUpd, p, st)
+              : launch_behind(paged_weights_kernel<false>, grid, kUpd, p, st);
   }
   return e;
 }

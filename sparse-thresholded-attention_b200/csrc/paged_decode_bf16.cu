@@ -137,15 +137,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
   const int fr = lane >> 2, fc = lane & 3;
 
   grid_dependents();
-  // ---- cos / sin of the key offsets t * pos_scale, t = 0 .. 63, by all warps: t = 8 i + j as the
-  // product of the turns by 8 i and by j (16 sincos per frequency instead of 64)
-  const int len0 = first_len(p.c);
-  for (int i = threadIdx.x; i < 16 * HALF; i += NW * 32) {
-    const int f = i % HALF, t = i / HALF;
-    turn((double)(t < 8 ? t : (t - 8) * 8) * p.pos_scale, __ldg(p.inv_freq + f), sm.turns[t][f].x, sm.turns[t][f].y);
-  }
+  // The start is a chain of loads (lengths, page table, rows) that nothing may stand ahead of: what
+  // can be computed meanwhile comes once the rows have been asked for.
   const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;
-  const Share share = find_share(p, me, len0);
+  const Share share = find_share(p, me, first_len(p.c));
   const int count = share.count;
   Place nx = share.at;              // the unit whose K rows are loaded next
   Rows rows{-1, 0, 0, true};
@@ -263,42 +258,52 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
     asm volatile("cp.async.commit_group;\n" ::: "memory");
   };
 
-  // ---- a segment's raw queries, as the lanes rotate them
-  auto raw_queries = [&](const int4& at) {
+  // ---- a segment's raw queries, as the lanes rotate them: asked for, then stored
+  uint32_t raw[NT][NH][4];
+  auto ask_queries = [&](const int4& at) {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int g = at.z * GT + nt * 8 + fr;
       const uint16_t* src = static_cast<const uint16_t*>(p.q) + at.x * p.qsb + (at.y * p.G + g) * p.qsh + fc * 2;
 #pragma unroll
-      for (int ks = 0; ks < NH; ++ks) {
-        uint32_t x[4] = {0u, 0u, 0u, 0u};
-        if (g < p.G) {
+      for (int ks = 0; ks < NH; ++ks)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int d = ks * 16 + (i & 1) * 8 + (i >> 1) * HALF;
-            x[i] = p.q_words ? *reinterpret_cast<const uint32_t*>(src + d) : src[d] | (uint32_t)src[d + 1] << 16;
-          }
+        for (int i = 0; i < 4; ++i) {
+          const int d = ks * 16 + (i & 1) * 8 + (i >> 1) * HALF;
+          raw[nt][ks][i] = 0u;
+          if (g < p.G)
+            raw[nt][ks][i] = p.q_words ? *reinterpret_cast<const uint32_t*>(src + d)
+                                       : src[d] | (uint32_t)src[d + 1] << 16;
         }
-        sm.q[warp][nt][ks][lane] = make_uint4(x[0], x[1], x[2], x[3]);
-      }
     }
+  };
+  auto keep_queries = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int ks = 0; ks < NH; ++ks)
+        sm.q[warp][nt][ks][lane] = make_uint4(raw[nt][ks][0], raw[nt][ks][1], raw[nt][ks][2], raw[nt][ks][3]);
   };
   const char* vcur = p.c.v;   // the V rows that follow next
   int64_t vocur = 0;
   int vlcur = 0;
   if (count > 0) {
     lookup(true);
-    // (ahead of the rows: what is asked for behind them waits until they have come)
-    raw_queries(make_int4(share.at.b, share.at.h, share.at.grp, 0));
-  }
-  __syncthreads();
-  if (count > 0) {
+    ask_queries(make_int4(share.at.b, share.at.h, share.at.grp, 0));
     load_k();
     vcur = vnext; vocur = vonext; vlcur = vleft;
     load_v(0, vcur, vocur, vlcur);
     load_k();
     vcur = vnext; vocur = vonext; vlcur = vleft;
+    keep_queries();
   }
+  // ---- cos / sin of the key offsets t * pos_scale, t = 0 .. 63, by all warps: t = 8 i + j as the
+  // product of the turns by 8 i and by j (16 sincos per frequency instead of 64)
+  for (int i = threadIdx.x; i < 16 * HALF; i += NW * 32) {
+    const int f = i % HALF, t = i / HALF;
+    turn((double)(t < 8 ? t : (t - 8) * 8) * p.pos_scale, __ldg(p.inv_freq + f), sm.turns[t][f].x, sm.turns[t][f].y);
+  }
+  __syncthreads();
   for (int i = threadIdx.x; i < 4 * NH * 4 * 32; i += NW * 32) {
     const int l = i & 31, r = (i >> 5) & 3, ks = (i >> 7) % NH, u = i / (128 * NH);
     const int f = ks * 16 + (l & 3) * 2 + (r >> 1) * 8;
@@ -361,7 +366,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
           ac[e] = c;
         }
       }
-      if (fresh_seg && it > 0) raw_queries(at);
+      if (fresh_seg && it > 0) {
+        ask_queries(at);
+        keep_queries();
+      }
 #pragma unroll
       for (int e = 0; e < FPL; ++e) {
         float* x = reinterpret_cast<float*>(&sm.ang[warp][(lane * FPL + e) / 2]) + ((lane * FPL + e) & 1);
