@@ -42,6 +42,7 @@ struct SmemB {
   float4 ang[NW][D / 4];                  // (cos, cos, sin, sin) of the query's angle, two dims, times the scale
   uint4 q[NW][NT][D / 32][32];            // a lane's raw queries of a k step: dims 0, 8, d/2, d/2 + 8 on, two each
   float2 turns[16][D / 2];                // cos / sin of turns by 0 .. 7 and by 0, 8 .. 56 positions
+  float inv_freq[D / 2];
   int4 seg[NW][4];                        // segments entered by the loads: sequence, kv head, group, length
 };
 
@@ -139,6 +140,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
   grid_dependents();
   // The start is a chain of loads (lengths, page table, rows) that nothing may stand ahead of: what
   // can be computed meanwhile comes once the rows have been asked for.
+  static_assert(NW * 32 % HALF == 0, "a thread's turns share one frequency");
+  const float my_freq = __ldg(p.inv_freq + threadIdx.x % HALF);
   const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;
   const Share share = find_share(p, me, first_len(p.c));
   const int count = share.count;
@@ -301,8 +304,9 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
   // product of the turns by 8 i and by j (16 sincos per frequency instead of 64)
   for (int i = threadIdx.x; i < 16 * HALF; i += NW * 32) {
     const int f = i % HALF, t = i / HALF;
-    turn((double)(t < 8 ? t : (t - 8) * 8) * p.pos_scale, __ldg(p.inv_freq + f), sm.turns[t][f].x, sm.turns[t][f].y);
+    turn((double)(t < 8 ? t : (t - 8) * 8) * p.pos_scale, my_freq, sm.turns[t][f].x, sm.turns[t][f].y);
   }
+  if (threadIdx.x < HALF) sm.inv_freq[threadIdx.x] = my_freq;
   __syncthreads();
   for (int i = threadIdx.x; i < 4 * NH * 4 * 32; i += NW * 32) {
     const int l = i & 31, r = (i >> 5) & 3, ks = (i >> 7) % NH, u = i / (128 * NH);
@@ -320,7 +324,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
   float ac[FPL], as[FPL], dc[FPL], ds[FPL];
 #pragma unroll
   for (int e = 0; e < FPL; ++e) {
-    turn(-(double)kTile * p.pos_scale, __ldg(p.inv_freq + lane * FPL + e), dc[e], ds[e]);
+    turn(-(double)kTile * p.pos_scale, sm.inv_freq[lane * FPL + e], dc[e], ds[e]);
     ac[e] = as[e] = 0.f;
   }
   uint32_t qb[NT][2 * NH][4];      // B fragments of a k step: hi b0, hi b1, lo b0, lo b1
@@ -357,7 +361,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
       if (it == 0 || tile % kRenew == 0 || (p.L > 0 && tile * kTile % p.L == 0)) {
         const double x = query_offset(p, len, tile);
 #pragma unroll
-        for (int e = 0; e < FPL; ++e) turn(x, __ldg(p.inv_freq + lane * FPL + e), ac[e], as[e]);
+        for (int e = 0; e < FPL; ++e) turn(x, sm.inv_freq[lane * FPL + e], ac[e], as[e]);
       } else {
 #pragma unroll
         for (int e = 0; e < FPL; ++e) {
