@@ -79,7 +79,8 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
   S& sm = *reinterpret_cast<S*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   grid_dependents();
-  const Share share = find_share(p, blockIdx.x, first_len(p.c));
+  int64_t me;
+  const Share share = find_share<false>(p, first_len(p.c), me);
   const int count = share.count;
   if (count == 0) return;
   Place cur = share.at;
@@ -349,11 +350,11 @@ __device__ __forceinline__ Cut cut_of(const PDecP& p, int b, int hg, int units) 
 __device__ __forceinline__ int64_t slot_of(const Cut& c, int64_t w) { return 2 * w + (w == c.w0 ? 1 : 0); }
 
 // One block per (sequence, q head) joins the partials of the shares that cut its segment: each of
-// NW warps joins every NW-th, eight of them in flight, then the warps' results are joined.  Empty
+// NW warps joins every NW-th, four of them in flight, then the warps' results are joined.  Empty
 // sequences give zeros.
 template <int D, typename TV, int NW>
 __global__ void __launch_bounds__(NW * 32) paged_join_kernel(const PDecP p) {
-  constexpr int V = D / 32, U = 8;
+  constexpr int V = D / 32, U = 4;
   __shared__ float s_o[NW][D];
   __shared__ float2 s_ml[NW];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -373,40 +374,50 @@ __global__ void __launch_bounds__(NW * 32) paged_join_kernel(const PDecP p) {
   float M = -INFINITY, L = 0.f, o[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) o[i] = 0.f;
-  for (int64_t w = c.w0 + warp; w <= c.w1; w += NW * U) {
-    float x[U][V];
-    float2 ml[U];
+  // a warp looks at 32 partials at a time and loads those that are not empty, up to U at once
+  for (int64_t w = c.w0 + warp; w <= c.w1; w += NW * 32) {
+    const int64_t mine = w + (int64_t)lane * NW;
+    float2 my = make_float2(-INFINITY, 0.f);
+    if (mine <= c.w1) my = p.part_ml[slot_of(c, mine) * p.GT + g];
+    uint32_t full = __ballot_sync(0xffffffffu, my.y != 0.f);
+    while (full) {
+      float x[U][V];
+      float2 ml[U];
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const bool in = w + u * NW <= c.w1;
-      const int64_t at = slot_of(c, in ? w + u * NW : w) * p.GT + g;
-      ml[u] = p.part_ml[at];
-      if (!in) ml[u].x = -INFINITY;
-      const float* part = p.part + at * D + lane * V;
-      if (V == 4) {
-        const float4 y = *reinterpret_cast<const float4*>(part);
-        x[u][0] = y.x; x[u][1] = y.y; x[u][V - 2] = y.z; x[u][V - 1] = y.w;
-      } else {
-        const float2 y = *reinterpret_cast<const float2*>(part);
-        x[u][0] = y.x; x[u][V - 1] = y.y;
+      for (int u = 0; u < U; ++u) {
+        const int src = full ? __ffs(full) - 1 : -1;
+        full &= full - 1u;
+        ml[u].x = __shfl_sync(0xffffffffu, my.x, src & 31);
+        ml[u].y = __shfl_sync(0xffffffffu, my.y, src & 31);
+        if (src < 0) ml[u] = make_float2(-INFINITY, 0.f);
+        const float* part = p.part + (slot_of(c, w + (int64_t)(src < 0 ? 0 : src) * NW) * p.GT + g) * D + lane * V;
+#pragma unroll
+        for (int i = 0; i < V; ++i) x[u][i] = 0.f;
+        if (src < 0) continue;
+        if (V == 4) {
+          const float4 y = *reinterpret_cast<const float4*>(part);
+          x[u][0] = y.x; x[u][1] = y.y; x[u][V - 2] = y.z; x[u][V - 1] = y.w;
+        } else {
+          const float2 y = *reinterpret_cast<const float2*>(part);
+          x[u][0] = y.x; x[u][V - 1] = y.y;
+        }
       }
+      float mn = M;
+#pragma unroll
+      for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
+      const float ms = mn == -INFINITY ? 0.f : mn, a = exp2f(M - ms);
+      L *= a;
+#pragma unroll
+      for (int i = 0; i < V; ++i) o[i] *= a;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const float f = exp2f(ml[u].x - ms);
+        L = fmaf(ml[u].y, f, L);
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = fmaf(x[u][i], f, o[i]);
+      }
+      M = mn;
     }
-    float mn = M;
-#pragma unroll
-    for (int u = 0; u < U; ++u) mn = fmaxf(mn, ml[u].x);
-    const float ms = mn == -INFINITY ? 0.f : mn, a = exp2f(M - ms);
-    L *= a;
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] *= a;
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      if (w + u * NW > c.w1) break;
-      const float f = exp2f(ml[u].x - ms);
-      L = fmaf(ml[u].y, f, L);
-#pragma unroll
-      for (int i = 0; i < V; ++i) o[i] = fmaf(x[u][i], f, o[i]);
-    }
-    M = mn;
   }
 #pragma unroll
   for (int i = 0; i < V; ++i) s_o[warp][lane * V + i] = o[i];

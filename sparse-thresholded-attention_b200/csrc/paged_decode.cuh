@@ -96,14 +96,18 @@ __device__ __forceinline__ void step(const PDecP& p, Place& a) {
   seek_sequence(p, a);
 }
 
-// What share `me` holds: `count` units from the place `at` on (count 0: nothing).  Found by a warp;
-// `len` is the length of sequence `lane` (0 beyond the batch), loaded by the caller ahead of time.
+// What the share of this warp holds: `count` units from the place `at` on (count 0: nothing).  The
+// shares are dealt to the CTAs in runs of (nearly) equal length; `me` receives the warp's (of a
+// CTA that is a share by itself: every warp's is the CTA's).  `len` is the length of sequence
+// `lane` (0 beyond the batch).
 struct Share {
   int count;
+  bool merge;  // enough shares per CTA to join their partials there (else the join takes them all)
   Place at;
 };
 
-__device__ __forceinline__ Share find_share(const PDecP& p, int64_t me, int len) {
+template <bool WARP_SHARES = true>
+__device__ __forceinline__ Share find_share(const PDecP& p, int len, int64_t& me) {
   const int lane = threadIdx.x & 31;
   const int64_t hg = (int64_t)p.c.Hkv * p.NG;
   int64_t mine = n_units(p, len) * hg, inc = mine;  // of the first 32 sequences
@@ -123,7 +127,14 @@ __device__ __forceinline__ Share find_share(const PDecP& p, int64_t me, int len)
   }
   const int64_t shares = n_shares(p, total);
   Share s{};
-  if (me >= shares) return s;
+  s.merge = shares > 3 * (int64_t)gridDim.x;
+  int64_t end = shares;
+  me = blockIdx.x;
+  if (WARP_SHARES) {
+    me = share_begin(shares, blockIdx.x, gridDim.x) + (threadIdx.x >> 5);
+    end = share_begin(shares, blockIdx.x + 1, gridDim.x);
+  }
+  if (me >= end) return s;
   const int64_t t = share_begin(total, me, shares);
   s.count = (int)(share_begin(total, me + 1, shares) - t);
   int b0 = 0;

@@ -43,6 +43,8 @@ struct SmemB {
   uint4 q[NW][NT][D / 32][32];            // a lane's raw queries of a k step: dims 0, 8, d/2, d/2 + 8 on, two each
   float2 turns[16][D / 2];                // cos / sin of turns by 0 .. 7 and by 0, 8 .. 56 positions
   float inv_freq[D / 2];
+  float2 end_ml[NW][8 * NT];              // the partials that the shares end with: max and sum,
+  int4 end[NW];                           // sequence (-1: none), kv head, group, first unit included
   int4 seg[NW][4];                        // segments entered by the loads: sequence, kv head, group, length
 };
 
@@ -142,8 +144,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
   // can be computed meanwhile comes once the rows have been asked for.
   static_assert(NW * 32 % HALF == 0, "a thread's turns share one frequency");
   const float my_freq = __ldg(p.inv_freq + threadIdx.x % HALF);
-  const int64_t me = (int64_t)warp * gridDim.x + blockIdx.x;
-  const Share share = find_share(p, me, first_len(p.c));
+  int64_t me;  // this warp's share: a CTA has neighbouring ones, all CTAs as many
+  const Share share = find_share(p, first_len(p.c), me);
   const int count = share.count;
   Place nx = share.at;              // the unit whose K rows are loaded next
   Rows rows{-1, 0, 0, true};
@@ -316,8 +318,8 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
     sm.rot[u][ks][r][l] = make_float4(a.x * b.x - a.y * b.y, a.z * b.z - a.w * b.w,
                                       a.x * b.y + a.y * b.x, a.z * b.w + a.w * b.z);
   }
+  if (lane == 0) sm.end[warp].x = -1;
   __syncthreads();
-  if (count == 0) return;
 
   // ---- the query's angle at a tile, this lane's frequencies; it moves by a constant from tile to
   // tile of a segment (of a chunk)
@@ -530,7 +532,12 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
       const int4 at = sm.seg[warp][seg & 3];
       const bool started = n <= it;  // the segment's first unit lies in this share
       const bool whole = fresh_seg && started;
+      // what is left open at the share's end is joined with the neighbours' below; it waits in the
+      // ring, which is free by then
+      const bool last = share.merge && it + 1 == count;
       const int64_t slot = 2 * me + (started ? 1 : 0);
+      float* part = last ? reinterpret_cast<float*>(sm.k[warp][0]) : p.part + slot * GT * D;
+      if (last && !whole && lane == 0) sm.end[warp] = make_int4(at.x, at.y, at.z, started ? 1 : 0);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -551,13 +558,16 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
               }
               if (fr == 0) p.ml[head] = make_float2(mref[nt][c], f);
             } else {
-              float* part = p.part + (slot * GT + g) * D + fr;
+              float* to = part + g * D + fr;
 #pragma unroll
               for (int mt = 0; mt < MT; ++mt) {
-                part[mt * 16] = acc[nt][mt][c];
-                part[mt * 16 + 8] = acc[nt][mt][c + 2];
+                to[mt * 16] = acc[nt][mt][c];
+                to[mt * 16 + 8] = acc[nt][mt][c + 2];
               }
-              if (fr == 0) p.part_ml[slot * GT + g] = make_float2(mx[nt][c], l);
+              if (fr == 0) {
+                if (last) sm.end_ml[warp][g] = make_float2(mx[nt][c], l);
+                else p.part_ml[slot * GT + g] = make_float2(mx[nt][c], l);
+              }
             }
           }
 #pragma unroll
@@ -567,6 +577,38 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
         }
     }
     n = fresh_seg ? 0 : n + 1;
+  }
+
+  // ---- the open ends of neighbouring shares that lie in one segment become one partial, that of
+  // the first; the others' are marked as empty
+  if (!share.merge) return;
+  __syncthreads();
+#pragma unroll 1
+  for (int w0 = 0; w0 < NW;) {
+    const int4 at = sm.end[w0];
+    int w1 = w0 + 1;
+    if (at.x >= 0) {
+      while (w1 < NW && sm.end[w1].x == at.x && sm.end[w1].y == at.y && sm.end[w1].z == at.z) ++w1;
+      const int64_t slot = 2 * (me - warp + w0) + at.w;
+      const int heads = min(GT, p.G - at.z * GT);
+      for (int i = threadIdx.x; i < heads * D; i += NW * 32) {
+        const int g = i / D;
+        float M = -INFINITY, L = 0.f, o = 0.f;
+        for (int w = w0; w < w1; ++w) M = fmaxf(M, sm.end_ml[w][g].x);
+        const float ms = M == -INFINITY ? 0.f : M;
+        for (int w = w0; w < w1; ++w) {
+          const float2 ml = sm.end_ml[w][g];
+          const float f = ex2(ml.x - ms);
+          L = fmaf(ml.y, f, L);
+          o = fmaf(reinterpret_cast<const float*>(sm.k[w][0])[i], f, o);
+        }
+        p.part[slot * GT * D + i] = o;
+        if (i % D == 0) p.part_ml[slot * GT + g] = make_float2(M, L);
+      }
+      for (int i = threadIdx.x; i < (w1 - w0 - 1) * GT; i += NW * 32)
+        p.part_ml[2 * (me - warp + w0 + 1) * GT + i / GT * 2 * GT + i % GT] = make_float2(-INFINITY, 0.f);
+    }
+    w0 = w1;
   }
 }
 
