@@ -62,7 +62,7 @@ template <int CH, bool VEC>
 __device__ __forceinline__ void move_rows(const char* ksrc, const char* vsrc, char* kdst, char* vdst,
                                           int64_t ks, int64_t vs, int64_t kd, int64_t vd, int n, int es) {
   constexpr int LPU = 2 * CH < 32 ? 2 * CH : 32;  // lanes of a row
-  constexpr int PER = 32 / LPU, PASS = 2 * CH / LPU, U = 8 / PER / PASS;
+  constexpr int PER = 32 / LPU, PASS = 2 * CH / LPU, U = 4;
   const int lane = threadIdx.x & 31, sub = lane / LPU, ch = lane % CH;
   const bool is_v = PASS == 1 && (lane / CH) % 2 == 1;
 #pragma unroll 1
@@ -104,24 +104,32 @@ __device__ __forceinline__ void move_rows(const char* ksrc, const char* vsrc, ch
   }
 }
 
-// Programmatic launch: the next kernel of the stream may be set up from here on / its inputs, the
-// results of the kernel ahead, are complete from here on.
+// Programmatic launches: every kernel of the paged cache may be set up while the one ahead of it in
+// the stream runs.  grid_wait: what the kernel ahead, and all before it, wrote is there from here
+// on; every block passes it.  grid_dependents: the next kernel may be set up.  The first kernel of
+// a call waits before it lets the next one start, so that the later kernels of the call may read
+// what the call was given (not what their predecessor writes) ahead of their own wait.
 __device__ __forceinline__ void grid_dependents() { asm volatile("griddepcontrol.launch_dependents;"); }
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Launches a kernel that may begin before the one ahead of it in the stream has ended (it waits
 // for that kernel's results itself), so that its launch does not add to the call.
 template <typename K, typename P>
-inline cudaError_t launch_behind(K kernel, dim3 grid, int threads, const P& p, cudaStream_t st) {
+inline cudaError_t launch_behind(K kernel, dim3 grid, int threads, const P& p, cudaStream_t st,
+                                 size_t smem = 0, unsigned cluster = 0) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = grid;
   cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, kernel, p);
 }
 

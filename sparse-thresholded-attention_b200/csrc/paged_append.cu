@@ -39,6 +39,8 @@ __device__ __forceinline__ int new_len(const AppP& p, int b, int len, int& cnt) 
 template <int CH, bool VEC>
 __global__ void __launch_bounds__(kThreads) paged_append_kernel(const AppP p) {
   const int tid = threadIdx.x, lane = tid & 31;
+  grid_wait();
+  grid_dependents();
   for (int b = blockIdx.y; b < p.c.B; b += gridDim.y) {
     const int len = paged_len(p.c, b);
     int cnt;
@@ -74,15 +76,16 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(const AppP p) {
 
 __global__ void __launch_bounds__(kThreads) paged_lens_kernel(const AppP p) {
   const int b = blockIdx.x * kThreads + threadIdx.x;
+  grid_wait();
   if (b >= p.c.B) return;
   int cnt;
   p.lens_out[b] = new_len(p, b, paged_len(p.c, b), cnt);
 }
 
 template <int CH>
-void launch(const AppP& p, bool vec, dim3 grid, cudaStream_t st) {
-  if (vec) paged_append_kernel<CH, true><<<grid, kThreads, 0, st>>>(p);
-  else paged_append_kernel<CH, false><<<grid, kThreads, 0, st>>>(p);
+cudaError_t launch(const AppP& p, bool vec, dim3 grid, cudaStream_t st) {
+  return vec ? launch_behind(paged_append_kernel<CH, true>, grid, kThreads, p, st)
+             : launch_behind(paged_append_kernel<CH, false>, grid, kThreads, p, st);
 }
 
 }  // namespace
@@ -118,12 +121,10 @@ int paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, cudaS
   const dim3 grid((unsigned)(gx > 0 ? gx : 1), (unsigned)(c->batch < 65535 ? c->batch : 65535));
   // a length that is overwritten in place is read by one block only, or stored by a second launch
   p.store_lens = a->lens_out != c->lens || grid.x == 1;
-  if (ch == 8) launch<8>(p, vec, grid, st);
-  else if (ch == 16) launch<16>(p, vec, grid, st);
-  else launch<32>(p, vec, grid, st);
-  if (!p.store_lens)
-    paged_lens_kernel<<<(unsigned)((c->batch + kThreads - 1) / kThreads), kThreads, 0, st>>>(p);
-  const cudaError_t e = cudaGetLastError();
+  cudaError_t e = ch == 8 ? launch<8>(p, vec, grid, st)
+                          : (ch == 16 ? launch<16>(p, vec, grid, st) : launch<32>(p, vec, grid, st));
+  if (e == cudaSuccess && !p.store_lens)
+    e = launch_behind(paged_lens_kernel, dim3((unsigned)((c->batch + kThreads - 1) / kThreads)), kThreads, p, st);
   return e == cudaSuccess ? STA_OK : fail(STA_ERR_CUDA, cudaGetErrorString(e));
 }
 

@@ -50,34 +50,41 @@ __device__ __forceinline__ float warp_reduce(float (&v)[NV]) {
   return v[0];
 }
 
-// The f32 kernel: CUDA cores, so that scores keep full fp32 products (8 warps, 8 keys of a tile
-// each; a lane holds D / 32 dims and reduces its partial dots with the other lanes').
-constexpr int kF32Threads = 256;
-constexpr int kF32Warps = kF32Threads / 32;
-constexpr int kF32Keys = kTile / kF32Warps;  // keys of a tile per warp
+// The f32 kernel: CUDA cores, so that scores keep full fp32 products (a warp has 4 or 8 keys of a
+// tile; a lane holds D / 32 dims and reduces its partial dots with the other lanes').
+template <int D, int GT>
+struct F32 {
+  // one CTA per SM at d = 128 (its ring takes 192 KB), of 16 warps (8 where 8 heads' accumulators
+  // need the registers: 16 warps spill and take 204 us instead of 165 at 65536 keys of 8 kv heads);
+  // two CTAs of 8 warps at d = 64
+  static constexpr int THREADS = D == 128 && GT < 8 ? 512 : 256, WARPS = THREADS / 32;
+  static constexpr int KEYS = kTile / WARPS;  // keys of a tile per warp
+};
 
 template <int D, int GT>
 struct Smem {
-  static constexpr int STAGES = 3;
+  static constexpr int STAGES = 3, NWF = F32<D, GT>::WARPS, KPW = F32<D, GT>::KEYS;
   static constexpr int CH = D / 4;   // 16-byte chunks of a row
   uint4 kv[STAGES][2][kTile * CH];   // K rows, V rows (also the flush's scratch)
   float q[2][GT][D];                 // rotated, scaled queries of this tile and the next
-  float p[kF32Warps][kF32Keys][GT];  // a warp's probabilities
-  float m[kF32Warps][GT], l[kF32Warps][GT];
+  float p[NWF][KPW][GT];  // a warp's probabilities
+  float m[NWF][GT], l[NWF][GT];
   int64_t koff[2][kTile], voff[2][kTile];
 };
 
 template <int D, int GT>
-__global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDecP p) {
+__global__ void __launch_bounds__(F32<D, GT>::THREADS) paged_decode_f32_kernel(const PDecP p) {
   using S = Smem<D, GT>;
+  constexpr int NTH = F32<D, GT>::THREADS, NWF = F32<D, GT>::WARPS, KPW = F32<D, GT>::KEYS;
   constexpr int HALF = D / 2, CH = S::CH, ST = S::STAGES;
   constexpr int FP = HALF / 32;               // frequencies of a lane
-  constexpr int KB = GT == 8 ? 4 : 8, NV = KB * GT;  // keys of one reduction
+  constexpr int KB = KPW * GT > 32 ? 32 / GT : KPW, NV = KB * GT;  // keys of one reduction
   constexpr int LPV = 32 / NV;                // lanes that hold the same value
-  constexpr int QH = GT * HALF / kF32Threads > 0 ? GT * HALF / kF32Threads : 1;  // q pairs of a thread
+  constexpr int QH = GT * HALF / NTH > 0 ? GT * HALF / NTH : 1;  // q pairs of a thread
   extern __shared__ __align__(128) unsigned char smem_raw[];
   S& sm = *reinterpret_cast<S*>(smem_raw);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  grid_wait();
   grid_dependents();
   int64_t me;
   const Share share = find_share<false>(p, first_len(p.c), me);
@@ -87,22 +94,28 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
   Place qa = cur, oa = cur;  // where queries and row offsets stand
   int q_it = 0, l_it = 0, o_it = 0;
 
-  // ---- row offsets of a tile (threads 0 .. 63), -1: no row, -2: a page outside the pool
+  // ---- row offsets of a tile (threads 0 .. 63), -1: no row, -2: a page outside the pool.  The
+  // table entry is asked for in lookup() and used in offsets(), a tile's work later.
+  int32_t entry = -1;
+  auto lookup = [&]() {
+    if (o_it < count && tid < kTile) {
+      const int j = oa.n * kTile + tid;
+      if (j < oa.len) entry = __ldg(p.c.table + oa.b * p.c.ts + (uint32_t)j / p.c.page);
+    }
+  };
   auto offsets = [&]() {
     if (o_it < count) {
       if (tid < kTile) {
         const int j = oa.n * kTile + tid;
         int64_t ko = -1, vo = -1;
         if (j < oa.len) {
-          const uint32_t t = (uint32_t)j / p.c.page;
-          const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, oa.b, t);
-          if (pg < 0) {
+          if (entry < 0 || entry >= p.c.n_pages) {
             ko = -2;
             atomicCAS(p.err, 0, kErrPageDecode);
           } else {
-            const int64_t slot = (uint32_t)j - t * p.c.page, h = oa.h;
-            ko = pg * p.c.ksp + h * p.c.ksh + slot * p.c.ksn;
-            vo = pg * p.c.vsp + h * p.c.vsh + slot * p.c.vsn;
+            const int64_t slot = (uint32_t)j % p.c.page, h = oa.h;
+            ko = entry * p.c.ksp + h * p.c.ksh + slot * p.c.ksn;
+            vo = entry * p.c.vsp + h * p.c.vsh + slot * p.c.vsn;
           }
         }
         sm.koff[o_it & 1][tid] = ko;
@@ -117,7 +130,7 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
     if (l_it < count) {
       const int st = l_it % ST;
 #pragma unroll 4
-      for (int i = tid; i < kTile * CH; i += kF32Threads) {
+      for (int i = tid; i < kTile * CH; i += NTH) {
         const int row = i / CH, ch = i % CH;
         const int64_t ko = sm.koff[l_it & 1][row], vo = sm.voff[l_it & 1][row];
         cp_async16(&sm.kv[st][1][i], p.c.v + (vo >= 0 ? vo + ch * 16 : 0), vo >= 0 ? 16 : 0);
@@ -133,14 +146,14 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
   };
   // ---- queries of a tile: rotated by p_i - p_0
   float q1[QH], q2[QH];
-  const int qf = tid % HALF, qg = tid / HALF;  // frequency, first head (step kF32Threads / HALF)
+  const int qf = tid % HALF, qg = tid / HALF;  // frequency, first head (step NTH / HALF)
   auto queries = [&]() {
     if (q_it < count) {
       if (q_it == 0 || qa.n == 0) {
         const int h0 = qa.h * p.G + qa.grp * GT;
 #pragma unroll
         for (int i = 0; i < QH; ++i) {
-          const int g = qg + i * (kF32Threads / HALF);
+          const int g = qg + i * (NTH / HALF);
           const bool in = g < GT && qa.grp * GT + g < p.G;
           const float* src = static_cast<const float*>(p.q) + qa.b * p.qsb + (h0 + g) * p.qsh;
           q1[i] = in ? (src[qf]) * p.qscale : 0.f;
@@ -151,7 +164,7 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
       turn(query_offset(p, qa.len, qa.n), __ldg(p.inv_freq + qf), c, s);
 #pragma unroll
       for (int i = 0; i < QH; ++i) {
-        const int g = qg + i * (kF32Threads / HALF);
+        const int g = qg + i * (NTH / HALF);
         if (g < GT) {
           sm.q[q_it & 1][g][qf] = q1[i] * c - q2[i] * s;
           sm.q[q_it & 1][g][qf + HALF] = q2[i] * c + q1[i] * s;
@@ -163,18 +176,20 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
   };
 
   for (int i = 0; i < ST - 1; ++i) {
+    lookup();
     offsets();
     __syncthreads();
     loads();
   }
+  lookup();
   offsets();
   queries();
-  float2 rot[kF32Keys][FP];  // cos / sin of the warp's key offsets at the lane's frequencies
+  float2 rot[KPW][FP];  // cos / sin of the warp's key offsets at the lane's frequencies
 #pragma unroll
-  for (int t = 0; t < kF32Keys; ++t)
+  for (int t = 0; t < KPW; ++t)
 #pragma unroll
     for (int e = 0; e < FP; ++e)
-      turn((double)(warp * kF32Keys + t) * p.pos_scale, __ldg(p.inv_freq + lane * FP + e), rot[t][e].x,
+      turn((double)(warp * KPW + t) * p.pos_scale, __ldg(p.inv_freq + lane * FP + e), rot[t][e].x,
            rot[t][e].y);
 
   float acc[GT][2 * FP];
@@ -188,6 +203,7 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
     asm volatile("cp.async.wait_group %0;\n" ::"n"(ST - 2) : "memory");
     __syncthreads();
     loads();
+    lookup();
     const int st = it % ST;
     const float* ks = reinterpret_cast<const float*>(sm.kv[st][0]);
     const float* vs = reinterpret_cast<const float*>(sm.kv[st][1]);
@@ -204,8 +220,8 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
         ? p.scores + ((((int64_t)cur.b * p.c.Hkv * p.NG + cur.h * p.NG + cur.grp) * p.cap_tiles + cur.n) * GT) * kTile
         : nullptr;
 #pragma unroll
-    for (int kb = 0; kb < kF32Keys / KB; ++kb) {
-      const int key0 = warp * kF32Keys + kb * KB;
+    for (int kb = 0; kb < KPW / KB; ++kb) {
+      const int key0 = warp * KPW + kb * KB;
       float v[NV];
 #pragma unroll
       for (int kk = 0; kk < KB; ++kk) {
@@ -289,16 +305,16 @@ __global__ void __launch_bounds__(kF32Threads) paged_decode_f32_kernel(const PDe
       const bool whole = seg_end && started;
       const int slot = 2 * blockIdx.x + (started ? 1 : 0);
       const int h0 = cur.h * p.G + cur.grp * GT;
-      for (int i = tid; i < GT * D; i += kF32Threads) {
+      for (int i = tid; i < GT * D; i += NTH) {
         const int g = i / D, d = i % D;
         if (cur.grp * GT + g >= p.G) continue;
         float M = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kF32Warps; ++w) M = fmaxf(M, sm.m[w][g]);
+        for (int w = 0; w < NWF; ++w) M = fmaxf(M, sm.m[w][g]);
         const float ms = M == -INFINITY ? 0.f : M;
         float L = 0.f, o = 0.f;
 #pragma unroll
-        for (int w = 0; w < kF32Warps; ++w) {
+        for (int w = 0; w < NWF; ++w) {
           const float f = exp2f(sm.m[w][g] - ms);
           L += sm.l[w][g] * f;
           o += part_acc[(w * GT + g) * D + d] * f;
@@ -582,8 +598,8 @@ int launch_f32(const PDecP& p, cudaStream_t st) {
   static bool ready[64];
   const cudaError_t e = allow_smem(paged_decode_f32_kernel<D, GT>, bytes, ready);
   if (e != cudaSuccess) return fail(STA_ERR_CUDA, cudaGetErrorString(e));
-  paged_decode_f32_kernel<D, GT><<<p.W, kF32Threads, bytes, st>>>(p);
-  return STA_OK;
+  const cudaError_t r = launch_behind(paged_decode_f32_kernel<D, GT>, dim3((unsigned)p.W), F32<D, GT>::THREADS, p, st, bytes);
+  return r == cudaSuccess ? STA_OK : fail(STA_ERR_CUDA, cudaGetErrorString(r));
 }
 
 template <int D>
@@ -666,9 +682,7 @@ int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void*
   if (f32) rc = c->d == 128 ? launch_f32<128>(p, st) : launch_f32<64>(p, st);
   else rc = launch_paged_decode_bf16(p, c->d, st);
   if (rc != STA_OK) return rc;
-  cudaError_t e = cudaGetLastError();
-  if (e == cudaSuccess)
-    e = f32 ? launch_finish<float>(p, c->d, st) : launch_finish<__nv_bfloat16>(p, c->d, st);
+  const cudaError_t e = f32 ? launch_finish<float>(p, c->d, st) : launch_finish<__nv_bfloat16>(p, c->d, st);
   return e == cudaSuccess ? STA_OK : fail(STA_ERR_CUDA, cudaGetErrorString(e));
 }
 

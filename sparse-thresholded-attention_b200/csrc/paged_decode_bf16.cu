@@ -139,6 +139,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int fr = lane >> 2, fc = lane & 3;
 
+  grid_wait();
   grid_dependents();
   // The start is a chain of loads (lengths, page table, rows) that nothing may stand ahead of: what
   // can be computed meanwhile comes once the rows have been asked for.
@@ -620,8 +621,8 @@ int launch(const PDecP& p, cudaStream_t st) {
   if (e != cudaSuccess) return fail(STA_ERR_CUDA, cudaGetErrorString(e));
   // shares go to the CTAs in turn, so few shares spread over the SMs
   const int grid = p.W < p.sms * Cfg<D, NT>::CTAS ? p.W : p.sms * Cfg<D, NT>::CTAS;
-  paged_decode_bf16_kernel<D, NT, MODE><<<grid, NW * 32, bytes, st>>>(p);
-  return STA_OK;
+  const cudaError_t r = launch_behind(paged_decode_bf16_kernel<D, NT, MODE>, dim3((unsigned)grid), NW * 32, p, st, bytes);
+  return r == cudaSuccess ? STA_OK : fail(STA_ERR_CUDA, cudaGetErrorString(r));
 }
 
 template <int D, int NT>

@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP 
   extern __shared__ uint32_t s_keys[];
   __shared__ SmemE sm;
   cg::cluster_group cluster = cg::this_cluster();
+  grid_wait();
   grid_dependents();
   const int rank = blockIdx.x, CL = gridDim.x;  // the cluster is the grid's first dimension
   const int h = blockIdx.y, b = blockIdx.z;
@@ -327,18 +328,9 @@ cudaError_t launch_select(const EvP& p, int cl, cudaStream_t st) {
   static bool ready[64];
   const cudaError_t e = allow_smem(paged_evict_select_kernel, kSliceSmem * 4, ready);
   if (e != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)cl, (unsigned)p.c.Hkv, (unsigned)p.c.B);
-  cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = p.keys ? 0 : ((size_t)(p.c.cap + cl - 1) / cl + 3) * 4;
-  cfg.stream = st;
-  cudaLaunchAttribute attr;
-  attr.id = cudaLaunchAttributeClusterDimension;
-  attr.val.clusterDim.x = (unsigned)cl;
-  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, paged_evict_select_kernel, p);
+  const size_t bytes = p.keys ? 0 : ((size_t)(p.c.cap + cl - 1) / cl + 3) * 4;
+  return launch_behind(paged_evict_select_kernel, dim3((unsigned)cl, (unsigned)p.c.Hkv, (unsigned)p.c.B), kThreads,
+                       p, st, bytes, (unsigned)cl);
 }
 
 }  // namespace
