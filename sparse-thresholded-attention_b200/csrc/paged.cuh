@@ -145,7 +145,7 @@ inline cudaError_t allow_smem(K kernel, int bytes, bool (&ready)[64]) {
 }
 
 inline int paged_check(const sta_paged_cache* c) {
-  if (!c || !c->k || !c->v || !c->table || !c->lens)
+  if (!c || !c->k || !c->v || (c->batch != 0 && (!c->table || !c->lens)))
     return fail(STA_ERR_ARG, "sta_paged: null pointer");
   if (c->d != 64 && c->d != 128) return fail(STA_ERR_UNSUPPORTED, "sta_paged: d must be 64 or 128");
   if (c->dtype != STA_DTYPE_F32 && c->dtype != STA_DTYPE_BF16)

@@ -93,11 +93,11 @@ cudaError_t launch(const AppP& p, bool vec, dim3 grid, cudaStream_t st) {
 int paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, cudaStream_t st) {
   const int rc = paged_check(c);
   if (rc != STA_OK) return rc;
-  if (!a || !a->lens_out) return fail(STA_ERR_ARG, "sta_paged_append: null pointer");
+  if (!a || (c->batch > 0 && !a->lens_out)) return fail(STA_ERR_ARG, "sta_paged_append: null pointer");
   if (a->n < 0 || a->n > ((int64_t)1 << 31) - 65) return fail(STA_ERR_ARG, "sta_paged_append: bad n");
   for (int64_t x : {a->k_stride_h, a->k_stride_n, a->v_stride_h, a->v_stride_n})
     if (x < 0) return fail(STA_ERR_ARG, "sta_paged_append: negative stride");
-  if (a->n > 0 && (!a->k || !a->v)) return fail(STA_ERR_ARG, "sta_paged_append: null pointer");
+  if (a->n > 0 && c->batch > 0 && (!a->k || !a->v)) return fail(STA_ERR_ARG, "sta_paged_append: null pointer");
   if (a->lens_out != c->lens && a->lens_out < c->lens + c->batch && c->lens < a->lens_out + c->batch)
     return fail(STA_ERR_ARG, "sta_paged_append: lens_out overlaps lens without being it");
   if (c->batch == 0) return STA_OK;

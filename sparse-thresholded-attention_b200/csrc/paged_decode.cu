@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(F32<D, GT>::THREADS) paged_decode_f32_kernel(c
       }
     const int valid = cur.len - cur.n * kTile;  // keys of this tile
     float* sc = p.scores
-        ? p.scores + ((((int64_t)cur.b * p.c.Hkv * p.NG + cur.h * p.NG + cur.grp) * p.cap_tiles + cur.n) * GT) * kTile
+        ? p.scores + ((((int64_t)cur.b * p.c.Hkv * p.NG + cur.h * p.NG + cur.grp) * p.cap_tiles + cur.n) * p.SG) * kTile
         : nullptr;
 #pragma unroll
     for (int kb = 0; kb < KPW / KB; ++kb) {
@@ -246,7 +246,7 @@ __global__ void __launch_bounds__(F32<D, GT>::THREADS) paged_decode_f32_kernel(c
       float s = warp_reduce<NV>(v);
       const int idx = lane / LPV, kk = idx / GT, g = idx % GT;
       if (key0 + kk >= valid) s = -INFINITY;
-      if (sc && (LPV == 1 || lane % LPV == 0)) sc[g * kTile + key0 + kk] = s;
+      if (sc && g < p.SG && (LPV == 1 || lane % LPV == 0)) sc[g * kTile + key0 + kk] = s;
       float mb = s;
 #pragma unroll
       for (int o = GT * LPV; o < 32; o <<= 1) mb = fmaxf(mb, __shfl_xor_sync(0xffffffffu, mb, o));
@@ -489,9 +489,9 @@ __global__ void __launch_bounds__(kUpd) paged_weights_kernel(const PDecP p) {
   }
   grid_wait();
   const float2* ml = p.ml + (int64_t)b * p.H + h * p.G;
-  const float* sc = p.scores + (((int64_t)b * p.c.Hkv + h) * p.NG * p.cap_tiles + j / kTile) * p.GT * kTile + j % kTile;
+  const float* sc = p.scores + (((int64_t)b * p.c.Hkv + h) * p.NG * p.cap_tiles + j / kTile) * p.SG * kTile + j % kTile;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int grp = 0; grp < p.NG; ++grp, sc += p.cap_tiles * p.GT * kTile) {
+  for (int grp = 0; grp < p.NG; ++grp, sc += p.cap_tiles * p.SG * kTile) {
     const int heads = min(p.GT, p.G - grp * p.GT);
 #pragma unroll 4
     for (int g = 0; g < heads; ++g) {
@@ -563,7 +563,7 @@ PLayout layout(const sta_paged_cache* c, const sta_paged_decode_args* a) {
   L.part = take((size_t)2 * L.W * L.GT * c->d * 4);
   L.part_ml = take((size_t)2 * L.W * L.GT * 8);
   L.ml = take((size_t)c->batch * a->n_heads * 8);
-  L.scores = a->weights_out ? take((size_t)(c->batch * c->n_kv_heads * L.NG) * L.cap_tiles * L.GT * kTile * 4) : 0;
+  L.scores = a->weights_out ? take((size_t)(c->batch * c->n_kv_heads * L.NG) * L.cap_tiles * (G < L.GT ? G : L.GT) * kTile * 4) : 0;
   L.total = o + 256;
   return L;
 }
@@ -660,6 +660,7 @@ int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void*
   p.G = (int)(a->n_heads / c->n_kv_heads);
   p.NG = L.NG;
   p.GT = L.GT;
+  p.SG = p.G < L.GT ? p.G : L.GT;
   p.unit = L.unit;
   p.W = L.W;
   p.min_log = f32 ? 0 : 1;

@@ -15,6 +15,7 @@ struct PDecP {
   int q_words;       // 16-bit queries start on 4-byte boundaries
   void* out;
   int H, G, NG, GT;  // q heads, per kv head, groups of GT of them
+  int SG;            // heads of a group that are there: min(G, GT)
   int unit;          // log2 of the keys of a unit of work
   int W, min_log;    // shares at most, log2 of the units of a share at least
   int sms;
@@ -26,7 +27,7 @@ struct PDecP {
   float* part;       // (2 * W, GT, D): unnormalised outputs of cut segments
   float2* part_ml;   // (2 * W, GT): their max and sum
   float2* ml;        // (B, H): max and 1 / sum of segments that one share holds
-  float* scores;     // (B, Hkv * NG, capacity tiles, GT, 64) or null
+  float* scores;     // (B, Hkv * NG, capacity tiles, SG, 64) or null
   int64_t cap_tiles;
   float* w_out;
   int* err;

@@ -484,7 +484,7 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
     if (p.scores) {
       const int4 at = sm.seg[warp][seg & 3];
       float* out = p.scores + ((((int64_t)at.x * p.c.Hkv + at.y) * p.NG + at.z) * p.cap_tiles + (n >> 2)) *
-                                  GT * kTile + (n & 3) * 16 + fr;
+                                  p.SG * kTile + (n & 3) * 16 + fr;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll

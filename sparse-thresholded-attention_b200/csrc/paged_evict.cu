@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(kCopy) paged_evict_copy_kernel(const EvP p) {
 int check(const sta_paged_cache* c, const sta_paged_evict_args* a) {
   const int rc = paged_check(c);
   if (rc != STA_OK) return rc;
-  if (!a || !a->table_out || !a->kept || !a->lens_out)
+  if (!a || (c->batch > 0 && (!a->table_out || !a->kept || !a->lens_out)))
     return fail(STA_ERR_ARG, "sta_paged_evict: null pointer");
   if (!c->weights) return fail(STA_ERR_ARG, "sta_paged_evict: the cache has no weights");
   if (a->budget <= 0 || a->budget > ((int64_t)1 << 31) - 65)

@@ -23,47 +23,51 @@ from .core import Geometry, dtype_code
 
 def _on(t, dev, dtype, shape, name):
     """t is a tensor of this device, type and shape (None entries: any) with a dense last dim."""
-    if torch.is_tensor(t) and t.dtype is dtype and t.device == dev and t.dim() == len(shape):
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == dev:
         s = t.shape
-        for i, n in enumerate(shape):
-            if n is not None and s[i] != n:
-                break
-        else:
-            if not s or s[-1] <= 1 or t.stride(-1) == 1:
-                return
-    if not torch.is_tensor(t) or t.device != dev:
+        if len(s) == len(shape):
+            for m, n in zip(s, shape):
+                if n is not None and m != n:
+                    break
+            else:
+                if not s or s[-1] <= 1 or t.stride(-1) == 1:
+                    return
+    if not isinstance(t, torch.Tensor) or t.device != dev:
         raise ValueError(f"{name} must be a tensor on {dev}")
     if t.dtype != dtype:
         raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
-    if t.dim() != len(shape) or any(n is not None and s != n for s, n in zip(t.shape, shape)):
+    if t.dim() != len(shape) or any(n is not None and m != n for m, n in zip(t.shape, shape)):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
-    if t.dim() and t.shape[-1] > 1 and t.stride(-1) != 1:
-        raise ValueError(f"the last dimension of {name} must be contiguous")
+    raise ValueError(f"the last dimension of {name} must be contiguous")
 
 
-def _run(cache, name, *args):
+def _run(cache, entry, name, *args):
     """Call a library entry with the cache, on the current stream of the cache's device."""
-    dev = cache.device.index
-    if torch._C._cuda_getDevice() == dev:
-        rc = getattr(L.lib(), name)(cache._ref, *args, torch._C._cuda_getCurrentRawStream(dev))
+    dev = cache._index
+    if _device() == dev:
+        rc = entry(cache._ref, *args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = getattr(L.lib(), name)(cache._ref, *args, torch._C._cuda_getCurrentRawStream(dev))
+            rc = entry(cache._ref, *args, _raw_stream(dev))
     if rc:
         L.check(rc, name)
 
 
-def _workspace(cache, name, key, ref):
-    """Scratch of one call (its size depends on the shapes alone and is asked for once).  Every call
-    has its own: torch's allocator keeps it from other streams and from other captured graphs."""
+_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
+
+def _size(cache, key, entry, name, ref):
+    """Bytes of scratch that a call needs (by the shapes alone, so asked for once).  Every call has
+    scratch of its own: torch's allocator keeps it from other streams and from other graphs."""
     n = cache._sizes.get(key)
     if n is None:
-        with torch.cuda.device(cache.device):
-            n = getattr(L.lib(), name + "_workspace_bytes")(cache._ref, ref)
+        with torch.cuda.device(cache._index):
+            n = entry(cache._ref, ref)
         if n == 0:
             L.check(1, name)
         cache._sizes[key] = n
-    return torch.empty(n, dtype=torch.uint8, device=cache.device), n
+    return n
 
 
 class PagedCache:
@@ -76,12 +80,16 @@ class PagedCache:
     weights (n_pages, Hkv, page_size) float32, optional: the attention weight that each key has
     received so far (``decode(weights_out=...)``), which ``evict`` ranks by.
 
+    Keys, values and queries are finite numbers where a sequence has tokens; a head that reads an
+    infinity or NaN there is NaN.  What lies in slots without a token is never read.
+
     The tensors are used in place and may be written by the program between calls (new table
     entries, new lengths); the object itself only keeps them and their addresses.  A page number
     outside the pool never faults: its sequence's result is NaN, its rows are dropped, and
     ``core.device_error()`` is 201 (append), 202 (decode) or 203 (evict)."""
 
-    __slots__ = ("k", "v", "table", "lens", "weights", "device", "_args", "_ref", "_sizes")
+    __slots__ = ("k", "v", "table", "lens", "weights", "device", "_index", "_args", "_ref", "_sizes",
+                 "_scale")
 
     def __init__(self, k, v, table, lens, weights=None):
         if not (torch.is_tensor(k) and k.is_cuda):
@@ -108,6 +116,7 @@ class PagedCache:
         a.n_pages, a.n_kv_heads, a.page_size = n_pages, hk, page
         a.batch, a.table_width = table.shape
         self._args, self._ref, self._sizes = a, ctypes.byref(a), {}
+        self._index, self._scale = dev.index, 1.0 / math.sqrt(d)
 
     @property
     def batch(self):
@@ -125,6 +134,7 @@ class PagedCache:
         a.table, a.lens = table.data_ptr(), lens.data_ptr()
         a.table_stride, a.table_width = table.stride(0), table.shape[1]
         c._args, c._ref, c._sizes = a, ctypes.byref(a), {}
+        c._index, c._scale = self._index, self._scale
         return c
 
 
@@ -136,7 +146,7 @@ def append(cache: PagedCache, k, v, *, counts=None, lens_out=None):
     dropped and reported by ``core.device_error()``."""
     a = cache._args
     dev = cache.device
-    if not (torch.is_tensor(k) and torch.is_tensor(v)):
+    if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
         raise ValueError("k and v must be tensors")
     shape = (a.batch, a.n_kv_heads, k.shape[2] if k.dim() == 4 else None, a.d)
     if k.dim() == 4 and k.stride(3) != 1:
@@ -158,7 +168,7 @@ def append(cache: PagedCache, k, v, *, counts=None, lens_out=None):
     vb, vh, vn, _ = v.stride()
     b = L.PagedAppendArgs(k.data_ptr(), kb, kh, kn, v.data_ptr(), vb, vh, vn, shape[2],
                           None if counts is None else counts.data_ptr(), lens_out.data_ptr())
-    _run(cache, "sta_paged_append", ctypes.byref(b))
+    _run(cache, L.lib().sta_paged_append, "sta_paged_append", ctypes.byref(b))
     return lens_out
 
 
@@ -185,12 +195,13 @@ def decode(q, cache: PagedCache, geometry: Geometry, *, sm_scale=None, weights_o
     out = q.new_empty((a.batch, H, a.d))
     qb, qh, _ = q.stride()
     b = L.PagedDecodeArgs(q.data_ptr(), qb, qh, out.data_ptr(), H, inv.data_ptr(),
-                          geometry.pos_scale, geometry.rope_scale,
-                          1.0 / math.sqrt(a.d) if sm_scale is None else sm_scale)
+                          float(geometry.pos_scale), float(geometry.rope_scale),
+                          cache._scale if sm_scale is None else float(sm_scale))
     if geometry.dca is not None:
-        b.chunk_size, b.local_window = int(geometry.dca[0]), int(geometry.dca[1])
-        if b.chunk_size <= 0:
-            raise ValueError("dca needs a positive chunk_size")
+        size, window = int(geometry.dca[0]), int(geometry.dca[1])
+        if window <= 0 or size <= window or (size - window) % 64:
+            raise ValueError(f"dca {size, window}: chunk_size - local_window must be a positive multiple of 64")
+        b.chunk_size, b.local_window = size, window
     if weights_out is not None:
         if cache.weights is None:
             raise ValueError("weights_out needs a cache with weights")
@@ -199,8 +210,10 @@ def decode(q, cache: PagedCache, geometry: Geometry, *, sm_scale=None, weights_o
             raise ValueError("weights_out must have the strides of the cache's weights")
         b.weights_out = weights_out.data_ptr()
     ref = ctypes.byref(b)
-    ws, n = _workspace(cache, "sta_paged_decode", (H, weights_out is not None), ref)
-    _run(cache, "sta_paged_decode", ref, ws.data_ptr(), n)
+    lib = L.lib()
+    n = _size(cache, (H, weights_out is None), lib.sta_paged_decode_workspace_bytes, "sta_paged_decode", ref)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    _run(cache, lib.sta_paged_decode, "sta_paged_decode", ref, ws.data_ptr(), n)
     return out
 
 
@@ -224,6 +237,9 @@ def evict(cache: PagedCache, budget: int, table_out, *, n_global=32, n_local=32)
     b = L.PagedEvictArgs(budget, int(n_global), int(n_local), table_out.data_ptr(),
                          table_out.stride(0), table_out.shape[1], kept.data_ptr(), lens.data_ptr())
     ref = ctypes.byref(b)
-    ws, n = _workspace(cache, "sta_paged_evict", ("evict", budget, b.n_global, b.n_local, b.table_out_width), ref)
-    _run(cache, "sta_paged_evict", ref, ws.data_ptr(), n)
+    lib = L.lib()
+    n = _size(cache, (budget, n_global, n_local, b.table_out_width), lib.sta_paged_evict_workspace_bytes,
+              "sta_paged_evict", ref)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    _run(cache, lib.sta_paged_evict, "sta_paged_evict", ref, ws.data_ptr(), n)
     return cache._moved(table_out, lens), kept

@@ -466,3 +466,152 @@ def test_outputs_do_not_depend_on_the_other_sequences():
     a = paged.decode(q, cache, Geometry(inv_freq(D)))
     b = paged.decode(q, cache, Geometry(inv_freq(D)))
     assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("dtype,D,G", [(torch.bfloat16, 64, 20), (torch.bfloat16, 128, 33), (torch.bfloat16, 128, 12),
+                                       (torch.float32, 128, 8), (torch.float32, 64, 19)])
+def test_decode_of_many_heads_per_kv_head(dtype, D, G):
+    """Groups of q heads that one pass over the keys cannot serve."""
+    lens = [333, 64, 0, 17]
+    c = ref.make(lens, hk=2, D=D, page=32, dtype=dtype, seed=101)
+    q = queries(4, 2 * G, D, dtype, 102)
+    d, cache = on_gpu(c)
+    w = torch.zeros_like(d["weights"])
+    out = paged.decode(q.cuda(), cache, Geometry(inv_freq(D)), weights_out=w)
+    probs, size = check_decode(q, c, out, inv_freq=inv_freq(D))
+    want = ref.added_weights(c, probs, c["weights"])
+    rel = relative_p(dtype, size, D, 333).max().item()
+    got = torch.where(w.cpu() == 0, want, w.cpu().double())  # slots without a key stay zero
+    assert ((got - want).abs() <= 2.0 ** -24 * want + 1.01 * rel * (want - c["weights"].double())).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("page,lens", [
+    (16, [int(7.7 * i) % 90 if i % 5 else 0 for i in range(77)]),      # more sequences than lanes
+    (24, [0] * 40 + [700] + [0] * 30 + [3, 0]),
+    (64, [0] * 35),
+    (256, [33]),
+])
+def test_decode_of_many_and_empty_sequences(dtype, page, lens):
+    c = ref.make(lens, hk=2, D=64, page=page, dtype=dtype, seed=103)
+    q = queries(len(lens), 4, 64, dtype, 104)
+    _, cache = on_gpu(c)
+    out = paged.decode(q.cuda(), cache, Geometry(inv_freq(64)))
+    check_decode(q, c, out, inv_freq=inv_freq(64))
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float32, 128), (torch.float32, 64)])
+@pytest.mark.parametrize("page", [8, 16, 24, 100])
+def test_a_bad_page_reaches_its_own_sequence_only(dtype, D, page):
+    lens = [300, 290, 310]
+    c = ref.make(lens, hk=2, D=D, page=page, dtype=dtype, seed=105)
+    c["table"][1, 2] = c["k"].shape[0] + 5
+    q = queries(3, 8, D, dtype, 106)
+    _, cache = on_gpu(c)
+    out = paged.decode(q.cuda(), cache, Geometry(inv_freq(D)))
+    assert core.device_error() == 202
+    assert out[1].isnan().all()
+    keep = [0, 2]
+    check_decode(q[keep], dict(c, table=c["table"][keep], lens=c["lens"][keep]), out[keep], inv_freq=inv_freq(D))
+
+
+def test_evict_of_more_slots_than_shared_memory_holds():
+    """A table that names 204800 slots: the selection keeps its keys in the workspace."""
+    page, lens, budget = 4096, [150001, 300], 70000
+    c = ref.make(lens, hk=1, D=64, page=page, dtype=torch.bfloat16, seed=107, width=50, spare=20)
+    g = torch.Generator().manual_seed(108)
+    c["weights"] = torch.randint(0, 5000, c["weights"].shape, generator=g).float()
+    table_out = torch.full((2, 18), -1, dtype=torch.int32)
+    table_out[0] = c["free"][:18]
+    table_out[1, 0] = c["free"][18]
+    d, cache = on_gpu(c)
+    after, kept = paged.evict(cache, budget, table_out.cuda(), n_global=4, n_local=8)
+    assert core.device_error() == 0 and after.lens.tolist() == [70000, 300]
+    want = ref.evict(c, budget, 4, 8)
+    assert torch.equal(kept.cpu(), want)
+    j = want[0, 0].long()
+    src = c["k"][c["table"][0].long()[j // page], 0, j % page]
+    r = torch.arange(budget)
+    assert torch.equal(d["k"].cpu()[table_out[0].long()[r // page], 0, r % page], src)
+
+
+def test_evict_in_a_graph():
+    lens, D, page = [400, 90], 64, 16
+    c = ref.make(lens, hk=2, D=D, page=page, dtype=torch.float32, seed=109, spare=20)
+    table_out = c["free"][:16].reshape(2, 8)
+    d, cache = on_gpu(c)
+    out_dev = table_out.cuda()
+    paged.evict(cache, 128, out_dev, n_global=2, n_local=2)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            after, kept = paged.evict(cache, 128, out_dev, n_global=2, n_local=2)
+    for seed in (1, 2):
+        g = torch.Generator().manual_seed(seed)
+        c["weights"] = torch.rand(c["weights"].shape, generator=g)
+        d["weights"].copy_(c["weights"])
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(kept.cpu(), ref.evict(c, 128, 2, 2)) and after.lens.tolist() == [128, 90]
+
+
+def test_an_empty_batch():
+    c = ref.make([5], hk=2, D=64, page=4, dtype=torch.float32, seed=110)
+    d, _ = on_gpu(c)
+    cache = paged.PagedCache(d["k"], d["v"], d["table"][:0], d["lens"][:0], weights=d["weights"])
+    assert paged.decode(torch.zeros((0, 4, 64), device="cuda"), cache, Geometry(inv_freq(64))).shape == (0, 4, 64)
+    assert paged.append(cache, torch.zeros((0, 2, 1, 64), device="cuda"), torch.zeros((0, 2, 1, 64), device="cuda")).numel() == 0
+    after, kept = paged.evict(cache, 4, torch.zeros((0, 1), dtype=torch.int32, device="cuda"), n_global=0, n_local=0)
+    assert kept.shape == (0, 2, 4) and after.lens.numel() == 0
+
+
+def test_more_sequences_than_a_grid_dimension():
+    B, D = 66000, 64
+    k = torch.zeros((B, 1, 2, D), dtype=torch.bfloat16, device="cuda")
+    v = torch.zeros_like(k)
+    table = torch.arange(B, dtype=torch.int32, device="cuda").flip(0)[:, None].contiguous()
+    lens = (torch.arange(B, device="cuda") % 2).to(torch.int32)
+    cache = paged.PagedCache(k, v, table, lens)
+    rows = torch.randn((B, 1, 1, D), device="cuda").to(torch.bfloat16)
+    paged.append(cache, rows, rows)
+    at = torch.arange(B, device="cuda")
+    assert torch.equal(k[table[:, 0].long(), 0, at % 2], rows[:, 0, 0])
+    assert torch.equal(lens, (at % 2 + 1).to(torch.int32))
+    out = paged.decode(rows[:, 0].expand(B, 2, D), cache, Geometry(inv_freq(D)))
+    one = at % 2 == 0  # a single key: the output is its value
+    assert torch.equal(out[one, 0], rows[one, 0, 0])
+    with pytest.raises(ValueError):
+        paged.evict(paged.PagedCache(k, v, table, lens, weights=torch.zeros((B, 1, 2), device="cuda")), 1, table,
+                    n_global=0, n_local=0)
+
+
+def test_steps_in_a_row_do_not_overtake_each_other():
+    """Appends and decodes with weights in place, back to back without a wait: each kernel sees what
+    the ones ahead of it wrote."""
+    D, Hk, H, page, B = 64, 2, 4, 16, 4
+    pages = torch.arange(B * 20, dtype=torch.int32).reshape(B, 20)
+    g = torch.Generator().manual_seed(111)
+    xs = torch.randn((60, B, Hk, 1, D), generator=g).to(torch.bfloat16).cuda()
+    qs = torch.randn((60, B, H, D), generator=g).to(torch.bfloat16).cuda()
+    geo = Geometry(inv_freq(D).cuda())
+    results = []
+    for wait in (True, False):
+        k = torch.zeros((B * 20, Hk, page, D), dtype=torch.bfloat16, device="cuda")
+        v, w = torch.zeros_like(k), torch.ones((B * 20, Hk, page), device="cuda")
+        cache = paged.PagedCache(k, v, pages.cuda(), torch.tensor([0, 100, 200, 7], dtype=torch.int32, device="cuda"), weights=w)
+        outs = []
+        torch.cuda.synchronize()
+        for x, q in zip(xs, qs):
+            paged.append(cache, x, x)
+            if wait:
+                torch.cuda.synchronize()
+            outs.append(paged.decode(q, cache, geo, weights_out=w))
+            if wait:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        results.append((torch.stack(outs), w, cache.lens))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
