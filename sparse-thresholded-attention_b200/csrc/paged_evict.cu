@@ -23,10 +23,10 @@ namespace sta {
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kSlice = 8192;           // slots of a CTA that call for a larger cluster
+constexpr int kSlice = 16384;          // slots of a CTA that call for a larger cluster
 constexpr int kCopy = 256;             // threads of the copy
 constexpr int kItems = 8;              // consecutive slots of a thread in the compaction
 constexpr int kChunk = kThreads * kItems;
@@ -60,26 +60,27 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
 }
 
-__device__ __forceinline__ uint32_t block_excl_sum(uint32_t x, uint32_t* sh, uint32_t& total) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-  uint32_t inc = x;
+__device__ __forceinline__ uint32_t warp_incl_sum(uint32_t x) {
+  const int lane = threadIdx.x & 31;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const uint32_t y = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += y;
+    const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
   }
+  return x;
+}
+
+// (ends behind a barrier; every warp sums the warps' totals for itself)
+__device__ __forceinline__ uint32_t block_excl_sum(uint32_t x, uint32_t* sh, uint32_t& total) {
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const uint32_t inc = warp_incl_sum(x);
   if (lane == 31) sh[w] = inc;
   __syncthreads();
-  uint32_t base = 0, all = 0;
-#pragma unroll
-  for (int i = 0; i < kWarps; ++i) {
-    const uint32_t y = sh[i];
-    if (i < w) base += y;
-    all += y;
-  }
+  const uint32_t sums = warp_incl_sum(lane < kWarps ? sh[lane] : 0u);
+  const uint32_t base = __shfl_sync(0xffffffffu, sums, w == 0 ? 0 : w - 1);
+  total = __shfl_sync(0xffffffffu, sums, 31);
   __syncthreads();
-  total = all;
-  return base + inc - x;
+  return (w == 0 ? 0u : base) + inc - x;
 }
 
 // four words of CTA q's shared memory
