@@ -55,14 +55,14 @@ __device__ __forceinline__ int64_t paged_page(const PagedView& c, const int32_t*
 }
 
 // Moves up to 32 rows of K and V by one warp: lane l has row l's byte offsets (ks < 0: no row), `n`
-// rows in all.  Neighbouring lanes hold the 16-byte chunks (CH of a row) of K, then of V; eight
-// rows are loaded before the first is stored, which keeps 4 to 8 KB per warp in flight.  VEC:
-// sources lie on 16-byte boundaries; otherwise they are read by elements of `es` bytes.
+// rows in all.  Neighbouring lanes hold the 16-byte chunks (CH of a row) of K, then of V; four
+// loads of a lane are in flight before the first store.  VEC: sources lie on 16-byte boundaries;
+// otherwise they are read by elements of `es` bytes.
 template <int CH, bool VEC>
 __device__ __forceinline__ void move_rows(const char* ksrc, const char* vsrc, char* kdst, char* vdst,
                                           int64_t ks, int64_t vs, int64_t kd, int64_t vd, int n, int es) {
   constexpr int LPU = 2 * CH < 32 ? 2 * CH : 32;  // lanes of a row
-  constexpr int PER = 32 / LPU, PASS = 2 * CH / LPU, U = 4;
+  constexpr int PER = 32 / LPU, PASS = 2 * CH / LPU, U = 4 / PASS;
   const int lane = threadIdx.x & 31, sub = lane / LPU, ch = lane % CH;
   const bool is_v = PASS == 1 && (lane / CH) % 2 == 1;
 #pragma unroll 1

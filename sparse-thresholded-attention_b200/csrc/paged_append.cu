@@ -37,7 +37,7 @@ __device__ __forceinline__ int new_len(const AppP& p, int b, int len, int& cnt) 
 
 // CH: 16-byte chunks of a row (8, 16 or 32)
 template <int CH, bool VEC>
-__global__ void __launch_bounds__(kThreads) paged_append_kernel(const AppP p) {
+__global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const AppP p) {
   const int tid = threadIdx.x, lane = tid & 31;
   grid_wait();
   grid_dependents();

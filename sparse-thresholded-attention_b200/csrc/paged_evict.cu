@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP 
 }
 
 template <int CH>
-__global__ void __launch_bounds__(kCopy) paged_evict_copy_kernel(const EvP p) {
+__global__ void __launch_bounds__(kCopy, 4) paged_evict_copy_kernel(const EvP p) {
   const int lane = threadIdx.x & 31, h = blockIdx.y, b = blockIdx.z;
   const int n = (int)min((int64_t)paged_len(p.c, b), p.budget);
   const int r0 = (int)(blockIdx.x * (kCopy / 32) + threadIdx.x / 32) * p.rows, r = r0 + lane;
