@@ -49,7 +49,8 @@ extern "C" {
  * ------------------------------------------------------------------------------------- */
 const char* sta_last_error(void);
 /* ABI version: 5 (2: query slabs, PQ-Stream pass 2 on Kernel A keep bits, decode; 3: select wait
- * limit; 4: screened select scoring, sta_select_args.screen_ws; 5: vote histograms) */
+ * limit; 4: screened select scoring, sta_select_args.screen_ws; 5: vote histograms; the paged
+ * cache, sta_paged_*, came as new entry points alone) */
 int sta_version(void);
 /* Number of elements of one head of a compact selection array. */
 int64_t sta_tri_head_stride(int64_t n, int32_t tile);
@@ -626,6 +627,7 @@ typedef struct sta_paged_evict_args {
   int32_t* lens_out;       /* (batch,), not the cache's lens */
 } sta_paged_evict_args;
 
+/* (256 bytes where the selection fits shared memory: they are not touched then) */
 size_t sta_paged_evict_workspace_bytes(const sta_paged_cache* c, const sta_paged_evict_args* a);
 int sta_paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* workspace,
                     size_t workspace_bytes, void* stream);

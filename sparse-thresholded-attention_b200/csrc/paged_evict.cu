@@ -331,7 +331,7 @@ cudaError_t launch_select(const EvP& p, int cl, cudaStream_t st) {
   if (e != cudaSuccess) return e;
   const size_t bytes = p.keys ? 0 : ((size_t)(p.c.cap + cl - 1) / cl + 3) * 4;
   return launch_behind(paged_evict_select_kernel, dim3((unsigned)cl, (unsigned)p.c.Hkv, (unsigned)p.c.B), kThreads,
-                       p, st, bytes, (unsigned)cl);
+                       p, st, bytes, cl > 1 ? (unsigned)cl : 0u);
 }
 
 }  // namespace

@@ -192,7 +192,7 @@ def decode(q, cache: PagedCache, geometry: Geometry, *, sm_scale=None, weights_o
     if inv.numel() != a.d // 2:
         raise ValueError("inv_freq must have head_dim/2 entries")
     H = q.shape[1]
-    out = q.new_empty((a.batch, H, a.d))
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     qb, qh, _ = q.stride()
     b = L.PagedDecodeArgs(q.data_ptr(), qb, qh, out.data_ptr(), H, inv.data_ptr(),
                           float(geometry.pos_scale), float(geometry.rope_scale),
@@ -240,6 +240,7 @@ def evict(cache: PagedCache, budget: int, table_out, *, n_global=32, n_local=32)
     lib = L.lib()
     n = _size(cache, (budget, n_global, n_local, b.table_out_width), lib.sta_paged_evict_workspace_bytes,
               "sta_paged_evict", ref)
-    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    # 256 bytes: the selection fits shared memory, and no scratch is touched
+    ws = kept if n == 256 else torch.empty(n, dtype=torch.uint8, device=dev)
     _run(cache, lib.sta_paged_evict, "sta_paged_evict", ref, ws.data_ptr(), n)
     return cache._moved(table_out, lens), kept
