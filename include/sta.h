@@ -575,8 +575,8 @@ typedef struct sta_paged_cache {
 
 /* Write rows i < counts[b] of k_new / v_new (batch, n_kv_heads, n, d) to the slots lens[b] + i
  * (counts NULL: all n), zero their weights (when the cache has them) and store the new lengths
- * lens[b] + counts[b] in lens_out, which may be the cache's own lens.  Rows past the table's
- * last slot are dropped (device error word). */
+ * lens[b] + counts[b] in lens_out, which may be the cache's own lens, or counts.  Rows past the
+ * table's last slot are dropped (device error word). */
 typedef struct sta_paged_append_args {
   const void* k; int64_t k_stride_b; int64_t k_stride_h; int64_t k_stride_n;
   const void* v; int64_t v_stride_b; int64_t v_stride_h; int64_t v_stride_n;
@@ -594,7 +594,7 @@ int sta_paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, v
  * chunk_size - local_window a multiple of 64, pos_scale 1).  Angles are formed in 64 bits.
  * With weights_out (laid out like the cache's weights, possibly the same array) slot j of kv
  * head h gets weights[j] + the sum over h's q heads of the attention weight of j; other slots
- * are left as they were, and pages must not be shared between sequences then. */
+ * are left as they were, and no page may stand in the table twice then (among the entries in use). */
 typedef struct sta_paged_decode_args {
   const void* q; int64_t q_stride_b; int64_t q_stride_h;   /* (batch, n_heads, d) */
   void* out;               /* (batch, n_heads, d) contiguous, dtype, 16-byte aligned */
@@ -615,7 +615,7 @@ int sta_paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, v
 /* Keep min(lens[b], budget) slots of every sequence and kv head: the first n_global, the last
  * n_local, and of the others those with the largest weight (ties: lowest slot; NaN counts as
  * the smallest).  Kept rows of K, V and weights are copied in order into the pages of table_out
- * (none of which may hold rows of the input), so a kept key's rank is its slot and position
+ * (all different, and none of which may hold rows of the input), so a kept key's rank is its slot and position
  * there; kept receives the original slots (-1 beyond), lens_out the new lengths.
  * n_global + n_local <= budget. */
 typedef struct sta_paged_evict_args {

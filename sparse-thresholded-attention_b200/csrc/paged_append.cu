@@ -31,7 +31,7 @@ struct AppP {
 
 __device__ __forceinline__ int new_len(const AppP& p, int b, int len, int& cnt) {
   cnt = (int)p.n;
-  if (p.counts) cnt = min(max(__ldg(p.counts + b), 0), (int)p.n);
+  if (p.counts) cnt = min(max(p.counts[b], 0), (int)p.n);  // (may be overwritten: not a read-only load)
   return (uint32_t)len + (uint32_t)cnt > p.c.cap ? (int)p.c.cap : len + cnt;
 }
 
@@ -68,7 +68,7 @@ __global__ void __launch_bounds__(kThreads, 4) paged_append_kernel(const AppP p)
                          (int)min((int64_t)32, units - u0), p.es);
     }
     if (p.store_lens && blockIdx.x == 0) {
-      __syncthreads();  // lens_out may be lens: every thread of the (then only) block has read it
+      __syncthreads();  // lens_out may be lens or counts: every thread of the (then only) block has read them
       if (tid == 0) p.lens_out[b] = total;
     }
   }
@@ -100,6 +100,8 @@ int paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, cudaS
   if (a->n > 0 && c->batch > 0 && (!a->k || !a->v)) return fail(STA_ERR_ARG, "sta_paged_append: null pointer");
   if (a->lens_out != c->lens && a->lens_out < c->lens + c->batch && c->lens < a->lens_out + c->batch)
     return fail(STA_ERR_ARG, "sta_paged_append: lens_out overlaps lens without being it");
+  if (a->counts && a->lens_out != a->counts && a->lens_out < a->counts + c->batch && a->counts < a->lens_out + c->batch)
+    return fail(STA_ERR_ARG, "sta_paged_append: lens_out overlaps counts without being it");
   if (c->batch == 0) return STA_OK;
   AppP p;
   p.c = paged_view(c);
@@ -119,8 +121,9 @@ int paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, cudaS
   const int64_t gx = (a->n * c->n_kv_heads + kUnits - 1) / kUnits;
   if (gx > ((int64_t)1 << 31) - 1) return fail(STA_ERR_UNSUPPORTED, "sta_paged_append: too many rows");
   const dim3 grid((unsigned)(gx > 0 ? gx : 1), (unsigned)(c->batch < 65535 ? c->batch : 65535));
-  // a length that is overwritten in place is read by one block only, or stored by a second launch
-  p.store_lens = a->lens_out != c->lens || grid.x == 1;
+  // a length or count that is overwritten in place is read by one block only, or the lengths are
+  // stored by a second launch
+  p.store_lens = (a->lens_out != c->lens && a->lens_out != a->counts) || grid.x == 1;
   cudaError_t e = ch == 8 ? launch<8>(p, vec, grid, st)
                           : (ch == 16 ? launch<16>(p, vec, grid, st) : launch<32>(p, vec, grid, st));
   if (e == cudaSuccess && !p.store_lens)

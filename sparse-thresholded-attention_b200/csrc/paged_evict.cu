@@ -3,7 +3,7 @@
 // Per (sequence, kv head) the min(len, budget) slots to keep are the forced ones (first n_global,
 // last n_local) and the heaviest others, ties to the lowest slot.  Two launches:
 //
-// Selection, one CTA per (sequence, kv head), or a cluster of up to 8 where the slots exceed 8192
+// Selection, one CTA per (sequence, kv head), or a cluster of up to 8 where the slots exceed 16384
 // per CTA; each CTA holds a contiguous slice.  The weights become order-preserving integer keys in
 // shared memory; the key of the last kept slot is found by radix selection (11 + 11 + 10 bits):
 // every CTA counts its slice, reads all CTAs' counts (distributed shared memory) and finds the

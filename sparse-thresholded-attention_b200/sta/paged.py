@@ -141,7 +141,8 @@ class PagedCache:
 def append(cache: PagedCache, k, v, *, counts=None, lens_out=None):
     """Write the first ``counts[b]`` of the rows k, v (batch, Hkv, n, D) to slots ``lens[b]`` on of
     sequence b (counts None: all n; a decode step has n = 1), set their weights to zero, and
-    return the new lengths in ``lens_out`` (batch,) int32 (default: the cache's own ``lens``).
+    return the new lengths in ``lens_out`` (batch,) int32 (default: the cache's own ``lens``; it may
+    be ``counts``).
     The caller has put pages for the new slots into the table; rows past its last slot are
     dropped and reported by ``core.device_error()``."""
     a = cache._args
@@ -181,8 +182,8 @@ def decode(q, cache: PagedCache, geometry: Geometry, *, sm_scale=None, weights_o
 
     With ``weights_out`` (a tensor with the shape and strides of the cache's ``weights``, or the
     weights themselves) every slot receives its weight plus the attention weight that this token
-    gave it, summed over the q heads of its kv head; pages must not be shared between sequences
-    then."""
+    gave it, summed over the q heads of its kv head; no page may stand in the table twice then
+    (among the entries in use)."""
     a = cache._args
     dev = cache.device
     _on(q, dev, cache.k.dtype, (a.batch, None, a.d), "q")
@@ -199,8 +200,9 @@ def decode(q, cache: PagedCache, geometry: Geometry, *, sm_scale=None, weights_o
                           cache._scale if sm_scale is None else float(sm_scale))
     if geometry.dca is not None:
         size, window = int(geometry.dca[0]), int(geometry.dca[1])
-        if window <= 0 or size <= window or (size - window) % 64:
-            raise ValueError(f"dca {size, window}: chunk_size - local_window must be a positive multiple of 64")
+        if window <= 0 or size <= window or (size - window) % 64 or size >= 1 << 31:
+            raise ValueError(f"dca {size, window}: chunk_size - local_window must be a positive multiple of 64"
+                             " (and chunk_size below 2^31)")
         b.chunk_size, b.local_window = size, window
     if weights_out is not None:
         if cache.weights is None:
@@ -221,8 +223,8 @@ def evict(cache: PagedCache, budget: int, table_out, *, n_global=32, n_local=32)
     """Cut every sequence to at most ``budget`` keys per kv head: the first ``n_global``, the last
     ``n_local``, and of the others those with the largest ``weights`` (ties: lowest slot).  The
     kept rows of k, v and weights are copied, in order, into the pages of ``table_out`` (batch,
-    >= ceil(min(budget, slots) / page_size)) int32, which must not hold rows of the cache; the old
-    pages stay as they are (they may be shared) until the caller frees them.
+    >= ceil(min(budget, slots) / page_size)) int32, all different, which must not hold rows of the
+    cache; the old pages stay as they are (they may be shared) until the caller frees them.
 
     Returns (the cache over the new pages, kept (batch, Hkv, budget) int32: the original slots in
     order, -1 beyond a sequence's new length)."""

@@ -270,6 +270,26 @@ def test_append(dtype, D, hk, page, lens, n, counts):
                 assert torch.equal(d[x].cpu(), want[x]), x
 
 
+@pytest.mark.parametrize("n", [1, 90, 5000])  # one block per sequence, and many
+def test_append_leaves_the_lengths_in_the_counts(n):
+    lens, counts = [0, 10, 3], [n, n // 2, 0]
+    total = [a + b for a, b in zip(lens, counts)]
+    c = ref.make([n + 10] * 3, hk=4, D=64, page=16, dtype=torch.bfloat16, seed=44)
+    c["lens"] = torch.tensor(lens, dtype=torch.int32)
+    new = torch.randn((3, 4, n, 64), generator=torch.Generator().manual_seed(45)).bfloat16()
+    want = c["k"].clone()
+    for b in range(3):
+        j = torch.arange(lens[b], total[b])
+        want[c["table"][b, j // 16].long(), :, j % 16] = new[b, :, :counts[b]].transpose(0, 1)
+    rows = new.cuda()
+    for _ in range(5):
+        d, cache = on_gpu(c)
+        cnt = torch.tensor(counts, dtype=torch.int32, device="cuda")
+        assert paged.append(cache, rows, rows, counts=cnt, lens_out=cnt) is cnt
+        assert cnt.tolist() == total and d["lens"].tolist() == lens
+        assert torch.equal(d["k"].cpu(), want)
+
+
 def test_append_without_weights_and_of_nothing():
     c = ref.make([5], hk=2, D=64, page=4, dtype=torch.float32, seed=43)
     d, cache = on_gpu(c, weights=False)

@@ -116,6 +116,14 @@ def test_bad_appends_are_refused():
     refused(lib.sta_paged_append(ctypes.byref(c), app(lens_out=256 + 4), None), b"overlaps")
 
 
+@pytest.mark.parametrize("offset", [-4, 4])
+def test_lengths_must_not_overlap_part_of_the_counts(offset):
+    lib, c = L.lib(), cache_args()
+    assert c.batch > 1
+    a = L.PagedAppendArgs(256, 128, 128, 128, 256, 128, 128, 128, 1, 4096, 4096 + offset)
+    refused(lib.sta_paged_append(ctypes.byref(c), ctypes.byref(a), None), b"overlaps counts")
+
+
 def test_an_empty_batch_is_a_no_op():
     lib, c = L.lib(), cache_args(batch=0)
     app = L.PagedAppendArgs(256, 128, 128, 128, 256, 128, 128, 128, 1, None, 4096)
