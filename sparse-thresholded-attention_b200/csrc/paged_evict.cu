@@ -8,11 +8,16 @@
 // shared memory; the key of the last kept slot is found by radix selection (11 + 11 + 10 bits):
 // every CTA counts its slice, reads all CTAs' counts (distributed shared memory) and finds the
 // digit, one cluster barrier per digit; then each CTA writes its kept slots in order.  It reads 4
-// bytes per slot and is bound by latency.
+// bytes per slot and is bound by latency: 14 us for 128 heads of up to 8192 slots (a CTA each),
+// 23 us for 32 heads of 65536 (clusters of four).  Weights are read four at a time where pages and
+// strides allow it (one at a time: 17 and 28 us), and the keys lie in shared memory as long as a
+// slice fits (in global memory: 15 and 32 us).
 //
 // Copy of the kept rows of K, V and weights into the new pages, 8 to 32 rows per warp wherever
 // they come from, set up while the selection runs (programmatic launch).  Source and destination pages
-// are disjoint, so rows move independently.  Bound by HBM: rows are read and written once.
+// are disjoint, so rows move independently.  Bound by HBM: rows are read and written once (16
+// sequences cut to 2048 keys of 8 kv heads, f32, d = 128: 71 us behind the selection, 427 MB at 6.0 TB/s; 4
+// sequences cut to 8192 keys, bf16: 48 us, 270 MB at 5.6 TB/s).
 #include <cooperative_groups.h>
 
 #include "paged.cuh"
@@ -26,7 +31,12 @@ namespace {
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
-constexpr int kSlice = 16384;          // slots of a CTA that call for a larger cluster
+// Slots of a CTA that call for a larger cluster where that makes kFewCtas CTAs at most, so that the
+// clusters run at once (a CTA takes an SM): 8 heads of 65536 slots take 19 us in clusters of 8 and
+// 22 in clusters of 4, but 16 heads 38 and 23 us, 32 heads 57 and 23 us (87 with a CTA each).
+// Otherwise only twice the slots call for it.
+constexpr int kSlice = 8192;
+constexpr int kFewCtas = 64;
 constexpr int kCopy = 256;             // threads of the copy
 constexpr int kItems = 8;              // consecutive slots of a thread in the compaction
 constexpr int kChunk = kThreads * kItems;
@@ -315,8 +325,9 @@ int check(const sta_paged_cache* c, const sta_paged_evict_args* a) {
 
 int cluster_size(const sta_paged_cache* c) {
   const int64_t cap = c->table_width * c->page_size;
+  const int64_t segs = c->batch * c->n_kv_heads;
   int cl = 1;
-  while (cl < 8 && cap / cl > kSlice) cl *= 2;
+  while (cl < 8 && (cap / cl > 2 * kSlice || (cap / cl > kSlice && 2 * cl * segs <= kFewCtas))) cl *= 2;
   return cl;
 }
 
@@ -366,8 +377,10 @@ int paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* w
   if (!p.err) return fail(STA_ERR_CUDA, "sta_paged_evict: no device");
   const int ch = c->d * (c->dtype == STA_DTYPE_F32 ? 4 : 2) / 16;
   const int64_t most = p.c.cap < a->budget ? p.c.cap : a->budget;
-  // a warp has few rows where that is what it takes to give 16 warps to every SM
-  p.rows = 32;
+  // 16 rows of a warp even out ragged sequences (16 of them as above: 71 us, with 32 rows 74; equal
+  // ones 48 and 47 us), 8 where that is what it takes to give 16 warps to every SM (1024 rows of 8
+  // kv heads: the call's device time is 9 us, with 32 rows 12)
+  p.rows = 16;
   while (p.rows > 8 && most * p.c.Hkv * p.c.B < (int64_t)p.rows * 16 * 148) p.rows /= 2;
   const int64_t per = (int64_t)p.rows * (kCopy / 32);
   const dim3 grid((unsigned)((most + per - 1) / per), (unsigned)p.c.Hkv, (unsigned)p.c.B);
