@@ -19,6 +19,7 @@ struct PDecP {
   int unit;          // log2 of the keys of a unit of work
   int W, min_log;    // shares at most, log2 of the units of a share at least
   int sms;
+  int merge;         // bf16: whether a CTA may join its shares' partials; shares from which on it does
   int64_t k16, v16;  // bytes of 16 rows
   const float* inv_freq;
   double pos_scale;
@@ -103,7 +104,7 @@ __device__ __forceinline__ void step(const PDecP& p, Place& a) {
 // `lane` (0 beyond the batch).
 struct Share {
   int count;
-  bool merge;  // enough shares per CTA to join their partials there (else the join takes them all)
+  bool merge;  // the CTA joins its shares' partials (else the join takes them all)
   Place at;
 };
 
@@ -128,7 +129,7 @@ __device__ __forceinline__ Share find_share(const PDecP& p, int len, int64_t& me
   }
   const int64_t shares = n_shares(p, total);
   Share s{};
-  s.merge = shares > 3 * (int64_t)gridDim.x;
+  s.merge = shares >= p.merge;
   int64_t end = shares;
   me = blockIdx.x;
   if (WARP_SHARES) {

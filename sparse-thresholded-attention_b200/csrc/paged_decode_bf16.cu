@@ -15,6 +15,12 @@
 // per warp (d = 128) are in flight all the time; 12 warps per SM hide each other's latencies.  The
 // cos / sin of the 64 key offsets of a tile lie in shared memory in the order the lanes read them,
 // the queries of a tile in registers as B fragments.
+//
+// Measured with 4 q heads per kv head, d = 128, the join included: 131072 keys of 8 kv heads 98 us
+// (537 MB of cache, 5.5 TB/s; a call by itself 94, in a row the card is at its power limit and the SM
+// clock falls from 1965 to 1690 MHz), 32768 keys 35 us.  The read itself runs at 7 TB/s; some 16 us
+// go to the start (lengths, page table, first rows: a chain of loads), uneven ends and the join.
+// An SM issues in 53 % of its cycles, the tensor pipe is active in 25 %.
 #include "mma_frag.cuh"
 #include "paged_decode.cuh"
 
@@ -621,12 +627,20 @@ int launch(const PDecP& p, cudaStream_t st) {
   if (e != cudaSuccess) return fail(STA_ERR_CUDA, cudaGetErrorString(e));
   // shares go to the CTAs in turn, so few shares spread over the SMs
   const int grid = p.W < p.sms * Cfg<D, NT>::CTAS ? p.W : p.sms * Cfg<D, NT>::CTAS;
-  const cudaError_t r = launch_behind(paged_decode_bf16_kernel<D, NT, MODE>, dim3((unsigned)grid), NW * 32, p, st, bytes);
+  // a CTA joins its shares' open ends where it has more than three shares, so that it has some to
+  // join, and segments are cut into many (16 on average): then the join gets shorter by more than
+  // the barrier at the end costs (one sequence of 32768 keys, 8 kv heads: 35.0 us, without 36.3;
+  // 32 ragged sequences up to 8192, 7 shares each: 91.6 us with, 89.6 without)
+  PDecP q = p;
+  q.merge = p.merge ? 3 * grid + 1 : 1 << 30;
+  const cudaError_t r = launch_behind(paged_decode_bf16_kernel<D, NT, MODE>, dim3((unsigned)grid), NW * 32, q, st, bytes);
   return r == cudaSuccess ? STA_OK : fail(STA_ERR_CUDA, cudaGetErrorString(r));
 }
 
 template <int D, int NT>
 int launch(const PDecP& p, cudaStream_t st) {
+  // rows found one by one cost more (32768 keys of 8 kv heads, d = 128: 38.7 us, in one page of dense
+  // rows 35.1); the stride of dense rows folds into the copies' addresses (as a variable 36.3 us)
   if (p.c.page % 16 != 0) return launch<D, NT, kAnyRows>(p, st);
   if (p.c.ksn == 2 * D && p.c.vsn == 2 * D) return launch<D, NT, kDenseRows>(p, st);
   return launch<D, NT, kPageRows>(p, st);
