@@ -52,7 +52,7 @@ struct EvP {
   int32_t* lens_out;
   int rows;           // rows of a warp in the copy: 8, 16 or 32
   int quads;          // weights of four neighbouring slots may be loaded at once
-  uint32_t* keys;     // (B, Hkv, cap) where a slice exceeds shared memory, else null
+  uint32_t* keys;     // (B, Hkv, cap rounded up to 4) where a slice exceeds shared memory, else null
   int* err;
 };
 
@@ -104,7 +104,7 @@ __device__ __forceinline__ uint4 far_words(const uint32_t* mine, int q) {
 }
 
 __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP p) {
-  extern __shared__ uint32_t s_keys[];
+  extern __shared__ __align__(16) uint32_t s_keys[];
   __shared__ SmemE sm;
   cg::cluster_group cluster = cg::this_cluster();
   grid_wait();
@@ -123,55 +123,73 @@ __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP 
     for (int i = tid; i < cnt; i += kThreads) kept[lo + i] = lo + i;
     return;
   }
-  uint32_t* keys = p.keys ? p.keys + ((int64_t)b * p.c.Hkv + h) * p.c.cap + lo : s_keys;
+  uint32_t* keys = p.keys ? p.keys + ((int64_t)b * p.c.Hkv + h) * ((p.c.cap + 3) & ~3u) + lo : s_keys;
 
-  // ---- keys
+  // ---- keys, and the count of their first digits; the loads of a thread are asked for together
   for (int i = tid; i < 3 * kBins; i += kThreads) sm.hist[0][i] = 0u;
-  auto key_of = [&](int j, float w) {
-    return j < p.n_global || j >= len - p.n_local ? 0xffffffffu : weight_key(w);
-  };
-  if (p.quads) {  // four neighbouring slots share a page and a 16-byte load
-#pragma unroll 4
-    for (int i = tid * 4; i < cnt; i += kThreads * 4) {
-      const int j = lo + i;
-      const uint32_t t = (uint32_t)j / p.c.page;
-      const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
-      float4 w = make_float4(__int_as_float(0x7fffffff), 0.f, 0.f, 0.f);
-      if (pg < 0) {
-        atomicCAS(p.err, 0, kErrPageEvict);
-        w.y = w.z = w.w = w.x;
-      } else {
-        w = *reinterpret_cast<const float4*>(p.c.w + pg * p.c.wsp + h * p.c.wsh + ((uint32_t)j - t * p.c.page));
-      }
-      const float x[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        if (i + k < cnt) keys[i + k] = key_of(j + k, x[k]);
-    }
-  } else {
-#pragma unroll 4
-    for (int i = tid; i < cnt; i += kThreads) {
-      const int j = lo + i;
-      const uint32_t t = (uint32_t)j / p.c.page;
-      const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
-      float w = __int_as_float(0x7fffffff);  // of a bad page: the smallest
-      if (pg < 0) atomicCAS(p.err, 0, kErrPageEvict);
-      else w = p.c.w[pg * p.c.wsp + h * p.c.wsh + ((uint32_t)j - t * p.c.page)];
-      keys[i] = key_of(j, w);
-    }
-  }
   if (tid < 4) sm.counts[tid] = 0u;
   __syncthreads();
+  auto take_key = [&](int i, float w) {  // of slot lo + i
+    const int j = lo + i;
+    const uint32_t key = j < p.n_global || j >= len - p.n_local ? 0xffffffffu : weight_key(w);
+    if (i < cnt) atomicAdd(&sm.hist[0][~(key >> 21) & (kBins - 1)], 1u);
+    return key;
+  };
+  constexpr int U = 4;
+  const int32_t* table = p.c.table + b * p.c.ts;
+  const float* weights = p.c.w + h * p.c.wsh;
+  const float nan = __int_as_float(0x7fffffff);  // of a bad page: the smallest
+  const int step = p.quads ? 4 : 1;  // quads: four neighbouring slots share a page and a 16-byte load
+  for (int i0 = tid * step; i0 < cnt; i0 += U * kThreads * step) {
+    int32_t entry[U];
+    uint32_t slot[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint32_t j = (uint32_t)(lo + i0 + u * kThreads * step), t = j / p.c.page;
+      slot[u] = j - t * p.c.page;
+      entry[u] = i0 + u * kThreads * step < cnt ? __ldg(table + t) : 0;
+    }
+    float4 w[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kThreads * step;
+      const bool ok = entry[u] >= 0 && entry[u] < p.c.n_pages;
+      const float* src = weights + entry[u] * p.c.wsp + slot[u];
+      w[u] = make_float4(nan, nan, nan, nan);
+      if (i < cnt && ok) {
+        if (p.quads) w[u] = *reinterpret_cast<const float4*>(src);
+        else w[u].x = *src;
+      }
+      if (!ok) atomicCAS(p.err, 0, kErrPageEvict);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int i = i0 + u * kThreads * step;
+      if (i >= cnt) break;
+      if (p.quads)  // (a slice has room for a multiple of four)
+        *reinterpret_cast<uint4*>(keys + i) = make_uint4(take_key(i, w[u].x), take_key(i + 1, w[u].y),
+                                                         take_key(i + 2, w[u].z), take_key(i + 3, w[u].w));
+      else
+        keys[i] = take_key(i, w[u].x);
+    }
+  }
 
   // ---- the n-th largest key of all slices, and how many of its equals are kept
   uint32_t prefix = 0u, mask = 0u, need = (uint32_t)n;
+  uint32_t above = 0u, equal = 0u;  // this slice's slots above the key (this thread's bins), and equal
 #pragma unroll 1
   for (int round = 0; round < 3; ++round) {
     const int bits = round < 2 ? 11 : 10, shift = round == 0 ? 21 : (round == 1 ? 10 : 0);
     uint32_t* hist = sm.hist[round];
-    for (int i = tid; i < cnt; i += kThreads) {
-      const uint32_t key = keys[i];
-      if ((key & mask) == prefix) atomicAdd(&hist[~(key >> shift) & ((1u << bits) - 1u)], 1u);
+    if (round > 0) {
+      for (int i = tid * 4; i < cnt; i += kThreads * 4) {
+        const uint4 four = *reinterpret_cast<const uint4*>(keys + i);
+        const uint32_t key[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (i + k < cnt && (key[k] & mask) == prefix)
+            atomicAdd(&hist[~(key[k] >> shift) & ((1u << bits) - 1u)], 1u);
+      }
     }
     cluster.sync();
     // this thread's four bins (bin i counts digit bins - 1 - i) of all slices
@@ -200,6 +218,13 @@ __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP 
       before += c[i];
     }
     __syncthreads();
+    const uint32_t bin = ((1u << bits) - 1u) - sm.digit;
+    if (tid * 4 < (1 << bits)) {
+      const uint4 mine = *reinterpret_cast<const uint4*>(hist + tid * 4);
+      above += (tid * 4u < bin ? mine.x : 0u) + (tid * 4u + 1u < bin ? mine.y : 0u) +
+               (tid * 4u + 2u < bin ? mine.z : 0u) + (tid * 4u + 3u < bin ? mine.w : 0u);
+    }
+    equal = hist[bin];  // (of the last round)
     prefix |= sm.digit << shift;
     mask |= ((1u << bits) - 1u) << shift;
     need = sm.rest;
@@ -207,17 +232,9 @@ __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP 
   }
 
   // ---- where this slice's kept slots go
-  uint32_t above = 0, equal = 0;
-  for (int i = tid; i < cnt; i += kThreads) {
-    above += keys[i] > prefix;
-    equal += keys[i] == prefix;
-  }
   above = __reduce_add_sync(0xffffffffu, above);
-  equal = __reduce_add_sync(0xffffffffu, equal);
-  if (lane == 0) {
-    atomicAdd(&sm.counts[0], above);
-    atomicAdd(&sm.counts[1], equal);
-  }
+  if (lane == 0) atomicAdd(&sm.counts[0], above);
+  if (tid == 0) sm.counts[1] = equal;
   cluster.sync();
   // lane q: slots of slice q above and equal; the equals go to the slices in order
   uint4 c = lane < CL ? far_words(sm.counts, lane) : make_uint4(0u, 0u, 0u, 0u);
@@ -246,8 +263,12 @@ __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP 
     const int i = i0 + tid * kItems;
     uint32_t key[kItems], x = 0;
 #pragma unroll
+    for (int k = 0; k < kItems; k += 4) {
+      const uint4 four = i + k < cnt ? *reinterpret_cast<const uint4*>(keys + i + k) : make_uint4(0u, 0u, 0u, 0u);
+      key[k] = four.x; key[k + 1] = four.y; key[k + 2] = four.z; key[k + 3] = four.w;
+    }
+#pragma unroll
     for (int k = 0; k < kItems; ++k) {
-      key[k] = i + k < cnt ? keys[i + k] : 0u;
       if (i + k < cnt) x += key[k] > prefix ? 1u : (key[k] == prefix ? 1u << 16 : 0u);
     }
     uint32_t all;
@@ -349,7 +370,7 @@ cudaError_t launch_select(const EvP& p, int cl, cudaStream_t st) {
 
 size_t paged_evict_workspace_bytes(const sta_paged_cache* c, const sta_paged_evict_args* a) {
   if (check(c, a) != STA_OK) return 0;
-  const size_t keys = (size_t)(c->batch * c->n_kv_heads) * (c->table_width * c->page_size) * 4;
+  const size_t keys = (size_t)(c->batch * c->n_kv_heads) * ((c->table_width * c->page_size + 3) & ~(int64_t)3) * 4;
   return (keys_in_smem(c) ? 0 : keys) + 256;
 }
 
