@@ -8,10 +8,11 @@
 // shared memory; the key of the last kept slot is found by radix selection (11 + 11 + 10 bits):
 // every CTA counts its slice, reads all CTAs' counts (distributed shared memory) and finds the
 // digit, one cluster barrier per digit; then each CTA writes its kept slots in order.  It reads 4
-// bytes per slot and is bound by latency: 14 us for 128 heads of up to 8192 slots (a CTA each),
-// 23 us for 32 heads of 65536 (clusters of four).  Weights are read four at a time where pages and
-// strides allow it (one at a time: 17 and 28 us), and the keys lie in shared memory as long as a
-// slice fits (in global memory: 15 and 32 us).
+// bytes per slot and is bound by latency: 12 us for 128 heads of up to 8192 slots (a CTA each),
+// 20 us for 32 heads of 65536 (clusters of four: 6 us until the keys are there, 2.4 us per digit,
+// 4 us for the order).  Weights are read four at a time where pages and strides allow it (one at a
+// time: 13.5 us for the 128 heads), and the keys lie in shared memory as long as a slice fits (in
+// global memory: 22 us for the 32 heads).
 //
 // Copy of the kept rows of K, V and weights into the new pages, 8 to 32 rows per warp wherever
 // they come from, set up while the selection runs (programmatic launch).  Source and destination pages
@@ -32,9 +33,9 @@ constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 2048;
 // Slots of a CTA that call for a larger cluster where that makes kFewCtas CTAs at most, so that the
-// clusters run at once (a CTA takes an SM): 8 heads of 65536 slots take 19 us in clusters of 8 and
-// 22 in clusters of 4, but 16 heads 38 and 23 us, 32 heads 57 and 23 us (87 with a CTA each).
-// Otherwise only twice the slots call for it.
+// clusters run at once (a CTA takes an SM): 8 heads of 16384 slots take 12.5 us in clusters of 2 and
+// 15 with a CTA each, but 16 heads of 65536 slots 38 us in clusters of 8 and 18.5 in clusters of 4,
+// 32 heads 57 and 20 us (46 with a CTA each).  Otherwise only twice the slots call for it.
 constexpr int kSlice = 8192;
 constexpr int kFewCtas = 64;
 constexpr int kCopy = 256;             // threads of the copy
@@ -58,8 +59,8 @@ struct EvP {
 
 struct __align__(16) SmemE {
   uint32_t hist[3][kBins];  // of each digit (others may still read the one before)
-  uint32_t scan[kWarps];
-  uint32_t digit, rest;  // the digit found and how many of its slots are kept
+  uint32_t scan[2][kWarps];
+  uint32_t digit[3], rest[3];  // the digits found and how many of their slots are kept
   __align__(16) uint32_t counts[4];  // slots of the slice above the last kept key, and equal to it
 };
 
@@ -80,7 +81,7 @@ __device__ __forceinline__ uint32_t warp_incl_sum(uint32_t x) {
   return x;
 }
 
-// (ends behind a barrier; every warp sums the warps' totals for itself)
+// (every warp sums the warps' totals for itself; calls in a row take two buffers in turn)
 __device__ __forceinline__ uint32_t block_excl_sum(uint32_t x, uint32_t* sh, uint32_t& total) {
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const uint32_t inc = warp_incl_sum(x);
@@ -89,7 +90,6 @@ __device__ __forceinline__ uint32_t block_excl_sum(uint32_t x, uint32_t* sh, uin
   const uint32_t sums = warp_incl_sum(lane < kWarps ? sh[lane] : 0u);
   const uint32_t base = __shfl_sync(0xffffffffu, sums, w == 0 ? 0 : w - 1);
   total = __shfl_sync(0xffffffffu, sums, 31);
-  __syncthreads();
   return (w == 0 ? 0u : base) + inc - x;
 }
 
@@ -208,27 +208,26 @@ __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP 
     }
     const uint32_t sum = c[0] + c[1] + c[2] + c[3];
     uint32_t all;
-    uint32_t before = block_excl_sum(sum, sm.scan, all);
+    uint32_t before = block_excl_sum(sum, sm.scan[0], all);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       if (before < need && before + c[i] >= need) {
-        sm.digit = (uint32_t)((1 << bits) - 1 - tid * 4 - i);
-        sm.rest = need - before;
+        sm.digit[round] = (uint32_t)((1 << bits) - 1 - tid * 4 - i);
+        sm.rest[round] = need - before;
       }
       before += c[i];
     }
     __syncthreads();
-    const uint32_t bin = ((1u << bits) - 1u) - sm.digit;
+    const uint32_t bin = ((1u << bits) - 1u) - sm.digit[round];
     if (tid * 4 < (1 << bits)) {
       const uint4 mine = *reinterpret_cast<const uint4*>(hist + tid * 4);
       above += (tid * 4u < bin ? mine.x : 0u) + (tid * 4u + 1u < bin ? mine.y : 0u) +
                (tid * 4u + 2u < bin ? mine.z : 0u) + (tid * 4u + 3u < bin ? mine.w : 0u);
     }
     equal = hist[bin];  // (of the last round)
-    prefix |= sm.digit << shift;
+    prefix |= sm.digit[round] << shift;
     mask |= ((1u << bits) - 1u) << shift;
-    need = sm.rest;
-    __syncthreads();
+    need = sm.rest[round];
   }
 
   // ---- where this slice's kept slots go
@@ -255,7 +254,6 @@ __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP 
   }
   const int base = (int)__shfl_sync(0xffffffffu, upto - holds, rank);
   const uint32_t ties = __shfl_sync(0xffffffffu, take, rank);
-  const int mine = (int)__shfl_sync(0xffffffffu, holds, rank);
 
   // ---- the kept slots in order
   uint32_t done_above = 0, done_equal = 0;
@@ -272,7 +270,7 @@ __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP 
       if (i + k < cnt) x += key[k] > prefix ? 1u : (key[k] == prefix ? 1u << 16 : 0u);
     }
     uint32_t all;
-    const uint32_t at = block_excl_sum(x, sm.scan, all);
+    const uint32_t at = block_excl_sum(x, sm.scan[i0 / kChunk & 1], all);
     uint32_t a = done_above + (at & 0xffffu), e = done_equal + (at >> 16);
 #pragma unroll
     for (int k = 0; k < kItems; ++k) {
@@ -400,7 +398,7 @@ int paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* w
   const int64_t most = p.c.cap < a->budget ? p.c.cap : a->budget;
   // 16 rows of a warp even out ragged sequences (16 of them as above: 71 us, with 32 rows 74; equal
   // ones 48 and 47 us), 8 where that is what it takes to give 16 warps to every SM (1024 rows of 8
-  // kv heads: the call's device time is 9 us, with 32 rows 12)
+  // kv heads: the copy adds 3.5 us, with 32 rows 7.5)
   p.rows = 16;
   while (p.rows > 8 && most * p.c.Hkv * p.c.B < (int64_t)p.rows * 16 * 148) p.rows /= 2;
   const int64_t per = (int64_t)p.rows * (kCopy / 32);

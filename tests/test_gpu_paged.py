@@ -354,6 +354,16 @@ def test_evict(dtype, D, hk, page, lens, budget, n_global, n_local, kind):
         assert torch.equal(torch.nan_to_num(got.float(), nan=-1.5), torch.nan_to_num(want.float(), nan=-1.5)), x
 
 
+def test_evict_with_keys_in_a_workspace_of_odd_rows():
+    """165005 slots a sequence (no multiple of four), two sequences of two heads, pages of five."""
+    page, lens, budget = 5, [9001, 4003], 1999
+    c = ref.make(lens, hk=2, D=64, page=page, dtype=torch.bfloat16, seed=53, spare=2 * 400, width=33001)
+    d, cache = on_gpu(c)
+    after, kept = paged.evict(cache, budget, c["free"][:800].reshape(2, 400).cuda(), n_global=3, n_local=5)
+    assert core.device_error() == 0 and after.lens.tolist() == [budget] * 2
+    assert torch.equal(kept.cpu(), ref.evict(c, budget, 3, 5))
+
+
 def test_serving_run():
     """Prompts stored, steps decoded with their weights, the caches cut back, more steps: every
     step against the definition on what the cache holds then."""
