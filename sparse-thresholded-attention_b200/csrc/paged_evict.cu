@@ -145,7 +145,7 @@ __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP 
     uint32_t slot[U];
 #pragma unroll
     for (int u = 0; u < U; ++u) {
-      const uint32_t j = (uint32_t)(lo + i0 + u * kThreads * step), t = j / p.c.page;
+      const uint32_t j = (uint32_t)lo + (uint32_t)(i0 + u * kThreads * step), t = j / p.c.page;
       slot[u] = j - t * p.c.page;
       entry[u] = i0 + u * kThreads * step < cnt ? __ldg(table + t) : 0;
     }
