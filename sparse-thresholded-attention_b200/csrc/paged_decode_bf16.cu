@@ -252,7 +252,10 @@ __global__ void __launch_bounds__(Cfg<D, NT>::NW * 32, Cfg<D, NT>::CTAS)
         copy(ring_k + (k_it & 1) * (D * 32), p.c.k, p.c.k, koff, 0, 16);
       }
       if (bad) {  // the whole unit: every output of the sequence is NaN
+        // a lane waits for its own copies only: without the barrier another lane's zeros could still
+        // land on the NaN stored here
         asm volatile("cp.async.wait_all;\n" ::: "memory");
+        __syncwarp();
         if (lane == 0) atomicCAS(p.err, 0, kErrPageDecode);
         for (int i = lane; i < 16 * CH; i += 32)
           sm.k[warp][k_it & 1][i] = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
