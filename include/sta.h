@@ -632,14 +632,16 @@ size_t sta_paged_evict_workspace_bytes(const sta_paged_cache* c, const sta_paged
 int sta_paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* workspace,
                     size_t workspace_bytes, void* stream);
 
-/* Error word of the bounded device waits on the current device (0 = none; 101-104 name the
- * wait of the selection kernel that expired).  Kernels report an expired wait only through
- * this word -- the launching call has already returned STA_OK -- so a C caller that needs to
- * know polls it after the stream's work: it synchronises `stream`, stores the word in
- * *code_out, clears it, and returns STA_ERR_TIMEOUT when it was set.  Codes 201-203 come from
- * the paged cache (append, decode, evict): a page number outside the pool, or rows past the
- * table's last slot; the call then returns STA_ERR_ARG. */
+/* Error words of the current device (0 = none).  101-104 name the bounded wait of the selection
+ * kernel that expired, 201-203 come from the paged cache (append, decode, evict): a page number
+ * outside the pool, or rows past the table's last slot.  Kernels report these only here -- the
+ * launching call has already returned STA_OK -- so a C caller that needs to know polls after
+ * the stream's work: the call synchronises `stream`, stores the code in *code_out and clears it.
+ * Waits and pages have a word of their own; where both are set the wait is reported first, the
+ * page by the next call.  Returns STA_ERR_TIMEOUT for an expired wait, STA_ERR_ARG for a page. */
 int sta_device_error(void* stream, int32_t* code_out);
+/* The bounded waits alone: what a paged cache has reported stays for sta_device_error. */
+int sta_wait_error(void* stream, int32_t* code_out);
 
 #ifdef __cplusplus
 }

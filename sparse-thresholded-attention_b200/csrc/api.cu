@@ -20,7 +20,9 @@ namespace sta {
 namespace {
 thread_local char g_last_error[512] = "";
 
-__device__ int g_device_error;  // bounded-wait failure code (0 = none)
+// [0] bounded waits that expired, [1] page numbers and slots that a paged cache does not have
+// (0 = none): words of their own, so that neither hides the other or is taken for it
+__device__ int g_device_error[2];
 
 int* g_err_ptr[64] = {nullptr};
 }  // namespace
@@ -43,6 +45,11 @@ int* device_error_word() {
     g_err_ptr[dev] = static_cast<int*>(p);
   }
   return g_err_ptr[dev];
+}
+
+int* page_error_word() {
+  int* p = device_error_word();
+  return p ? p + 1 : nullptr;
 }
 
 // ------------------------------------------------------------------------------------------
@@ -646,23 +653,27 @@ int sta_paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, voi
   return paged_evict(c, a, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
 }
 
-int sta_device_error(void* stream, int32_t* code_out) {
+// reads the first `words` error words and clears the one that is reported (the first that is set)
+static int read_device_error(int words, void* stream, int32_t* code_out) {
   int* p = device_error_word();
   if (!p) return fail(STA_ERR_CUDA, "sta_device_error: symbol lookup failed");
-  int host = 0;
+  int host[2] = {0, 0};
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  cudaError_t e = cudaMemcpyAsync(&host, p, sizeof(int), cudaMemcpyDeviceToHost, st);
+  cudaError_t e = cudaMemcpyAsync(host, p, words * sizeof(int), cudaMemcpyDeviceToHost, st);
   if (e == cudaSuccess) e = cudaStreamSynchronize(st);
   if (e != cudaSuccess) return fail(STA_ERR_CUDA, cudaGetErrorString(e));
-  if (code_out) *code_out = host;
-  if (host != 0) {
-    const int zero = 0;
-    cudaMemcpyAsync(p, &zero, sizeof(int), cudaMemcpyHostToDevice, st);
-    cudaStreamSynchronize(st);
-  }
-  if (host >= 201)
-    return fail(STA_ERR_ARG, "a paged cache named a page outside its pool or had no slot for a row");
-  return host != 0 ? fail(STA_ERR_TIMEOUT, "a bounded device wait expired") : STA_OK;
+  const int at = host[0] != 0 ? 0 : 1;
+  if (code_out) *code_out = host[at];
+  if (host[at] == 0) return STA_OK;
+  const int zero = 0;
+  cudaMemcpyAsync(p + at, &zero, sizeof(int), cudaMemcpyHostToDevice, st);
+  cudaStreamSynchronize(st);
+  return at == 0 ? fail(STA_ERR_TIMEOUT, "a bounded device wait expired")
+                 : fail(STA_ERR_ARG, "a paged cache named a page outside its pool or had no slot for a row");
 }
+
+int sta_device_error(void* stream, int32_t* code_out) { return read_device_error(2, stream, code_out); }
+
+int sta_wait_error(void* stream, int32_t* code_out) { return read_device_error(1, stream, code_out); }
 
 }  // extern "C"

@@ -122,7 +122,7 @@ int paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, cudaS
   p.n = (uint32_t)a->n;
   p.counts = a->counts;
   p.lens_out = a->lens_out;
-  p.err = device_error_word();
+  p.err = page_error_word();
   if (!p.err) return fail(STA_ERR_CUDA, "sta_paged_append: no device");
   const bool vec = ((reinterpret_cast<uintptr_t>(p.k) | reinterpret_cast<uintptr_t>(p.v) | p.ksb |
                      p.ksh | p.ksn | p.vsb | p.vsh | p.vsn) & 15) == 0;

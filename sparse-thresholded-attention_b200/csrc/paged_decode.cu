@@ -685,7 +685,7 @@ int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void*
   p.scores = a->weights_out ? reinterpret_cast<float*>(w + L.scores) : nullptr;
   p.cap_tiles = L.cap_tiles;
   p.w_out = a->weights_out;
-  p.err = device_error_word();
+  p.err = page_error_word();
   if (!p.err) return fail(STA_ERR_CUDA, "sta_paged_decode: no device");
   if (f32) rc = c->d == 128 ? launch_f32<128>(p, st) : launch_f32<64>(p, st);
   else rc = launch_paged_decode_bf16(p, c->d, st);

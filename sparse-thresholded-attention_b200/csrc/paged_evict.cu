@@ -392,7 +392,7 @@ int paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* w
   p.keys = keys_in_smem(c) ? nullptr
                            : reinterpret_cast<uint32_t*>(w + (256 - reinterpret_cast<uintptr_t>(w) % 256) % 256);
   p.quads = p.c.page % 4 == 0 && (reinterpret_cast<uintptr_t>(p.c.w) & 15) == 0 && p.c.wsp % 4 == 0 && p.c.wsh % 4 == 0;
-  p.err = device_error_word();
+  p.err = page_error_word();
   if (!p.err) return fail(STA_ERR_CUDA, "sta_paged_evict: no device");
   const int ch = c->d * (c->dtype == STA_DTYPE_F32 ? 4 : 2) / 16;
   const int64_t most = p.c.cap < a->budget ? p.c.cap : a->budget;

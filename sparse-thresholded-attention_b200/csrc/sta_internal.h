@@ -18,6 +18,8 @@ int check_shared_forward(const sta_forward_args* a);
 
 // global device error word (bounded waits that expired)
 int* device_error_word();
+// that of the paged cache (pages outside the pool, rows without a slot)
+int* page_error_word();
 
 int launch_rope_split(const void* x, int dtype, int64_t heads, int64_t N, int D,
                       int64_t stride_h, int64_t stride_n, const float* inv_freq,

@@ -178,7 +178,7 @@ EXPORTED = ["sta_last_error", "sta_version", "sta_tri_head_stride", "sta_rope_sp
             "sta_decode_workspace_bytes", "sta_decode_forward", "sta_dca_workspace_bytes",
             "sta_dca_forward", "sta_select_screen_bytes", "sta_paged_append",
             "sta_paged_decode_workspace_bytes", "sta_paged_decode",
-            "sta_paged_evict_workspace_bytes", "sta_paged_evict"]
+            "sta_paged_evict_workspace_bytes", "sta_paged_evict", "sta_wait_error"]
 
 _lib = None
 
@@ -242,8 +242,10 @@ def lib():
     L.sta_select_screen_bytes.argtypes = [ctypes.POINTER(SelectArgs)]
     L.sta_shared_forward_static.restype = ctypes.c_int
     L.sta_shared_forward_static.argtypes = [ctypes.POINTER(ForwardArgs), c_vp]
-    L.sta_device_error.restype = ctypes.c_int
-    L.sta_device_error.argtypes = [c_vp, ctypes.POINTER(c_i32)]
+    for name in ("sta_device_error", "sta_wait_error"):
+        f = getattr(L, name)
+        f.restype = ctypes.c_int
+        f.argtypes = [c_vp, ctypes.POINTER(c_i32)]
     _lib = L
     return L
 

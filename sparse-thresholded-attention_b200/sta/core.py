@@ -575,10 +575,19 @@ def dca_dense(q, k, v, inv_freq, *, chunk_size, local_window, rope_scale=1.0, sm
 
 
 def device_error() -> int:
-    """Synchronise the current stream and return (and clear) the device error word of the
-    bounded waits: 0 when no wait expired since the last read."""
+    """Synchronise the current stream and return (and clear) what the kernels of the current device
+    have reported since the last read: 0 for nothing, 101-104 for a bounded wait that expired,
+    201 (append), 202 (decode) or 203 (evict) for a paged cache that named a page outside its pool
+    or had no slot for a row.  A wait is returned first, a paged cache's code by the next call."""
     code = L.c_i32(0)
     L.lib().sta_device_error(_stream(), ctypes.byref(code))
+    return int(code.value)
+
+
+def wait_error() -> int:
+    """device_error() for the bounded waits alone; a paged cache's code stays for device_error()."""
+    code = L.c_i32(0)
+    L.lib().sta_wait_error(_stream(), ctypes.byref(code))
     return int(code.value)
 
 

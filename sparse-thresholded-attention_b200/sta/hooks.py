@@ -19,8 +19,8 @@ def _check_device_waits():
     """Raise when a bounded device wait of the prefill kernels expired (the launches return
     before the kernels run, so such a failure only shows in the device error word; reading it
     synchronises the stream once per prefill call)."""
-    from .core import device_error
-    code = device_error()
+    from .core import wait_error
+    code = wait_error()
     if code:
         raise RuntimeError(f"thresholded attention: a bounded device wait expired (code {code}); "
                            "the layer output is incomplete")

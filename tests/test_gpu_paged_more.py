@@ -37,3 +37,31 @@ def test_every_key_of_a_unit_with_a_bad_page_is_nan(D, G, page, strided):
     assert core.device_error() == 202
     keep = [0, 2]
     check_decode(q[keep], dict(c, table=c["table"][keep], lens=c["lens"][keep]), out[keep], inv_freq=inv_freq(D))
+
+
+def test_a_bad_page_is_not_taken_for_an_expired_wait():
+    """The prefill hooks ask for expired waits after every layer; what a paged cache has reported by
+    then is not one, and is still there for who asks."""
+    from sta import hooks
+    c = ref.make([5], hk=1, D=64, page=4, dtype=torch.float32, seed=203)
+    c["table"][0, 1] = -1
+    _, cache = on_gpu(c)
+    assert core.device_error() == 0
+    paged.decode(torch.ones((1, 1, 64), device="cuda"), cache, Geometry(inv_freq(64).cuda()))
+    hooks._check_device_waits()
+    assert core.wait_error() == 0
+    assert core.device_error() == 202
+    assert core.device_error() == 0
+
+
+def test_an_expired_wait_and_a_bad_page_are_both_reported():
+    q = torch.randn((8, 4096, 128), generator=torch.Generator().manual_seed(204)).bfloat16().cuda()
+    c = ref.make([5], hk=1, D=64, page=4, dtype=torch.float32, seed=203)
+    c["table"][0, 1] = -1
+    _, cache = on_gpu(c)
+    assert core.device_error() == 0
+    paged.decode(torch.ones((1, 1, 64), device="cuda"), cache, Geometry(inv_freq(64).cuda()))
+    core.select(q, q[:2], torch.full((8,), 5.0), Geometry(inv_freq(128)), tile=64, wait_limit_ns=1)
+    assert core.device_error() in (101, 102, 103, 104)
+    assert core.device_error() == 202
+    assert core.device_error() == 0
