@@ -84,12 +84,20 @@ class PagedCache:
     infinity or NaN there is NaN.  What lies in slots without a token is never read.
 
     The tensors are used in place and may be written by the program between calls (new table
-    entries, new lengths); the object itself only keeps them and their addresses.  A page number
+    entries, new lengths); the object itself only keeps them and their addresses, so they are
+    read-only attributes (another table or other lengths: ``with_pages``) and their storage must
+    not be exchanged (``resize_``, ``set_``).  A page number
     outside the pool never faults: its sequence's result is NaN, its rows are dropped, and
     ``core.device_error()`` is 201 (append), 202 (decode) or 203 (evict)."""
 
-    __slots__ = ("k", "v", "table", "lens", "weights", "device", "_index", "_args", "_ref", "_sizes",
-                 "_scale")
+    __slots__ = ("_tensors", "_index", "_args", "_ref", "_sizes", "_scale")
+
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    table = property(lambda self: self._tensors[2])
+    lens = property(lambda self: self._tensors[3])
+    weights = property(lambda self: self._tensors[4])
+    device = property(lambda self: self._tensors[5])
 
     def __init__(self, k, v, table, lens, weights=None):
         if not (torch.is_tensor(k) and k.is_cuda):
@@ -105,7 +113,7 @@ class PagedCache:
         n_pages, hk, page, d = k.shape
         if weights is not None:
             _on(weights, dev, torch.float32, (n_pages, hk, page), "weights")
-        self.k, self.v, self.table, self.lens, self.weights, self.device = k, v, table, lens, weights, dev
+        self._tensors = (k, v, table, lens, weights, dev)
         a = L.PagedCacheArgs()
         a.k, a.k_stride_p, a.k_stride_h, a.k_stride_n = k.data_ptr(), k.stride(0), k.stride(1), k.stride(2)
         a.v, a.v_stride_p, a.v_stride_h, a.v_stride_n = v.data_ptr(), v.stride(0), v.stride(1), v.stride(2)
@@ -129,7 +137,8 @@ class PagedCache:
     def _moved(self, table, lens):
         """with_pages for a table (of the same batch) and lengths that have been checked."""
         c = PagedCache.__new__(PagedCache)
-        c.k, c.v, c.table, c.lens, c.weights, c.device = self.k, self.v, table, lens, self.weights, self.device
+        k, v, _, _, weights, dev = self._tensors
+        c._tensors = (k, v, table, lens, weights, dev)
         a = L.PagedCacheArgs.from_buffer_copy(self._args)
         a.table, a.lens = table.data_ptr(), lens.data_ptr()
         a.table_stride, a.table_width = table.stride(0), table.shape[1]
@@ -146,7 +155,7 @@ def append(cache: PagedCache, k, v, *, counts=None, lens_out=None):
     The caller has put pages for the new slots into the table; rows past its last slot are
     dropped and reported by ``core.device_error()``."""
     a = cache._args
-    dev = cache.device
+    pool, _, _, lens, _, dev = cache._tensors
     if not (isinstance(k, torch.Tensor) and isinstance(v, torch.Tensor)):
         raise ValueError("k and v must be tensors")
     shape = (a.batch, a.n_kv_heads, k.shape[2] if k.dim() == 4 else None, a.d)
@@ -154,7 +163,7 @@ def append(cache: PagedCache, k, v, *, counts=None, lens_out=None):
         k = k.contiguous()
     if v.dim() == 4 and v.stride(3) != 1:
         v = v.contiguous()
-    dt = cache.k.dtype
+    dt = pool.dtype
     if not (k.shape == shape and v.shape == shape and k.dtype is dt and v.dtype is dt
             and k.device == dev and v.device == dev):
         _on(k, dev, dt, shape, "k")
@@ -162,7 +171,7 @@ def append(cache: PagedCache, k, v, *, counts=None, lens_out=None):
     if counts is not None:
         _on(counts, dev, torch.int32, (a.batch,), "counts")
     if lens_out is None:
-        lens_out = cache.lens
+        lens_out = lens
     else:
         _on(lens_out, dev, torch.int32, (a.batch,), "lens_out")
     kb, kh, kn, _ = k.stride()
@@ -185,8 +194,8 @@ def decode(q, cache: PagedCache, geometry: Geometry, *, sm_scale=None, weights_o
     gave it, summed over the q heads of its kv head; no page may stand in the table twice then
     (among the entries in use)."""
     a = cache._args
-    dev = cache.device
-    _on(q, dev, cache.k.dtype, (a.batch, None, a.d), "q")
+    pool, _, _, _, weights, dev = cache._tensors
+    _on(q, dev, pool.dtype, (a.batch, None, a.d), "q")
     inv = geometry.inv_freq
     if inv.dtype is not torch.float32 or inv.device != dev or not inv.is_contiguous():
         inv = inv.to(device=dev, dtype=torch.float32).contiguous()
@@ -205,10 +214,10 @@ def decode(q, cache: PagedCache, geometry: Geometry, *, sm_scale=None, weights_o
                              " (and chunk_size below 2^31)")
         b.chunk_size, b.local_window = size, window
     if weights_out is not None:
-        if cache.weights is None:
+        if weights is None:
             raise ValueError("weights_out needs a cache with weights")
-        _on(weights_out, dev, torch.float32, cache.weights.shape, "weights_out")
-        if weights_out.stride() != cache.weights.stride():
+        _on(weights_out, dev, torch.float32, weights.shape, "weights_out")
+        if weights_out.stride() != weights.stride():
             raise ValueError("weights_out must have the strides of the cache's weights")
         b.weights_out = weights_out.data_ptr()
     ref = ctypes.byref(b)
@@ -229,7 +238,7 @@ def evict(cache: PagedCache, budget: int, table_out, *, n_global=32, n_local=32)
     Returns (the cache over the new pages, kept (batch, Hkv, budget) int32: the original slots in
     order, -1 beyond a sequence's new length)."""
     a = cache._args
-    dev = cache.device
+    dev = cache._tensors[5]
     budget = int(budget)
     _on(table_out, dev, torch.int32, (a.batch, None), "table_out")
     if budget <= 0:
