@@ -554,7 +554,8 @@ int sta_decode_forward(const sta_decode_args* a, void* workspace, size_t workspa
  * of `table` beyond a sequence's last page are not read.  A page number outside [0, n_pages)
  * never faults: what would be read there makes the sequence's result NaN, what would be written
  * there is dropped, and the device error word is set (sta_device_error).  Lengths are clamped to
- * [0, table_width * page_size].  K and V rows start on 16-byte boundaries.
+ * [0, table_width * page_size].  K and V rows start on 16-byte boundaries.  What a call writes
+ * must not lie in one place twice: strides of zero are refused there.
  * ------------------------------------------------------------------------------------- */
 typedef struct sta_paged_cache {
   void* k; int64_t k_stride_p; int64_t k_stride_h; int64_t k_stride_n;
@@ -592,7 +593,8 @@ int sta_paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, v
  * rotated where they are read: position i * pos_scale with inv_freq and cos / sin times
  * rope_scale, or, with chunk_size > 0, Dual Chunk Attention positions (as sta_dca_forward;
  * chunk_size - local_window a multiple of 64, pos_scale 1).  Angles are formed in 64 bits.
- * With weights_out (laid out like the cache's weights, possibly the same array) slot j of kv
+ * With weights_out (laid out like the cache's weights; the same array, or one that has no place
+ * in common with it) slot j of kv
  * head h gets weights[j] + the sum over h's q heads of the attention weight of j; other slots
  * are left as they were, and no page may stand in the table twice then (among the entries in use). */
 typedef struct sta_paged_decode_args {

@@ -169,4 +169,20 @@ inline int paged_check(const sta_paged_cache* c) {
   return STA_OK;
 }
 
+// Tensors that a call writes: a stride of zero (heads or pages broadcast) would send the rows of
+// several slots to one place.
+inline int paged_check_weights_written(const sta_paged_cache* c) {
+  if ((c->n_pages > 1 && c->weights_stride_p == 0) || (c->n_kv_heads > 1 && c->weights_stride_h == 0))
+    return fail(STA_ERR_ARG, "sta_paged: weights are written, their strides must not be zero");
+  return STA_OK;
+}
+
+inline int paged_check_rows_written(const sta_paged_cache* c) {
+  if ((c->n_pages > 1 && (c->k_stride_p == 0 || c->v_stride_p == 0)) ||
+      (c->n_kv_heads > 1 && (c->k_stride_h == 0 || c->v_stride_h == 0)) ||
+      (c->page_size > 1 && (c->k_stride_n == 0 || c->v_stride_n == 0)))
+    return fail(STA_ERR_ARG, "sta_paged: K / V are written, their strides must not be zero");
+  return c->weights ? paged_check_weights_written(c) : STA_OK;
+}
+
 }  // namespace sta

@@ -100,7 +100,8 @@ cudaError_t launch(const AppP& p, bool vec, dim3 grid, cudaStream_t st) {
 }  // namespace
 
 int paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, cudaStream_t st) {
-  const int rc = paged_check(c);
+  int rc = paged_check(c);
+  if (rc == STA_OK) rc = paged_check_rows_written(c);
   if (rc != STA_OK) return rc;
   if (!a || (c->batch > 0 && !a->lens_out)) return fail(STA_ERR_ARG, "sta_paged_append: null pointer");
   if (a->n < 0 || a->n > ((int64_t)1 << 31) - 65) return fail(STA_ERR_ARG, "sta_paged_append: bad n");

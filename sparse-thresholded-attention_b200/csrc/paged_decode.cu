@@ -18,6 +18,7 @@
 // f32 kernel here is bound by its fp32 arithmetic and shared memory reads: 65536 keys of 8 kv heads,
 // d = 128, take 110 us with one q head each (537 MB, 4.9 TB/s), 132 us with four.
 #include <float.h>
+#include <stdlib.h>
 
 #include <type_traits>
 
@@ -573,8 +574,21 @@ PLayout layout(const sta_paged_cache* c, const sta_paged_decode_args* a) {
   return L;
 }
 
+// Whether two arrays laid out like the weights, `delta` elements apart, have a place in common:
+// delta = a * stride_p + b * stride_h + r with |a|, |b|, |r| less than the sizes.
+bool share_places(const sta_paged_cache* c, int64_t delta) {
+  const int64_t sp = c->weights_stride_p, sh = c->weights_stride_h;
+  if (llabs(delta) > (c->n_pages - 1) * sp + (c->n_kv_heads - 1) * sh + c->page_size - 1) return false;
+  for (int64_t b = 1 - c->n_kv_heads; b < c->n_kv_heads; ++b) {
+    const int64_t rest = delta - b * sh, a0 = sp > 0 ? rest / sp : 0;  // (one of the three: |r| < stride_p)
+    for (int64_t a = a0 - 1; a <= a0 + 1; ++a)
+      if (llabs(a) < c->n_pages && llabs(rest - a * sp) < c->page_size) return true;
+  }
+  return false;
+}
+
 int check(const sta_paged_cache* c, const sta_paged_decode_args* a) {
-  const int rc = paged_check(c);
+  int rc = paged_check(c);
   if (rc != STA_OK) return rc;
   if (!a || (c->batch > 0 && (!a->q || !a->out)) || !a->inv_freq)
     return fail(STA_ERR_ARG, "sta_paged_decode: null pointer");
@@ -590,6 +604,10 @@ int check(const sta_paged_cache* c, const sta_paged_decode_args* a) {
     return fail(STA_ERR_ARG, "sta_paged_decode: Dual Chunk Attention positions take pos_scale 1");
   if (a->weights_out && !c->weights)
     return fail(STA_ERR_ARG, "sta_paged_decode: weights_out needs a cache with weights");
+  if (a->weights_out && (rc = paged_check_weights_written(c)) != STA_OK) return rc;
+  if (a->weights_out && a->weights_out != c->weights &&
+      share_places(c, (int64_t)(reinterpret_cast<intptr_t>(a->weights_out) - reinterpret_cast<intptr_t>(c->weights)) / 4))
+    return fail(STA_ERR_ARG, "sta_paged_decode: weights_out overlaps the weights without being them");
   if (a->weights_out && c->batch * c->n_kv_heads * (c->table_width * c->page_size / 1024 + 1) > ((int64_t)1 << 30))
     return fail(STA_ERR_UNSUPPORTED, "sta_paged_decode: too many slots for one update of the weights");
   if (c->batch * a->n_heads > ((int64_t)1 << 30))

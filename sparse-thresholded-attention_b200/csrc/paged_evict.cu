@@ -321,7 +321,8 @@ __global__ void __launch_bounds__(kCopy, 4) paged_evict_copy_kernel(const EvP p)
 }
 
 int check(const sta_paged_cache* c, const sta_paged_evict_args* a) {
-  const int rc = paged_check(c);
+  int rc = paged_check(c);
+  if (rc == STA_OK) rc = paged_check_rows_written(c);
   if (rc != STA_OK) return rc;
   if (!a || (c->batch > 0 && (!a->table_out || !a->kept || !a->lens_out)))
     return fail(STA_ERR_ARG, "sta_paged_evict: null pointer");

@@ -74,9 +74,10 @@ class PagedCache:
     """A batch of sequences over a pool of pages.
 
     k, v (n_pages, Hkv, page_size, D): the pool, float32 or bfloat16, D 64 or 128, any strides
-    that are multiples of 16 bytes (last dimension contiguous).  table (batch, width) int32: slot
-    j of sequence b lies in page ``table[b, j // page_size]`` at row ``j % page_size``; entries
-    past a sequence's last page are not read.  lens (batch,) int32: tokens each sequence holds.
+    that are multiples of 16 bytes (last dimension contiguous; no strides of zero where rows are
+    written).  table (batch, width) int32: slot j of sequence b lies in page
+    ``table[b, j // page_size]`` at row ``j % page_size``; entries past a sequence's last page are
+    not read.  lens (batch,) int32: tokens each sequence holds.
     weights (n_pages, Hkv, page_size) float32, optional: the attention weight that each key has
     received so far (``decode(weights_out=...)``), which ``evict`` ranks by.
 
@@ -189,8 +190,8 @@ def decode(q, cache: PagedCache, geometry: Geometry, *, sm_scale=None, weights_o
     chunk length that is a multiple of 64.  Returns out (batch, H, D); a sequence of length 0
     gives zeros.
 
-    With ``weights_out`` (a tensor with the shape and strides of the cache's ``weights``, or the
-    weights themselves) every slot receives its weight plus the attention weight that this token
+    With ``weights_out`` (a tensor with the shape and strides of the cache's ``weights`` that does
+    not overlap them, or the weights themselves) every slot receives its weight plus the attention weight that this token
     gave it, summed over the q heads of its kv head; no page may stand in the table twice then
     (among the entries in use)."""
     a = cache._args
