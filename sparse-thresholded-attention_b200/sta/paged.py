@@ -8,7 +8,9 @@ RAW keys: ``decode`` rotates them where it reads them, so one cache serves every
 (slot = position), like the sets of the PQ-Union rule.
 
 Every call launches on torch's current stream of the cache's device and reads the lengths on the
-device: nothing synchronises, and calls can be captured into CUDA graphs.
+device: nothing synchronises, and calls can be captured into CUDA graphs.  The one exception is a
+geometry whose ``inv_freq`` lies elsewhere: ``decode`` then copies it on every call, which waits
+for the copy, and refuses to be captured.
 """
 from __future__ import annotations
 
@@ -199,6 +201,8 @@ def decode(q, cache: PagedCache, geometry: Geometry, *, sm_scale=None, weights_o
     _on(q, dev, pool.dtype, (a.batch, None, a.d), "q")
     inv = geometry.inv_freq
     if inv.dtype is not torch.float32 or inv.device != dev or not inv.is_contiguous():
+        if inv.device != dev and torch.cuda.is_current_stream_capturing():
+            raise ValueError(f"inv_freq must lie on {dev} where decode is captured into a graph")
         inv = inv.to(device=dev, dtype=torch.float32).contiguous()
     if inv.numel() != a.d // 2:
         raise ValueError("inv_freq must have head_dim/2 entries")

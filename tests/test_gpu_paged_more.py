@@ -65,3 +65,23 @@ def test_an_expired_wait_and_a_bad_page_are_both_reported():
     assert core.device_error() in (101, 102, 103, 104)
     assert core.device_error() == 202
     assert core.device_error() == 0
+
+
+def test_a_capture_survives_the_refusal_of_frequencies_elsewhere():
+    c = ref.make([40], hk=2, D=64, page=16, dtype=torch.bfloat16, seed=205)
+    _, cache = on_gpu(c)
+    q = queries(1, 4, 64, torch.bfloat16, 206).cuda()
+    there = Geometry(inv_freq(64).cuda())
+    want = paged.decode(q, cache, Geometry(inv_freq(64)))
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            with pytest.raises(ValueError):
+                paged.decode(q, cache, Geometry(inv_freq(64)))
+            out = paged.decode(q, cache, there)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)

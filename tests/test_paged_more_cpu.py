@@ -72,3 +72,18 @@ def test_weights_out_is_the_weights_or_apart_from_them(strides, offset, overlaps
         refused(lib.sta_paged_decode(ctypes.byref(c), ctypes.byref(a), None, 0, None), b"overlaps the weights")
     else:
         assert need > 0 and lib.sta_paged_decode(ctypes.byref(c), ctypes.byref(a), None, 0, None) == 5
+
+
+def test_frequencies_elsewhere_are_refused_in_a_capture(monkeypatch):
+    """Copying them waits for the copy, which a capture does not survive."""
+    dev = torch.device("meta")
+    cache = paged.PagedCache.__new__(paged.PagedCache)
+    pool = torch.zeros((3, 2, 4, 64), device=dev)
+    cache._tensors = (pool, pool, None, None, None, dev)
+    cache._args, cache._sizes = cache_args(batch=2, d=64, n_kv_heads=2), {}
+    q = torch.zeros((2, 4, 64), device=dev)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    with pytest.raises(ValueError, match="inv_freq must lie on"):
+        paged.decode(q, cache, paged.Geometry(torch.ones(32)))
+    with pytest.raises(ValueError, match="head_dim/2"):  # there: the next check
+        paged.decode(q, cache, paged.Geometry(torch.ones(31, device=dev)))
