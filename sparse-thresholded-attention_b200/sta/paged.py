@@ -55,8 +55,9 @@ def _run(cache, entry, name, *args):
         L.check(rc, name)
 
 
-_device = torch._C._cuda_getDevice
-_raw_stream = torch._C._cuda_getCurrentRawStream
+# (a torch without CUDA has neither; no cache exists there that could call them)
+_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 
 def _size(cache, key, entry, name, ref):

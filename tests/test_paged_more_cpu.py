@@ -87,3 +87,17 @@ def test_frequencies_elsewhere_are_refused_in_a_capture(monkeypatch):
         paged.decode(q, cache, paged.Geometry(torch.ones(32)))
     with pytest.raises(ValueError, match="head_dim/2"):  # there: the next check
         paged.decode(q, cache, paged.Geometry(torch.ones(31, device=dev)))
+
+
+def test_the_package_imports_where_torch_has_no_cuda(monkeypatch):
+    """torch built without CUDA lacks the bindings that the calls use; importing needs none of them."""
+    import importlib.util
+    import sys
+    for name in ("_cuda_getDevice", "_cuda_getCurrentRawStream"):
+        monkeypatch.delattr(torch._C, name)
+    spec = importlib.util.spec_from_file_location("sta._paged_without_cuda", paged.__file__)
+    module = importlib.util.module_from_spec(spec)
+    monkeypatch.setitem(sys.modules, spec.name, module)
+    spec.loader.exec_module(module)
+    with pytest.raises(ValueError):
+        module.PagedCache(torch.zeros((4, 2, 16, 64)), None, None, None)
