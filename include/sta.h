@@ -594,9 +594,10 @@ int sta_paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, v
  * rope_scale, or, with chunk_size > 0, Dual Chunk Attention positions (as sta_dca_forward;
  * chunk_size - local_window a multiple of 64, pos_scale 1).  Angles are formed in 64 bits.
  * With weights_out (laid out like the cache's weights; the same array, or one that has no place
- * in common with it) slot j of kv
- * head h gets weights[j] + the sum over h's q heads of the attention weight of j; other slots
- * are left as they were, and no page may stand in the table twice then (among the entries in use). */
+ * in common with it) slot j of kv head h gets weights[j] + the sum over h's q heads of the
+ * attention weight of j; other slots are left as they were.  No page may stand in the table twice
+ * then (among the entries in use): of its places one adds its weights, which one is not defined,
+ * and the device error word is set to 204. */
 typedef struct sta_paged_decode_args {
   const void* q; int64_t q_stride_b; int64_t q_stride_h;   /* (batch, n_heads, d) */
   void* out;               /* (batch, n_heads, d) contiguous, dtype, 16-byte aligned */
@@ -636,7 +637,8 @@ int sta_paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, voi
 
 /* Error words of the current device (0 = none).  101-104 name the bounded wait of the selection
  * kernel that expired, 201-203 come from the paged cache (append, decode, evict): a page number
- * outside the pool, or rows past the table's last slot.  Kernels report these only here -- the
+ * outside the pool, or rows past the table's last slot; 204: a page that a call writes stands
+ * in the table twice.  Kernels report these only here -- the
  * launching call has already returned STA_OK -- so a C caller that needs to know polls after
  * the stream's work: the call synchronises `stream`, stores the code in *code_out and clears it.
  * Waits and pages have a word of their own; where both are set the wait is reported first, the

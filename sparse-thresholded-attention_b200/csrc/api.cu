@@ -669,7 +669,7 @@ static int read_device_error(int words, void* stream, int32_t* code_out) {
   cudaMemcpyAsync(p + at, &zero, sizeof(int), cudaMemcpyHostToDevice, st);
   cudaStreamSynchronize(st);
   return at == 0 ? fail(STA_ERR_TIMEOUT, "a bounded device wait expired")
-                 : fail(STA_ERR_ARG, "a paged cache named a page outside its pool or had no slot for a row");
+                 : fail(STA_ERR_ARG, "a paged cache named a page outside its pool or one page twice, or had no slot for a row");
 }
 
 int sta_device_error(void* stream, int32_t* code_out) { return read_device_error(2, stream, code_out); }

@@ -7,7 +7,7 @@
 
 namespace sta {
 
-enum : int { kErrPageAppend = 201, kErrPageDecode = 202, kErrPageEvict = 203 };
+enum : int { kErrPageAppend = 201, kErrPageDecode = 202, kErrPageEvict = 203, kErrPageTwice = 204 };
 
 struct PagedView {
   char* k;
@@ -47,12 +47,25 @@ __device__ __forceinline__ int paged_len(const PagedView& c, int b) {
   return n < 0 ? 0 : ((uint32_t)n > c.cap ? (int)c.cap : n);
 }
 
-// page number of slot j (j < cap) of sequence b, -1 where it lies outside the pool
+// page number in entry t of sequence b's table row, -1 where it lies outside the pool
 __device__ __forceinline__ int64_t paged_page(const PagedView& c, const int32_t* table, int64_t ts,
                                               int b, uint32_t t) {
   const int64_t pg = __ldg(table + b * ts + t);
   return pg >= 0 && pg < c.n_pages ? pg : -1;
 }
+
+// Where a page stands in a table: (sequence, entry).  Finding pages that stand there twice takes an
+// array of one place per page that nobody clears: every entry in use leaves its place at its page,
+// a later kernel looks whether its own is still there.  Of two entries that name one page exactly
+// one finds its own.  (What an earlier call left at other pages is never looked at.)
+__device__ __forceinline__ void leave_places(int2* places, int64_t n_pages, const int32_t* row, int b,
+                                             uint32_t entries, uint32_t first, uint32_t step) {
+  for (uint32_t t = first; t < entries; t += step) {
+    const int32_t pg = __ldg(row + t);
+    if (pg >= 0 && pg < n_pages) places[pg] = make_int2(b, (int)t);
+  }
+}
+__device__ __forceinline__ bool is_place(int2 x, int b, uint32_t t) { return x.x == b && x.y == (int)t; }
 
 // Moves up to 32 rows of K and V by one warp: lane l has row l's byte offsets (ks < 0: no row), `n`
 // rows in all.  Neighbouring lanes hold the 16-byte chunks (CH of a row) of K, then of V; four

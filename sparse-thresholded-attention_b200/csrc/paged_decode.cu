@@ -388,6 +388,10 @@ __global__ void __launch_bounds__(NW * 32) paged_join_kernel(const PDecP p) {
     return;
   }
   const Cut c = cut_of(p, b, hg, units);
+  // (scratch of this call, which the first kernel's wait has handed over)
+  if (p.places)
+    leave_places(p.places, p.c.n_pages, p.c.table + b * p.c.ts, b, ((uint32_t)paged_len(p.c, b) - 1) / p.c.page + 1,
+                 (uint32_t)(h * NW * 32 + tid), (uint32_t)(p.H * NW * 32));
   grid_wait();
   if (c.w0 == c.w1) return;
   float M = -INFINITY, L = 0.f, o[V];
@@ -463,7 +467,8 @@ __global__ void __launch_bounds__(NW * 32) paged_join_kernel(const PDecP p) {
 // per block.  QUADS: a thread's four neighbouring keys share a page and 16-byte accesses (page size
 // and strides multiples of four); otherwise each key is looked up.  Bound by the scores that it
 // reads, which the kernel before it left in L2: 6.5 us for 32 ragged sequences up to 8192 keys (8.4
-// key by key).
+// key by key).  A page that stands in the table twice would be read and written by several blocks
+// at once: one of its entries updates it, the others are dropped and reported.
 template <bool QUADS>
 __global__ void __launch_bounds__(kUpd) paged_weights_kernel(const PDecP p) {
   const int64_t chunks = (p.c.cap + kUpd * 4 - 1) / (kUpd * 4), seg = div_fast(blockIdx.x, chunks);
@@ -474,14 +479,17 @@ __global__ void __launch_bounds__(kUpd) paged_weights_kernel(const PDecP p) {
     grid_wait();  // no block of a chain of programmatic launches ends before the kernel ahead has
     return;
   }
-  int64_t to[QUADS ? 1 : 4];
+  constexpr int N = QUADS ? 1 : 4;
+  int64_t to[N], pg[N];
+  uint32_t t[N];
 #pragma unroll
-  for (int i = 0; i < (QUADS ? 1 : 4); ++i) {
-    to[i] = -1;
+  for (int i = 0; i < N; ++i) {
+    to[i] = pg[i] = -1;
+    t[i] = 0;
     if (j + i >= len) continue;
-    const uint32_t t = (uint32_t)(j + i) / p.c.page;
-    const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
-    if (pg >= 0) to[i] = pg * p.c.wsp + h * p.c.wsh + ((uint32_t)(j + i) - t * p.c.page);
+    t[i] = (uint32_t)(j + i) / p.c.page;
+    pg[i] = paged_page(p.c, p.c.table, p.c.ts, b, t[i]);
+    if (pg[i] >= 0) to[i] = pg[i] * p.c.wsp + h * p.c.wsh + ((uint32_t)(j + i) - t[i] * p.c.page);
   }
   float4 w = make_float4(0.f, 0.f, 0.f, 0.f);
   if (QUADS) {
@@ -493,6 +501,13 @@ __global__ void __launch_bounds__(kUpd) paged_weights_kernel(const PDecP p) {
     if (to[QUADS ? 0 : 3] >= 0) w.w = p.c.w[to[QUADS ? 0 : 3]];
   }
   grid_wait();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (to[i] >= 0 && !is_place(p.places[pg[i]], b, t[i])) {
+      to[i] = -1;
+      atomicCAS(p.err, 0, kErrPageTwice);
+    }
+  }
   const float2* ml = p.ml + (int64_t)b * p.H + h * p.G;
   const float* sc = p.scores + (((int64_t)b * p.c.Hkv + h) * p.NG * p.cap_tiles + j / kTile) * p.SG * kTile + j % kTile;
   float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -525,7 +540,7 @@ __global__ void __launch_bounds__(kUpd) paged_weights_kernel(const PDecP p) {
 }
 
 struct PLayout {
-  size_t part, part_ml, ml, scores, total;
+  size_t part, part_ml, ml, scores, places, total;
   int GT, NG, W, unit;
   int64_t cap_tiles;
 };
@@ -570,6 +585,7 @@ PLayout layout(const sta_paged_cache* c, const sta_paged_decode_args* a) {
   L.part_ml = take((size_t)2 * L.W * L.GT * 8);
   L.ml = take((size_t)c->batch * a->n_heads * 8);
   L.scores = a->weights_out ? take((size_t)(c->batch * c->n_kv_heads * L.NG) * L.cap_tiles * (G < L.GT ? G : L.GT) * kTile * 4) : 0;
+  L.places = a->weights_out ? take((size_t)c->n_pages * sizeof(int2)) : 0;
   L.total = o + 256;
   return L;
 }
@@ -701,6 +717,7 @@ int paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, void*
   p.part_ml = reinterpret_cast<float2*>(w + L.part_ml);
   p.ml = reinterpret_cast<float2*>(w + L.ml);
   p.scores = a->weights_out ? reinterpret_cast<float*>(w + L.scores) : nullptr;
+  p.places = a->weights_out ? reinterpret_cast<int2*>(w + L.places) : nullptr;
   p.cap_tiles = L.cap_tiles;
   p.w_out = a->weights_out;
   p.err = page_error_word();

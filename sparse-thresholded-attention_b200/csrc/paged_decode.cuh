@@ -31,6 +31,7 @@ struct PDecP {
   float* scores;     // (B, Hkv * NG, capacity tiles, SG, 64) or null
   int64_t cap_tiles;
   float* w_out;
+  int2* places;      // (n_pages,) with the weights: which table entry adds to a page's
   int* err;
 };
 

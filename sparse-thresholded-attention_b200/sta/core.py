@@ -578,7 +578,7 @@ def device_error() -> int:
     """Synchronise the current stream and return (and clear) what the kernels of the current device
     have reported since the last read: 0 for nothing, 101-104 for a bounded wait that expired,
     201 (append), 202 (decode) or 203 (evict) for a paged cache that named a page outside its pool
-    or had no slot for a row.  A wait is returned first, a paged cache's code by the next call."""
+    or had no slot for a row, 204 for one that named a page twice where it is written.  A wait is returned first, a paged cache's code by the next call."""
     code = L.c_i32(0)
     L.lib().sta_device_error(_stream(), ctypes.byref(code))
     return int(code.value)

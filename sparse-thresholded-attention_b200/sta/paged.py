@@ -195,8 +195,9 @@ def decode(q, cache: PagedCache, geometry: Geometry, *, sm_scale=None, weights_o
 
     With ``weights_out`` (a tensor with the shape and strides of the cache's ``weights`` that does
     not overlap them, or the weights themselves) every slot receives its weight plus the attention weight that this token
-    gave it, summed over the q heads of its kv head; no page may stand in the table twice then
-    (among the entries in use)."""
+    gave it, summed over the q heads of its kv head.  No page may stand in the table twice then
+    (among the entries in use): one of its places adds its weights, the others' are dropped, and
+    ``core.device_error()`` is 204."""
     a = cache._args
     pool, _, _, _, weights, dev = cache._tensors
     _on(q, dev, pool.dtype, (a.batch, None, a.d), "q")

@@ -8,7 +8,7 @@ import torch
 import paged_ref as ref
 from sta import core, paged
 from sta.core import Geometry
-from test_gpu_paged import check_decode, inv_freq, on_gpu, queries
+from test_gpu_paged import check_decode, inv_freq, on_gpu, queries, relative_p
 
 pytestmark = pytest.mark.gpu
 
@@ -85,3 +85,50 @@ def test_a_capture_survives_the_refusal_of_frequencies_elsewhere():
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(out, want)
+
+
+def weights_of(c, probs, base, b):
+    """What sequence b alone makes of the weights."""
+    return ref.added_weights(c, [p if i == b else p[:, :0] for i, p in enumerate(probs)], base)
+
+
+@pytest.mark.parametrize("dtype,D,page", [(torch.bfloat16, 128, 16), (torch.bfloat16, 64, 6), (torch.float32, 64, 16)])
+def test_weights_of_a_page_that_stands_in_the_table_twice(dtype, D, page):
+    """One of its places adds to them, the others are dropped and reported; pages of one sequence
+    alone are as ever.  Entries that are not in use may name any page."""
+    lens, hk, H = [64, 64, 80, 33], 2, 4
+    c = ref.make(lens, hk=hk, D=D, page=page, dtype=dtype, seed=207, width=20)
+    q = queries(4, H, D, dtype, 208)
+    geo = Geometry(inv_freq(D).cuda())
+    own = dict(c, table=c["table"].clone())
+    c["table"][3, -(-33 // page):] = c["table"][0, 0]  # not in use
+    d, cache = on_gpu(c)
+    out = paged.decode(q.cuda(), cache, geo, weights_out=d["weights"])
+    assert core.device_error() == 0
+    check_decode(q, c, out, inv_freq=inv_freq(D))
+    c["table"][1, :2] = c["table"][2, :2]  # a common prefix
+    c["table"][0, 3] = c["table"][0, 1]    # and one page twice in a sequence
+    d, cache = on_gpu(c)
+    for in_place in (False, True):
+        base = d["weights"].cpu()
+        got = d["weights"] if in_place else torch.full_like(d["weights"], -1.0)
+        out = paged.decode(q.cuda(), cache, geo, weights_out=got)
+        assert core.device_error() == 204 and core.device_error() == 0
+        check_decode(q, c, out, inv_freq=inv_freq(D))
+        got = got.cpu().double()
+        _, probs, _, size = ref.decode(q, c, inv_freq(D))
+        alone = [weights_of(c, probs, base, b) for b in range(4)]
+        # a key's added weight is below H / hk = 2, its sum below 4 (rounded to 2^-23); a lost or doubled
+        # update is off by about 1 / 32 on a page
+        tol = 2 * relative_p(dtype, size, D, 80).max() + 2.0 ** -22
+        assert tol < 1 / 64
+        for t in range(2):
+            pg = int(c["table"][2, t])
+            assert min((got[pg] - alone[b][pg]).abs().max() for b in (1, 2)) < tol
+        for b, t in ((1, 3), (2, 2), (3, 0), (0, 0)):
+            pg = int(c["table"][b, t])
+            assert (got[pg] - alone[b][pg])[:, :min(page, lens[b] - t * page)].abs().max() < tol
+        pg, n = int(c["table"][0, 1]), probs[0].shape[1]
+        p = probs[0].reshape(hk, H // hk, n).sum(1)
+        first, again = (base[pg].double() + p[:, t * page:(t + 1) * page] for t in (1, 3))
+        assert min((got[pg] - x).abs().max() for x in (first, again)) < tol
