@@ -617,10 +617,12 @@ int sta_paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, v
 
 /* Keep min(lens[b], budget) slots of every sequence and kv head: the first n_global, the last
  * n_local, and of the others those with the largest weight (ties: lowest slot; NaN counts as
- * the smallest).  Kept rows of K, V and weights are copied in order into the pages of table_out
- * (all different, and none of which may hold rows of the input), so a kept key's rank is its slot and position
- * there; kept receives the original slots (-1 beyond), lens_out the new lengths.
- * n_global + n_local <= budget. */
+ * the smallest).  Kept rows of K, V and weights are copied in order into the pages of table_out,
+ * so a kept key's rank is its slot and position there; kept receives the original slots (-1
+ * beyond), lens_out the new lengths.  n_global + n_local <= budget.
+ * The new pages must all be different and must not stand in the cache's table (among the entries
+ * in use): of a page that two entries name one entry's rows are written, of a page in use none,
+ * the other rows are dropped, and the device error word is set to 204. */
 typedef struct sta_paged_evict_args {
   int64_t budget;
   int64_t n_global;
@@ -630,15 +632,14 @@ typedef struct sta_paged_evict_args {
   int32_t* lens_out;       /* (batch,), not the cache's lens */
 } sta_paged_evict_args;
 
-/* (256 bytes where the selection fits shared memory: they are not touched then) */
 size_t sta_paged_evict_workspace_bytes(const sta_paged_cache* c, const sta_paged_evict_args* a);
 int sta_paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* workspace,
                     size_t workspace_bytes, void* stream);
 
 /* Error words of the current device (0 = none).  101-104 name the bounded wait of the selection
  * kernel that expired, 201-203 come from the paged cache (append, decode, evict): a page number
- * outside the pool, or rows past the table's last slot; 204: a page that a call writes stands
- * in the table twice.  Kernels report these only here -- the
+ * outside the pool, or rows past the table's last slot; 204: a page that a decode or
+ * evict call writes stands in a table twice.  Kernels report these only here -- the
  * launching call has already returned STA_OK -- so a C caller that needs to know polls after
  * the stream's work: the call synchronises `stream`, stores the code in *code_out and clears it.
  * Waits and pages have a word of their own; where both are set the wait is reported first, the

@@ -57,13 +57,17 @@ __device__ __forceinline__ int64_t paged_page(const PagedView& c, const int32_t*
 // Where a page stands in a table: (sequence, entry).  Finding pages that stand there twice takes an
 // array of one place per page that nobody clears: every entry in use leaves its place at its page,
 // a later kernel looks whether its own is still there.  Of two entries that name one page exactly
-// one finds its own.  (What an earlier call left at other pages is never looked at.)
+// one finds its own.  Whether a page is in use at all shows in the table entry that its place names
+// (where nobody left one, any place that an earlier call's scratch names is checked the same way).
+__device__ __forceinline__ void leave_place(int2* places, int64_t n_pages, int32_t pg, int b, uint32_t t) {
+  if (pg >= 0 && pg < n_pages) places[pg] = make_int2(b, (int)t);
+}
 __device__ __forceinline__ void leave_places(int2* places, int64_t n_pages, const int32_t* row, int b,
                                              uint32_t entries, uint32_t first, uint32_t step) {
-  for (uint32_t t = first; t < entries; t += step) {
-    const int32_t pg = __ldg(row + t);
-    if (pg >= 0 && pg < n_pages) places[pg] = make_int2(b, (int)t);
-  }
+  for (uint32_t t = first; t < entries; t += step) leave_place(places, n_pages, __ldg(row + t), b, t);
+}
+__device__ __forceinline__ uint32_t entries_of(const PagedView& c, int len) {
+  return len > 0 ? (uint32_t)(len - 1) / c.page + 1 : 0u;
 }
 __device__ __forceinline__ bool is_place(int2 x, int b, uint32_t t) { return x.x == b && x.y == (int)t; }
 

@@ -390,7 +390,7 @@ __global__ void __launch_bounds__(NW * 32) paged_join_kernel(const PDecP p) {
   const Cut c = cut_of(p, b, hg, units);
   // (scratch of this call, which the first kernel's wait has handed over)
   if (p.places)
-    leave_places(p.places, p.c.n_pages, p.c.table + b * p.c.ts, b, ((uint32_t)paged_len(p.c, b) - 1) / p.c.page + 1,
+    leave_places(p.places, p.c.n_pages, p.c.table + b * p.c.ts, b, entries_of(p.c, paged_len(p.c, b)),
                  (uint32_t)(h * NW * 32 + tid), (uint32_t)(p.H * NW * 32));
   grid_wait();
   if (c.w0 == c.w1) return;

@@ -14,9 +14,11 @@
 // time: 13.5 us for the 128 heads), and the keys lie in shared memory as long as a slice fits (in
 // global memory: 22 us for the 32 heads).
 //
-// Copy of the kept rows of K, V and weights into the new pages, 8 to 32 rows per warp wherever
+// Copy of the kept rows of K, V and weights into the new pages, 8 or 16 rows per warp wherever
 // they come from, set up while the selection runs (programmatic launch).  Source and destination pages
-// are disjoint, so rows move independently.  Bound by HBM: rows are read and written once (16
+// are disjoint, so rows move independently: a new page that holds rows of the cache, or that another
+// entry of the new table names too, is found by the places that the selection leaves, and its rows
+// are dropped and reported.  Bound by HBM: rows are read and written once (16
 // sequences cut to 2048 keys of 8 kv heads, f32, d = 128: 71 us behind the selection, 427 MB at 6.0 TB/s; 4
 // sequences cut to 8192 keys, bf16: 48 us, 270 MB at 5.6 TB/s).
 #include <cooperative_groups.h>
@@ -54,6 +56,8 @@ struct EvP {
   int rows;           // rows of a warp in the copy: 8, 16 or 32
   int quads;          // weights of four neighbouring slots may be loaded at once
   uint32_t* keys;     // (B, Hkv, cap rounded up to 4) where a slice exceeds shared memory, else null
+  int2* from;         // (n_pages,) places in the table, and in the new one
+  int2* to;
   int* err;
 };
 
@@ -119,8 +123,22 @@ __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP 
   for (int64_t r = n + (int64_t)rank * kThreads + tid; r < p.budget; r += (int64_t)CL * kThreads) kept[r] = -1;
   const int per = ((len + CL - 1) / CL + 3) & ~3;
   const int lo = min(rank * per, len), cnt = min(per, len - lo);  // this CTA's slots
+  // the places of the sequence's pages, old and new, left by all its CTAs; a thread's first entries
+  // are asked for here and left once the keys have been asked for
+  const int32_t* table = p.c.table + b * p.c.ts;
+  const int32_t* table_out = p.table_out + b * p.tos;
+  const uint32_t t0 = (uint32_t)(h * CL + rank) * kThreads + tid, steps = (uint32_t)p.c.Hkv * CL * kThreads;
+  const uint32_t olds = entries_of(p.c, len), news = entries_of(p.c, n);
+  const int32_t old0 = t0 < olds ? __ldg(table + t0) : -1, new0 = t0 < news ? __ldg(table_out + t0) : -1;
+  auto leave = [&]() {
+    leave_place(p.from, p.c.n_pages, old0, b, t0);
+    leave_place(p.to, p.c.n_pages, new0, b, t0);
+    if (olds - min(olds, t0) > steps) leave_places(p.from, p.c.n_pages, table, b, olds, t0 + steps, steps);
+    if (news - min(news, t0) > steps) leave_places(p.to, p.c.n_pages, table_out, b, news, t0 + steps, steps);
+  };
   if (len <= p.budget) {  // (the same for all CTAs of the cluster)
     for (int i = tid; i < cnt; i += kThreads) kept[lo + i] = lo + i;
+    leave();
     return;
   }
   uint32_t* keys = p.keys ? p.keys + ((int64_t)b * p.c.Hkv + h) * ((p.c.cap + 3) & ~3u) + lo : s_keys;
@@ -136,7 +154,6 @@ __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP 
     return key;
   };
   constexpr int U = 4;
-  const int32_t* table = p.c.table + b * p.c.ts;
   const float* weights = p.c.w + h * p.c.wsh;
   const float nan = __int_as_float(0x7fffffff);  // of a bad page: the smallest
   const int step = p.quads ? 4 : 1;  // quads: four neighbouring slots share a page and a 16-byte load
@@ -173,6 +190,8 @@ __global__ void __launch_bounds__(kThreads) paged_evict_select_kernel(const EvP 
         keys[i] = take_key(i, w[u].x);
     }
   }
+
+  leave();
 
   // ---- the n-th largest key of all slices, and how many of its equals are kept
   uint32_t prefix = 0u, mask = 0u, need = (uint32_t)n;
@@ -292,10 +311,12 @@ __global__ void __launch_bounds__(kCopy, 4) paged_evict_copy_kernel(const EvP p)
   const int n = (int)min((int64_t)paged_len(p.c, b), p.budget);
   const int r0 = (int)(blockIdx.x * (kCopy / 32) + threadIdx.x / 32) * p.rows, r = r0 + lane;
   const int end = min(n, r0 + p.rows);
-  int64_t kd = 0, vd = 0, wd = -1;
+  int64_t kd = 0, vd = 0, wd = -1, pd = -1;
+  uint32_t to = 0;
   if (r < end) {
-    const uint32_t to = (uint32_t)r / p.c.page, ds = (uint32_t)r - to * p.c.page;
-    const int64_t pd = (uint32_t)r < p.cap_out ? paged_page(p.c, p.table_out, p.tos, b, to) : -1;
+    to = (uint32_t)r / p.c.page;
+    const uint32_t ds = (uint32_t)r - to * p.c.page;
+    pd = (uint32_t)r < p.cap_out ? paged_page(p.c, p.table_out, p.tos, b, to) : -1;
     if (pd >= 0) {
       kd = pd * p.c.ksp + h * p.c.ksh + ds * p.c.ksn;
       vd = pd * p.c.vsp + h * p.c.vsh + ds * p.c.vsn;
@@ -306,11 +327,20 @@ __global__ void __launch_bounds__(kCopy, 4) paged_evict_copy_kernel(const EvP p)
   if (r0 >= n) return;
   int64_t ks = -1, vs = 0;
   if (r < end) {
+    // the row's slot and the places at its new page, then what they name: two chains of loads side by side
+    const int2 none = make_int2(-1, -1);
+    const int2 old = pd >= 0 ? p.from[pd] : none, own = pd >= 0 ? p.to[pd] : none;
     const uint32_t j = (uint32_t)p.kept[((int64_t)b * p.c.Hkv + h) * p.budget + r];
     const uint32_t t = j / p.c.page, slot = j - t * p.c.page;
+    const bool named = old.x >= 0 && old.x < p.c.B && (uint32_t)old.y < p.c.width;
+    const int len = named ? paged_len(p.c, old.x) : 0;
+    const int32_t entry = named ? __ldg(p.c.table + old.x * p.c.ts + old.y) : -1;
     const int64_t pg = paged_page(p.c, p.c.table, p.c.ts, b, t);
+    const bool used = entry == pd && (uint32_t)old.y < entries_of(p.c, len);
     if (pg < 0 || wd < 0) {
       atomicCAS(p.err, 0, kErrPageEvict);
+    } else if (used || !is_place(own, b, to)) {
+      atomicCAS(p.err, 0, kErrPageTwice);
     } else {
       ks = pg * p.c.ksp + h * p.c.ksh + slot * p.c.ksn;
       vs = pg * p.c.vsp + h * p.c.vsh + slot * p.c.vsn;
@@ -351,6 +381,8 @@ int cluster_size(const sta_paged_cache* c) {
   return cl;
 }
 
+size_t places_bytes(const sta_paged_cache* c) { return (2 * (size_t)c->n_pages * sizeof(int2) + 255) & ~size_t(255); }
+
 bool keys_in_smem(const sta_paged_cache* c) {
   const int64_t cap = c->table_width * c->page_size;
   return (cap + cluster_size(c) - 1) / cluster_size(c) + 3 <= kSliceSmem;
@@ -370,7 +402,7 @@ cudaError_t launch_select(const EvP& p, int cl, cudaStream_t st) {
 size_t paged_evict_workspace_bytes(const sta_paged_cache* c, const sta_paged_evict_args* a) {
   if (check(c, a) != STA_OK) return 0;
   const size_t keys = (size_t)(c->batch * c->n_kv_heads) * ((c->table_width * c->page_size + 3) & ~(int64_t)3) * 4;
-  return (keys_in_smem(c) ? 0 : keys) + 256;
+  return places_bytes(c) + (keys_in_smem(c) ? 0 : keys) + 256;
 }
 
 int paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* ws, size_t ws_len,
@@ -390,8 +422,10 @@ int paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, void* w
   p.kept = a->kept;
   p.lens_out = a->lens_out;
   uint8_t* w = static_cast<uint8_t*>(ws);
-  p.keys = keys_in_smem(c) ? nullptr
-                           : reinterpret_cast<uint32_t*>(w + (256 - reinterpret_cast<uintptr_t>(w) % 256) % 256);
+  w += (256 - reinterpret_cast<uintptr_t>(w) % 256) % 256;
+  p.from = reinterpret_cast<int2*>(w);
+  p.to = p.from + c->n_pages;
+  p.keys = keys_in_smem(c) ? nullptr : reinterpret_cast<uint32_t*>(w + places_bytes(c));
   p.quads = p.c.page % 4 == 0 && (reinterpret_cast<uintptr_t>(p.c.w) & 15) == 0 && p.c.wsp % 4 == 0 && p.c.wsh % 4 == 0;
   p.err = page_error_word();
   if (!p.err) return fail(STA_ERR_CUDA, "sta_paged_evict: no device");

@@ -239,8 +239,10 @@ def evict(cache: PagedCache, budget: int, table_out, *, n_global=32, n_local=32)
     """Cut every sequence to at most ``budget`` keys per kv head: the first ``n_global``, the last
     ``n_local``, and of the others those with the largest ``weights`` (ties: lowest slot).  The
     kept rows of k, v and weights are copied, in order, into the pages of ``table_out`` (batch,
-    >= ceil(min(budget, slots) / page_size)) int32, all different, which must not hold rows of the
-    cache; the old pages stay as they are (they may be shared) until the caller frees them.
+    >= ceil(min(budget, slots) / page_size)) int32; the old pages stay as they are (they may be
+    shared) until the caller frees them.  The new pages that are filled must all be different and
+    must not be in use by the cache: of a page that two entries name one entry's rows are written,
+    of a page in use none, the other rows are dropped, and ``core.device_error()`` is 204.
 
     Returns (the cache over the new pages, kept (batch, Hkv, budget) int32: the original slots in
     order, -1 beyond a sequence's new length)."""
@@ -258,7 +260,6 @@ def evict(cache: PagedCache, budget: int, table_out, *, n_global=32, n_local=32)
     lib = L.lib()
     n = _size(cache, (budget, n_global, n_local, b.table_out_width), lib.sta_paged_evict_workspace_bytes,
               "sta_paged_evict", ref)
-    # 256 bytes: the selection fits shared memory, and no scratch is touched
-    ws = kept if n == 256 else torch.empty(n, dtype=torch.uint8, device=dev)
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
     _run(cache, lib.sta_paged_evict, "sta_paged_evict", ref, ws.data_ptr(), n)
     return cache._moved(table_out, lens), kept

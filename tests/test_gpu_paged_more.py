@@ -132,3 +132,63 @@ def test_weights_of_a_page_that_stands_in_the_table_twice(dtype, D, page):
         p = probs[0].reshape(hk, H // hk, n).sum(1)
         first, again = (base[pg].double() + p[:, t * page:(t + 1) * page] for t in (1, 3))
         assert min((got[pg] - x).abs().max() for x in (first, again)) < tol
+
+
+@pytest.mark.parametrize("dtype,page,lens,budget", [
+    (torch.bfloat16, 16, [300, 200, 40, 33], 48),
+    (torch.float32, 5, [300, 90, 48, 7], 48),
+    (torch.bfloat16, 64, [20000, 9000, 100, 48], 1000),   # clusters, several entries per thread and none
+    (torch.float32, 1, [50, 3000, 48, 9], 48),
+])
+@pytest.mark.parametrize("kind", ["in use", "in use by a sequence that is kept whole", "twice", "twice in a sequence"])
+def test_evict_into_pages_that_are_not_free(dtype, page, lens, budget, kind):
+    """Rows of the cache are never overwritten; of a new page named twice one entry's rows are
+    written; the other new pages are as ever, and the call is reported."""
+    hk, D = 2, 64
+    new = [min(n, budget) for n in lens]
+    need = [-(-n // page) for n in new]
+    c = ref.make(lens, hk=hk, D=D, page=page, dtype=dtype, seed=209, spare=sum(need) + 2)
+    table_out = torch.full((4, max(need)), -1, dtype=torch.int32)
+    at = 0
+    for b, m in enumerate(need):
+        table_out[b, :m] = c["free"][at:at + m]
+        at += m
+    free = int(c["free"][at])
+    want_kept = ref.evict(c, budget, 2, 2)
+    d, cache = on_gpu(c)
+    before = {x: d[x].clone() for x in ("k", "v", "weights")}
+    entries = {"in use": [(0, 0)], "in use by a sequence that is kept whole": [(1, 0)], "twice": [(0, 0), (1, 0)],
+               "twice in a sequence": [(0, 0), (0, need[0] - 1)]}[kind]
+    odd = free if kind.startswith("twice") else int(c["table"][0 if kind == "in use" else 3, 0])
+    used = {int(x) for b, n in enumerate(lens) for x in c["table"][b, :-(-n // page)]}
+    assert (odd in used) != kind.startswith("twice")
+    for b, t in entries:
+        table_out[b, t] = odd
+    c["table"][3, need[3]:] = table_out[2, 0]  # not in use
+    d["table"].copy_(c["table"])
+    for _ in range(3):
+        for x in before:
+            d[x].copy_(before[x])
+        after, kept = paged.evict(cache, budget, table_out.cuda(), n_global=2, n_local=2)
+        assert core.device_error() == 204 and core.device_error() == 0
+        assert torch.equal(kept.cpu(), want_kept) and after.lens.tolist() == new
+
+        def rows(b, t, x):  # what entry t of sequence b brings: (heads, rows, ...)
+            r = want_kept[b, :, t * page:min(new[b], (t + 1) * page)].long()
+            return torch.stack([c[x][c["table"][b].long()[r[h] // page], h, r[h] % page] for h in range(hk)])
+
+        for x in before:
+            got = d[x].cpu()
+            want = before[x].cpu()
+            for b in range(4):
+                for t in range(need[b]):
+                    pg = int(table_out[b, t])
+                    y = rows(b, t, x)
+                    if pg != odd:
+                        want[pg, :, :y.shape[1]] = y
+            if odd not in used:  # one entry's rows
+                ys = [rows(b, t, x) for b, t in entries]
+                left = [torch.equal(got[odd, :, :y.shape[1]], y) for y in ys]
+                assert any(left)
+                got[odd] = want[odd]
+            assert torch.equal(got, want), x
