@@ -192,3 +192,43 @@ def test_evict_into_pages_that_are_not_free(dtype, page, lens, budget, kind):
                 assert any(left)
                 got[odd] = want[odd]
             assert torch.equal(got, want), x
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("page,wide,first", [(16, 17, 0), (8, 9, 0), (64, 64, 1), (4, 6, 2)])
+def test_weights_that_cannot_be_read_four_at_a_time(dtype, page, wide, first):
+    """Pages of a multiple of four whose weights have other strides, or begin between boundaries."""
+    lens, D, hk, H = [300, 17, 0, 65], 64, 2, 4
+    c = ref.make(lens, hk=hk, D=D, page=page, dtype=dtype, seed=211, spare=40)
+    n_pages = c["k"].shape[0]
+    d, _ = on_gpu(c)
+    flat = torch.full((n_pages * hk * wide + 4,), -3.0, device="cuda")
+    w, w2 = (flat.clone().as_strided((n_pages, hk, page), (hk * wide, wide, 1), first) for _ in range(2))
+    w.copy_(d["weights"])
+    cache = paged.PagedCache(d["k"], d["v"], d["table"], d["lens"], weights=w)
+    q = queries(4, H, D, dtype, 212)
+    geo = Geometry(inv_freq(D).cuda())
+    out = paged.decode(q.cuda(), cache, geo, weights_out=w2)
+    assert core.device_error() == 0
+    probs, size = check_decode(q, c, out, inv_freq=inv_freq(D))
+    want = ref.added_weights(c, probs, c["weights"])
+    live = torch.zeros(w.shape, dtype=torch.bool)
+    for b, n in enumerate(lens):
+        for j in range(n):
+            live[c["table"][b, j // page], :, j % page] = True
+    tol = 2.0 ** -24 * want + 1.01 * relative_p(dtype, size, D, 300).max() * (want - c["weights"].double())
+    assert ((w2.cpu().double() - want).abs() <= tol)[live].all()
+    assert (w2.cpu()[~live] == -3).all()
+    # and the selection reads them
+    need = -(-32 // page)
+    table_out = c["free"][:4 * need].reshape(4, need) if 4 * need <= len(c["free"]) else None
+    assert table_out is not None
+    after, kept = paged.evict(cache, 32, table_out.cuda(), n_global=2, n_local=2)
+    assert core.device_error() == 0
+    assert torch.equal(kept.cpu(), ref.evict(c, 32, 2, 2))
+    held = torch.full(flat.shape, True)
+    for pg in range(n_pages):
+        for h in range(hk):
+            held[first + (pg * hk + h) * wide:first + (pg * hk + h) * wide + page] = False
+    base = w._base if w._base is not None else w
+    assert (base.flatten().cpu()[held] == -3).all()  # nothing between the rows is written
