@@ -50,7 +50,7 @@ extern "C" {
 const char* sta_last_error(void);
 /* ABI version: 5 (2: query slabs, PQ-Stream pass 2 on Kernel A keep bits, decode; 3: select wait
  * limit; 4: screened select scoring, sta_select_args.screen_ws; 5: vote histograms; the paged
- * cache, sta_paged_*, came as new entry points alone) */
+ * cache, sta_paged_*, and sta_wait_error came as new entry points alone) */
 int sta_version(void);
 /* Number of elements of one head of a compact selection array. */
 int64_t sta_tri_head_stride(int64_t n, int32_t tile);
@@ -574,8 +574,11 @@ typedef struct sta_paged_cache {
   int64_t table_width;     /* table_width * page_size below 2^31 - 64 */
 } sta_paged_cache;
 
-/* Write rows i < counts[b] of k_new / v_new (batch, n_kv_heads, n, d) to the slots lens[b] + i
- * (counts NULL: all n), zero their weights (when the cache has them) and store the new lengths
+/* (A page that is written belongs to one sequence alone: a slot that two sequences share gets parts
+ * of both rows.  The new rows may lie in the pool, but not where the call writes.)
+ * Write rows i < counts[b] of k_new / v_new (batch, n_kv_heads, n, d) to the slots lens[b] + i
+ * (counts NULL: all n), zero their weights (when the cache has them; decode adds to them, so an
+ * eviction before the first decode ranks a prompt's keys by slot alone) and store the new lengths
  * lens[b] + counts[b] in lens_out, which may be the cache's own lens, or counts.  Rows past the
  * table's last slot are dropped (device error word). */
 typedef struct sta_paged_append_args {
@@ -597,7 +600,14 @@ int sta_paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, v
  * in common with it) slot j of kv head h gets weights[j] + the sum over h's q heads of the
  * attention weight of j; other slots are left as they were.  No page may stand in the table twice
  * then (among the entries in use): of its places one adds its weights, which one is not defined,
- * and the device error word is set to 204. */
+ * and the device error word is set to 204.
+ * bf16 caches: the scores carry some 16 bits (rotated keys and queries enter the products as pairs
+ * of bf16 values), so an added weight is off by up to 6 * 2^-16 |q| |k| sm_scale rope_scale^2
+ * relative to itself; f32 caches keep fp32 throughout.  The same call gives the same bits; a
+ * sequence's last bits may depend on the lengths of the others in the batch.
+ * Scratch depends on the shapes alone; with weights_out it holds 4 bytes for every slot that the
+ * table can name and every q head (batch * n_heads * table_width * page_size, slots rounded up to
+ * 64), so pass a table no wider than the longest sequence needs. */
 typedef struct sta_paged_decode_args {
   const void* q; int64_t q_stride_b; int64_t q_stride_h;   /* (batch, n_heads, d) */
   void* out;               /* (batch, n_heads, d) contiguous, dtype, 16-byte aligned */

@@ -14,9 +14,10 @@
 // Attention positions fit the same scheme: a tile lies in one chunk, whose relation to the
 // query's chunk sets p_i.
 //
-// Each key and value row is read from HBM once: the read of the cache bounds the bf16 kernel.  The
-// f32 kernel here is bound by its fp32 arithmetic and shared memory reads: 65536 keys of 8 kv heads,
-// d = 128, take 110 us with one q head each (537 MB, 4.9 TB/s), 132 us with four.
+// Each key and value row is read from HBM once.  The bf16 kernel comes to 5 TB/s and is bound by the
+// instructions it issues per key and, for short sequences, by its fixed part (there).  The f32 kernel
+// here is bound by its shared memory reads and a barrier per tile: 65536 keys of 8 kv heads, d = 128,
+// take 110 us with one q head each (537 MB, 4.9 TB/s), 132 us with four, 166 us with eight.
 #include <float.h>
 #include <stdlib.h>
 
@@ -466,9 +467,9 @@ __global__ void __launch_bounds__(NW * 32) paged_join_kernel(const PDecP p) {
 // weights_out[j] = weights[j] + sum_g exp2(s_gj - M_g) / L_g, 1024 keys of a (sequence, kv head)
 // per block.  QUADS: a thread's four neighbouring keys share a page and 16-byte accesses (page size
 // and strides multiples of four); otherwise each key is looked up.  Bound by the scores that it
-// reads, which the kernel before it left in L2: 6.5 us for 32 ragged sequences up to 8192 keys (8.4
-// key by key).  A page that stands in the table twice would be read and written by several blocks
-// at once: one of its entries updates it, the others are dropped and reported.
+// reads, which the kernel before it left in L2: 7.4 us for 32 ragged sequences up to 8192 keys (key by
+// key two more).  A page that stands in the table twice would be read and written by several blocks
+// at once: one of its entries updates it, the others are dropped and reported (0.7 us).
 template <bool QUADS>
 __global__ void __launch_bounds__(kUpd) paged_weights_kernel(const PDecP p) {
   const int64_t chunks = (p.c.cap + kUpd * 4 - 1) / (kUpd * 4), seg = div_fast(blockIdx.x, chunks);

@@ -7,8 +7,10 @@
 //   O^T (d x heads)      += V^T . P^T             A = V^T, B = P transposed in registers (movmatrix)
 // Rotated keys, queries and probabilities are fp32 values carried as hi + lo bf16 pieces (four
 // products for S, two for P.V: V is exact), which leaves errors of 2^-15 (keys, whose hi piece is
-// cut instead of rounded) and 2^-16, far below the output's own rounding; running max, sums and
-// accumulators are fp32.
+// cut instead of rounded) and 2^-16; running max, sums and accumulators are fp32.  For the output
+// that is far below its own rounding to bf16 (2^-8).  The fp32 weights show it: a weight comes from a
+// score that is off by up to 3 * 2^-16 |q| |k| scale (4096 keys, d = 128, scores over a range of 8:
+// 4e-6 in norm where the f32 kernel is at 1.6e-7; over 25: 1.3e-5 and 5.4e-7).
 //
 // Every warp walks a share of its own and needs no barrier: its rows come by cp.async (16-byte
 // chunks, swizzled by row) into a ring of its own, two units of K and one of V, so that some 7 KB
@@ -17,10 +19,11 @@
 // the queries of a tile in registers as B fragments.
 //
 // Measured with 4 q heads per kv head, d = 128, the join included: 131072 keys of 8 kv heads 98 us
-// (537 MB of cache, 5.5 TB/s; a call by itself 94, in a row the card is at its power limit and the SM
-// clock falls from 1965 to 1690 MHz), 32768 keys 35 us.  The read itself runs at 7 TB/s; some 16 us
-// go to the start (lengths, page table, first rows: a chain of loads), uneven ends and the join.
-// An SM issues in 53 % of its cycles, the tensor pipe is active in 25 %.
+// (537 MB of cache, 5.5 TB/s; 92 in short bursts, in a row the card is at its power limit and the SM
+// clock falls from 1965 to 1690 MHz), 65536 keys 54, 32768 keys 35, 8192 keys 19 us.  Each further
+// byte comes at 7 TB/s (6.0 beyond 65536 keys in a row); 13 to 17 us are fixed: the start (lengths,
+// page table, first rows: a chain of loads), uneven ends and the join.  An SM issues in 53 % of its
+// cycles and the tensor pipe is active in 25 %: what the loop waits for is its own arithmetic.
 #include "mma_frag.cuh"
 #include "paged_decode.cuh"
 

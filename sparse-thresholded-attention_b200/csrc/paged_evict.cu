@@ -8,7 +8,8 @@
 // shared memory; the key of the last kept slot is found by radix selection (11 + 11 + 10 bits):
 // every CTA counts its slice, reads all CTAs' counts (distributed shared memory) and finds the
 // digit, one cluster barrier per digit; then each CTA writes its kept slots in order.  It reads 4
-// bytes per slot and is bound by latency: 12 us for 128 heads of up to 8192 slots (a CTA each),
+// bytes per slot (and leaves the pages' places) and is bound by latency: 12 us for 128 heads of up to
+// 8192 slots (a CTA each),
 // 20 us for 32 heads of 65536 (clusters of four: 6 us until the keys are there, 2.4 us per digit,
 // 4 us for the order).  Weights are read four at a time where pages and strides allow it (one at a
 // time: 13.5 us for the 128 heads), and the keys lie in shared memory as long as a slice fits (in
@@ -53,7 +54,7 @@ struct EvP {
   uint32_t cap_out;
   int32_t* kept;
   int32_t* lens_out;
-  int rows;           // rows of a warp in the copy: 8, 16 or 32
+  int rows;           // rows of a warp in the copy: 8 or 16
   int quads;          // weights of four neighbouring slots may be loaded at once
   uint32_t* keys;     // (B, Hkv, cap rounded up to 4) where a slice exceeds shared memory, else null
   int2* from;         // (n_pages,) places in the table, and in the new one
