@@ -232,3 +232,47 @@ def test_weights_that_cannot_be_read_four_at_a_time(dtype, page, wide, first):
             held[first + (pg * hk + h) * wide:first + (pg * hk + h) * wide + page] = False
     base = w._base if w._base is not None else w
     assert (base.flatten().cpu()[held] == -3).all()  # nothing between the rows is written
+
+
+@pytest.mark.parametrize("dtype,page,prefix", [(torch.bfloat16, 16, 6), (torch.float32, 5, 20)])
+def test_a_shared_prefix_until_every_sequence_has_pages_of_its_own(dtype, page, prefix):
+    """Sequences that share their first pages are decoded without weights, cut into fresh pages (old
+    pages may be shared), and go on with weights: a narrow slice of a wide table serves them."""
+    D, hk, H, n = 64, 2, 4, prefix * page
+    lens = [n + 30, n + 3, n + 57]
+    c = ref.make(lens, hk=hk, D=D, page=page, dtype=dtype, seed=213, spare=120, width=100)
+    for b in (1, 2):
+        c["table"][b, :prefix] = c["table"][0, :prefix]
+    d, _ = on_gpu(c)
+    geo = Geometry(inv_freq(D).cuda())
+    whole = paged.PagedCache(d["k"], d["v"], d["table"], d["lens"], weights=d["weights"])
+    cache = whole.with_pages(d["table"][:, :-(-max(lens) // page)], d["lens"])
+    q = queries(3, H, D, dtype, 214)
+    out = paged.decode(q.cuda(), cache, geo)
+    assert torch.equal(paged.decode(q.cuda(), whole, geo), out)
+    check_decode(q, c, out, inv_freq=inv_freq(D))
+    budget = n + 10
+    need = -(-(budget + 8) // page)
+    table_out = c["free"][:3 * need].reshape(3, need)
+    after, kept = paged.evict(cache, budget, table_out.cuda(), n_global=4, n_local=4)
+    want = ref.evict(c, budget, 4, 4)
+    assert core.device_error() == 0 and torch.equal(kept.cpu(), want)
+    assert after.lens.tolist() == [budget, n + 3, budget]
+    for b, m in enumerate((budget, n + 3, budget)):
+        r = torch.arange(m)
+        for h in range(hk):
+            src = want[b, h, :m].long()
+            for x in ("k", "v", "weights"):
+                got = d[x].cpu()[table_out[b].long()[r // page], h, r % page]
+                assert torch.equal(got, c[x][c["table"][b].long()[src // page], h, src % page])
+    for step in range(8):  # room for them in the fresh pages
+        new = torch.randn((2, 3, hk, 1, D), generator=torch.Generator().manual_seed(step)).to(dtype).cuda()
+        paged.append(after, new[0], new[1])
+        now = dict(k=d["k"].cpu(), v=d["v"].cpu(), table=table_out, lens=after.lens.cpu())
+        base = d["weights"].cpu()
+        out = paged.decode(q.cuda(), after, geo, weights_out=d["weights"])
+        probs, size = check_decode(q, now, out, inv_freq=inv_freq(D))
+        want = ref.added_weights(now, probs, base)
+        rel = relative_p(dtype, size, D, max(lens)).max()
+        assert ((d["weights"].cpu().double() - want).abs() <= 2.0 ** -24 * want + 1.01 * rel * (want - base.double())).all()
+    assert core.device_error() == 0
