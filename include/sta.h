@@ -574,13 +574,13 @@ typedef struct sta_paged_cache {
   int64_t table_width;     /* table_width * page_size below 2^31 - 64 */
 } sta_paged_cache;
 
-/* (A page that is written belongs to one sequence alone: a slot that two sequences share gets parts
- * of both rows.  The new rows may lie in the pool, but not where the call writes.)
- * Write rows i < counts[b] of k_new / v_new (batch, n_kv_heads, n, d) to the slots lens[b] + i
+/* Write rows i < counts[b] of k_new / v_new (batch, n_kv_heads, n, d) to the slots lens[b] + i
  * (counts NULL: all n), zero their weights (when the cache has them; decode adds to them, so an
  * eviction before the first decode ranks a prompt's keys by slot alone) and store the new lengths
  * lens[b] + counts[b] in lens_out, which may be the cache's own lens, or counts.  Rows past the
- * table's last slot are dropped (device error word). */
+ * table's last slot are dropped (device error word).  A page that is written must belong to one
+ * sequence alone (a slot that two sequences share would get parts of both rows; this is not
+ * checked), and the new rows must not lie where the call writes. */
 typedef struct sta_paged_append_args {
   const void* k; int64_t k_stride_b; int64_t k_stride_h; int64_t k_stride_n;
   const void* v; int64_t v_stride_b; int64_t v_stride_h; int64_t v_stride_n;
@@ -602,12 +602,13 @@ int sta_paged_append(const sta_paged_cache* c, const sta_paged_append_args* a, v
  * then (among the entries in use): of its places one adds its weights, which one is not defined,
  * and the device error word is set to 204.
  * bf16 caches: the scores carry some 16 bits (rotated keys and queries enter the products as pairs
- * of bf16 values), so an added weight is off by up to 6 * 2^-16 |q| |k| sm_scale rope_scale^2
- * relative to itself; f32 caches keep fp32 throughout.  The same call gives the same bits; a
+ * of bf16 values), so an added weight is off by up to about 6 * 2^-16 |q| |k| sm_scale
+ * rope_scale^2 relative to itself; f32 caches keep fp32 throughout.  The same call gives the same bits; a
  * sequence's last bits may depend on the lengths of the others in the batch.
- * Scratch depends on the shapes alone; with weights_out it holds 4 bytes for every slot that the
- * table can name and every q head (batch * n_heads * table_width * page_size, slots rounded up to
- * 64), so pass a table no wider than the longest sequence needs. */
+ * Scratch depends on the shapes alone.  With weights_out it holds 8 bytes per page and 4 bytes for
+ * every slot that the table can name and every q head: batch * n_heads * table_width * page_size
+ * (slots rounded up to 64; above 16 q heads per kv head, f32 8, heads rounded up to a multiple of
+ * that), so pass a table no wider than the longest sequence needs. */
 typedef struct sta_paged_decode_args {
   const void* q; int64_t q_stride_b; int64_t q_stride_h;   /* (batch, n_heads, d) */
   void* out;               /* (batch, n_heads, d) contiguous, dtype, 16-byte aligned */
@@ -632,7 +633,8 @@ int sta_paged_decode(const sta_paged_cache* c, const sta_paged_decode_args* a, v
  * beyond), lens_out the new lengths.  n_global + n_local <= budget.
  * The new pages must all be different and must not stand in the cache's table (among the entries
  * in use): of a page that two entries name one entry's rows are written, of a page in use none,
- * the other rows are dropped, and the device error word is set to 204. */
+ * the other rows are dropped, and the device error word is set to 204.  Scratch: 16 bytes per page,
+ * and 4 per slot of the table and kv head where a table row can name more than 163816 slots. */
 typedef struct sta_paged_evict_args {
   int64_t budget;
   int64_t n_global;
@@ -648,10 +650,9 @@ int sta_paged_evict(const sta_paged_cache* c, const sta_paged_evict_args* a, voi
 
 /* Error words of the current device (0 = none).  101-104 name the bounded wait of the selection
  * kernel that expired, 201-203 come from the paged cache (append, decode, evict): a page number
- * outside the pool, or rows past the table's last slot; 204: a page that a decode or
- * evict call writes stands in a table twice.  Kernels report these only here -- the
- * launching call has already returned STA_OK -- so a C caller that needs to know polls after
- * the stream's work: the call synchronises `stream`, stores the code in *code_out and clears it.
+ * outside the pool, or rows past the table's last slot; 204: a page that a decode or evict call
+ * writes stands in a table twice.  Kernels report these only here -- the launching call has
+ * already returned STA_OK -- so a C caller that needs to know polls after the stream's work: the call synchronises `stream`, stores the code in *code_out and clears it.
  * Waits and pages have a word of their own; where both are set the wait is reported first, the
  * page by the next call.  Returns STA_ERR_TIMEOUT for an expired wait, STA_ERR_ARG for a page. */
 int sta_device_error(void* stream, int32_t* code_out);

@@ -9,9 +9,8 @@
 // every CTA counts its slice, reads all CTAs' counts (distributed shared memory) and finds the
 // digit, one cluster barrier per digit; then each CTA writes its kept slots in order.  It reads 4
 // bytes per slot (and leaves the pages' places) and is bound by latency: 12 us for 128 heads of up to
-// 8192 slots (a CTA each),
-// 20 us for 32 heads of 65536 (clusters of four: 6 us until the keys are there, 2.4 us per digit,
-// 4 us for the order).  Weights are read four at a time where pages and strides allow it (one at a
+// 8192 slots (a CTA each), 20 us for 32 heads of 65536 (clusters of four: 6 us until the keys are
+// there, 2.4 us per digit, 4 us for the order).  Weights are read four at a time where pages and strides allow it (one at a
 // time: 13.5 us for the 128 heads), and the keys lie in shared memory as long as a slice fits (in
 // global memory: 22 us for the 32 heads).
 //
